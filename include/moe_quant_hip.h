@@ -2,7 +2,8 @@
  * moe_quant_hip.h -- C ABI of the MI355X (gfx950) quantized-expert library
  * (libmoe_quant_hip.so).
  *
- * Two groups of entry points:
+ * Three groups of entry points (the third, the token mixers, is described with
+ * its declarations):
  *
  *  1. Drop-ins for the reference's CPU exports, same names, signatures,
  *     argument meaning and status codes.  Pointers are HOST pointers; the
@@ -35,7 +36,8 @@
  *   -4  non-finite output
  *   -5  HIP runtime failure (allocation, copy or launch)
  *   -6  workspace too small
- *   -9  an expert id outside [0, n_experts)
+ *   -9  an expert id outside [0, n_experts); in group 3 a slot, page, length
+ *       or start out of range
  */
 #ifndef MOE_QUANT_HIP_H
 #define MOE_QUANT_HIP_H
@@ -313,6 +315,79 @@ int mqh_workspace_init(void* workspace, int64_t workspace_bytes, void* stream);
 /* Synchronize `stream`, then read and clear the fault flags latched in
  * `workspace`: 0, -4 (non-finite output), -9 (bad expert id) or -5. */
 int mqh_status(void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* 3. Token mixers: paged key/value cache and attention over it              */
+/* ------------------------------------------------------------------------ */
+
+/* What a full-attention layer keeps between calls, and the attention that
+ * reads it (the reference keeps a preallocated FP16 cache per sequence and
+ * attends on the host, src/flash_moe/attention.py:144-306).  Device pointers,
+ * enqueued on `stream`; `flags` is device memory of at least 256 bytes, zeroed
+ * once (mqh_workspace_init(flags, 256, stream)): -9 latches for a slot, page
+ * number, length or start out of range, -4 for a value that is not finite,
+ * read and cleared with mqh_status(flags, stream).
+ *
+ * Element types of these calls: */
+#define MQH_MIX_F32 0
+#define MQH_MIX_F16 1
+#define MQH_MIX_BF16 2
+#define MQH_MIX_Q8 3   /* int8 codes with one FP32 scale per token and head */
+
+/* A cache: kc, vc [pages x kv_heads x page_size x dim] of F16, BF16 or Q8
+ * (16-byte aligned), for Q8 ks, vs [pages x kv_heads x page_size] FP32
+ * (16-byte aligned; else NULL).  page_size is a power of two from 16 to 1024,
+ * dim 64, 128 or 256, kv_heads at most 1024.  A token's slot is
+ * page * page_size + offset. */
+
+/* Store rows k, v [tokens x kv_heads x dim] (F32, F16 or BF16; element
+ * strides *_token and *_head, dim contiguous) at slots[tokens].  Negative
+ * slots are skipped, so are those past the cache (-9); a slot may occur once
+ * in a call.  16-bit caches round once.  Q8: s = max|x| / 127 in FP32, codes
+ * x / s to nearest, ties to even; a row with s < 2^-100 is zeros, a row that is
+ * not finite has s = NaN (-4).  Returns 0, -1, -2 or -5. */
+int mqh_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                 int type, const int64_t* slots, int tokens, void* kc, void* vc, float* ks, float* vs, int cache_type,
+                 int64_t pages, int kv_heads, int page_size, int dim, int32_t* flags, void* stream);
+
+/* Rows at slots[tokens] as values of `type` (F32, F16 or BF16) into k, v
+ * [tokens x kv_heads x dim], contiguous and 16-byte aligned; rows of negative
+ * slots and of slots past the cache (-9) are zeros.  Returns 0, -1, -2 or -5. */
+int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc, const float* ks, const float* vs,
+                int cache_type, int64_t pages, int kv_heads, int page_size, int dim, void* k, void* v, int type,
+                int32_t* flags, void* stream);
+
+/* Bytes of workspace mqh_attend needs (may be 0); single: starts == NULL;
+ * most_keys = table_cols * page_size. */
+int64_t mqh_attend_workspace_bytes(int tokens, int seqs, int single, int heads, int kv_heads, int dim,
+                                   int64_t most_keys);
+
+/* Attention of new tokens, whose rows are already in the cache: q [tokens x
+ * heads x dim] (strides q_token, q_head; F16 or BF16, for 16-bit caches the
+ * cache's own type), heads a multiple of kv_heads (at most 128 times), query
+ * head h reads kv head h / (heads / kv_heads).  table [seqs x table_cols]
+ * (row stride table_stride) int32 pages of each sequence in order,
+ * lengths[seqs] tokens it holds, the new ones included.  starts[seqs + 1]:
+ * sequence b's queries are rows starts[b] .. starts[b + 1] - 1, the last of its
+ * tokens; NULL: one query a sequence (tokens == seqs).  A query sees the keys
+ * up to its own position; a row that sees none is zeros; rows of no sequence
+ * are left as they were.  out [tokens x heads x dim] contiguous, 16-byte
+ * aligned, of q's type.  Products on the matrix cores with FP32 sums, maximum
+ * and probability sums in FP32, probabilities rounded to the cache's 16-bit
+ * type (FP16 for Q8).  The workspace (256-byte aligned) is the call's own until
+ * its kernels have run.  Returns 0, -1, -2, -5 or -6. */
+int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int tokens, const int32_t* starts,
+               int seqs, int heads, const void* kc, const void* vc, const float* ks, const float* vs, int cache_type,
+               int64_t pages, int kv_heads, int page_size, int dim, const int32_t* table, int64_t table_stride,
+               int table_cols, const int32_t* lengths, float scale, void* out, void* workspace,
+               int64_t workspace_bytes, int32_t* flags, void* stream);
+
+/* mqh_kv_write, mqh_kv_read and mqh_attend with their arguments, in order, as
+ * 64-bit words (20, 16 and 27; pointers as integers, the scale as the bits of
+ * a double). */
+int mqh_kv_write_words(const int64_t* args);
+int mqh_kv_read_words(const int64_t* args);
+int mqh_attend_words(const int64_t* args);
 
 #ifdef __cplusplus
 }

@@ -43,6 +43,13 @@ EXPORTS = (
     "mqh_profile_next_decode",
     "mqh_workspace_init",
     "mqh_status",
+    "mqh_kv_write",
+    "mqh_kv_read",
+    "mqh_attend_workspace_bytes",
+    "mqh_attend",
+    "mqh_kv_write_words",
+    "mqh_kv_read_words",
+    "mqh_attend_words",
 )
 
 STATUS_TEXT = {
@@ -53,7 +60,7 @@ STATUS_TEXT = {
     -4: "non-finite output",
     -5: "HIP runtime failure",
     -6: "workspace too small",
-    -9: "expert id out of range",
+    -9: "an id, slot, page or length out of range",
 }
 
 _P = C.c_void_p
@@ -142,6 +149,22 @@ def _declare(lib: C.CDLL) -> C.CDLL:
     lib.mqh_workspace_init.restype = _I
     lib.mqh_status.argtypes = [_P, _P]
     lib.mqh_status.restype = _I
+    cache = [_P, _P, _P, _P, _I, _I64, _I, _I, _I]   # kc, vc, ks, vs, type, pages, kv_heads, page_size, dim
+    lib.mqh_kv_write.argtypes = [_P, _I64, _I64, _P, _I64, _I64, _I, _P, _I, *cache, _P, _P]
+    lib.mqh_kv_write.restype = _I
+    lib.mqh_kv_read.argtypes = [_P, _I, *cache, _P, _P, _I, _P, _P]
+    lib.mqh_kv_read.restype = _I
+    lib.mqh_attend_workspace_bytes.argtypes = [_I, _I, _I, _I, _I, _I, _I64]
+    lib.mqh_attend_workspace_bytes.restype = _I64
+    lib.mqh_attend.argtypes = [
+        _P, _I64, _I64, _I, _I, _P, _I, _I, *cache,   # q, strides, type, tokens, starts, seqs, heads
+        _P, _I64, _I, _P, C.c_float,                  # table, its stride and columns, lengths, scale
+        _P, _P, _I64, _P, _P,                         # out, workspace, bytes, flags, stream
+    ]
+    lib.mqh_attend.restype = _I
+    for f in (lib.mqh_kv_write_words, lib.mqh_kv_read_words, lib.mqh_attend_words):
+        f.argtypes = [C.c_char_p]
+        f.restype = _I
     return lib
 
 

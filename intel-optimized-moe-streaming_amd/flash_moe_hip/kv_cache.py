@@ -1,0 +1,282 @@
+"""Paged key/value cache of an attention layer in HBM, and attention over it.
+
+``PagedCache`` holds one layer's keys and values as pages [pages, kv_heads,
+page_size, head_dim] in FP16, BF16 or as 8-bit codes with one FP32 scale per
+token and head.  ``write`` stores new tokens' rows (quantizing them for an 8-bit
+cache), ``read`` gives rows back as values, ``attend`` is attention of new
+tokens over what the sequences hold: chunks of prompts, drafts, or one token a
+sequence.  (The reference keeps a preallocated FP16 cache per sequence and
+attends on the host, attention.py:144-306.)
+
+Everything is enqueued on the current stream of the cache's device (or on
+``stream``); nothing synchronizes.  ``status()`` synchronizes and reports what
+the kernels latched.  There is no backward: tensors that require grad are
+refused.
+"""
+from __future__ import annotations
+
+import functools
+import struct
+
+from . import _lib
+
+HEAD_DIMS = (64, 128, 256)
+F32, F16, BF16, Q8 = 0, 1, 2, 3   # the library's element types (MQH_MIX_*)
+
+_WRITE_WORDS = struct.Struct("20q")
+_READ_WORDS = struct.Struct("16q")
+_ATTEND_WORDS = struct.Struct("21qd5q")
+
+
+@functools.lru_cache(maxsize=None)
+def _types():
+    import torch
+
+    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+@functools.lru_cache(maxsize=512)
+def _attend_bytes(lib, tokens, seqs, single, heads, kv_heads, dim, most):
+    return int(lib.mqh_attend_workspace_bytes(tokens, seqs, single, heads, kv_heads, dim, most))
+
+
+def check_rows(t, shape, types, device, what):
+    """A tensor of rows as the kernels take it: shape, a type of `types`, on
+    `device`, its last dimension contiguous (other strides are free)."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype not in types:
+        raise ValueError(f"{what} is {t.dtype}, expected one of {[str(d) for d in types]}")
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{what} must be contiguous in its last dimension")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, expected {device}")
+    if t.requires_grad:
+        raise ValueError(f"{what} requires grad; these calls have no backward")
+
+
+def check_index(t, shape, dtype, device, what):
+    """An index tensor: exact shape and type, contiguous, on `device`."""
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, expected {device}")
+
+
+class OnStream:
+    """The device and stream of a call: makes the device current and, where a
+    stream is given, has the call's tensors allocated on it."""
+
+    def __init__(self, device):
+        import torch
+
+        self.device = device
+        self.index = device.index
+        self._torch = torch
+        self._stream_of = _lib.stream_accessor()
+
+    def __call__(self, stream, call):
+        torch = self._torch
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return call(stream.cuda_stream)
+        if torch.cuda.current_device() != self.index:
+            with torch.cuda.device(self.index):
+                return call(self._stream_of(self.index))
+        return call(self._stream_of(self.index))
+
+
+class PagedCache:
+    """One layer's paged cache over tensors the caller keeps: k and v [pages,
+    kv_heads, page_size, head_dim], FP16, BF16 or int8 (then k_scale and v_scale
+    [pages, kv_heads, page_size] FP32), contiguous.  head_dim 64, 128 or 256,
+    page_size a power of two from 16 to 1024.
+
+    A *slot* is page * page_size + offset; a sequence's page table lists its
+    pages in order."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        import torch
+
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v must be [pages, kv_heads, page_size, head_dim] of one type")
+        pages, kv_heads, page_size, dim = k.shape
+        if dim not in HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {dim}")
+        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
+        if pages < 1 or kv_heads < 1 or kv_heads > 1024:
+            raise ValueError("a cache has at least one page and 1 to 1024 kv heads")
+        types = {torch.float16: F16, torch.bfloat16: BF16, torch.int8: Q8}
+        if k.dtype not in types:
+            raise ValueError(f"a cache is FP16, BF16 or int8, got {k.dtype}")
+        held = [k, v]
+        if k.dtype == torch.int8:
+            if k_scale is None or v_scale is None:
+                raise ValueError("an int8 cache needs k_scale and v_scale")
+            for s in (k_scale, v_scale):
+                if s.dtype != torch.float32 or tuple(s.shape) != (pages, kv_heads, page_size):
+                    raise ValueError("scales must be FP32 [pages, kv_heads, page_size]")
+            held += [k_scale, v_scale]
+        elif k_scale is not None or v_scale is not None:
+            raise ValueError("only int8 caches have scales")
+        if any(t.device != k.device or not t.is_contiguous() for t in held):
+            raise ValueError("a cache's tensors must be contiguous and on one device")
+        if k.device.type != "cuda":
+            raise ValueError(f"expected a CUDA device, got {k.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, dim
+        self.device = k.device
+        self.lib = _lib.load()
+        self._run = OnStream(k.device)
+        self._types = _types()
+        self._cache_type = types[k.dtype]
+        self._flags = torch.zeros(64, dtype=torch.int32, device=k.device)
+        scales = (k_scale.data_ptr(), v_scale.data_ptr()) if len(held) == 4 else (0, 0)
+        self._words = (k.data_ptr(), v.data_ptr(), *scales, self._cache_type, pages, kv_heads, page_size, dim)
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dtype=None, device="cuda"):
+        """A cache of zeros; dtype torch.float16 (default), torch.bfloat16 or torch.int8."""
+        import torch
+
+        dtype = torch.float16 if dtype is None else dtype
+        shape = (pages, kv_heads, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        if dtype != torch.int8:
+            return cls(k, v)
+        return cls(k, v, *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+
+    def slots(self, page_table, seq, position):
+        """Slots of positions of sequences: page_table [sequences, columns], seq
+        and position index tensors of one shape."""
+        page = page_table[seq, position // self.page_size].long()
+        return page * self.page_size + position % self.page_size
+
+    def write(self, k, v, slots, *, stream=None):
+        """Store rows k, v [tokens, kv_heads, head_dim] (FP32, FP16 or BF16, any
+        token and head strides) at `slots` [tokens] int64; a negative slot is
+        skipped, one past the cache is skipped and latched (-9).  Each slot may
+        occur once in a call.  16-bit caches round once; an int8 cache stores
+        round(x / s), s = max|x| / 127 of the row.  A value that is not finite (or
+        that an FP16 cache cannot hold) latches -4; in an int8 cache its row then
+        reads back as NaN."""
+        import torch
+
+        n = slots.shape[0] if slots.dim() == 1 else -1
+        check_index(slots, (n,), torch.int64, self.device, "slots")
+        shape = (n, self.kv_heads, self.head_dim)
+        check_rows(k, shape, self._types, self.device, "k")
+        check_rows(v, shape, (k.dtype,), self.device, "v")
+        if n == 0:
+            return
+        kt, kh, _ = k.stride()
+        vt, vh, _ = v.stride()
+
+        def call(handle):
+            return self.lib.mqh_kv_write_words(_WRITE_WORDS.pack(
+                k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, self._types[k.dtype], slots.data_ptr(), n, *self._words,
+                self._flags.data_ptr(), handle))
+
+        _lib.check(self._run(stream, call), "mqh_kv_write")
+
+    def read(self, slots, dtype=None, *, stream=None):
+        """(k, v) [tokens, kv_heads, head_dim] at `slots` [tokens] int64 as `dtype`
+        (the cache's own, FP32 for int8); rows of negative slots are zeros, so are
+        those past the cache, which latch -9."""
+        import torch
+
+        n = slots.shape[0] if slots.dim() == 1 else -1
+        check_index(slots, (n,), torch.int64, self.device, "slots")
+        if dtype is None:
+            dtype = torch.float32 if self._cache_type == Q8 else self.k.dtype
+        if dtype not in self._types:
+            raise ValueError(f"rows are read as FP32, FP16 or BF16, not {dtype}")
+        shape = (n, self.kv_heads, self.head_dim)
+
+        def call(handle):
+            k = torch.empty(shape, dtype=dtype, device=self.device)
+            v = torch.empty(shape, dtype=dtype, device=self.device)
+            rc = 0
+            if n:
+                rc = self.lib.mqh_kv_read_words(_READ_WORDS.pack(
+                    slots.data_ptr(), n, *self._words, k.data_ptr(), v.data_ptr(), self._types[dtype],
+                    self._flags.data_ptr(), handle))
+            _lib.check(rc, "mqh_kv_read")
+            return k, v
+
+        return self._run(stream, call)
+
+    def attend(self, q, page_table, lengths, starts=None, *, scale=None, out=None, stream=None):
+        """Attention of new tokens, whose rows are already written, over the cache.
+
+        q [tokens, heads, head_dim] (heads a multiple of kv_heads, at most 128
+        times; the cache's type, FP16 or BF16 for int8 caches; any token and head
+        strides); page_table [sequences, columns] int32; lengths [sequences] int32:
+        tokens a sequence holds, the new ones included.  starts [sequences + 1]
+        int32: sequence b's queries are rows starts[b] .. starts[b + 1] - 1, the
+        last of its tokens; without it every sequence has one.  Query head h reads
+        kv head h // (heads // kv_heads).  Each query sees the keys up to its own
+        position; a row that sees none (a length below its queries) is zeros; rows
+        of `out` that belong to no sequence are left as they were.  scale > 0
+        (default head_dim ** -0.5).  Returns out [tokens, heads, head_dim] of q's
+        type.  Page numbers, lengths and starts out of range latch -9 (the
+        rows concerned are then undefined), outputs that are not finite -4."""
+        import torch
+
+        if q.dim() != 3 or page_table.dim() != 2:
+            raise ValueError("q must be [tokens, heads, head_dim] and page_table [sequences, columns]")
+        tokens, heads, _ = q.shape
+        seqs, cols = page_table.shape
+        types = (torch.float16, torch.bfloat16) if self._cache_type == Q8 else (self.k.dtype,)
+        check_rows(q, (tokens, heads, self.head_dim), types, self.device, "q")
+        group = heads // self.kv_heads
+        if group * self.kv_heads != heads or not 1 <= group <= 128:
+            raise ValueError(f"heads must be 1 to 128 times the cache's {self.kv_heads}, got {heads}")
+        if page_table.dtype != torch.int32 or page_table.device != self.device or (
+                cols and page_table.stride(1) != 1 and cols != 1) or (seqs > 1 and page_table.stride(0) < cols):
+            raise ValueError(f"page_table must be int32 rows on {self.device}")
+        check_index(lengths, (seqs,), torch.int32, self.device, "lengths")
+        if starts is not None:
+            check_index(starts, (seqs + 1,), torch.int32, self.device, "starts")
+        elif tokens != seqs:
+            raise ValueError("without starts there is one query a sequence")
+        scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        if not 0 < scale < float("inf"):
+            raise ValueError("scale must be positive and finite")
+        if out is not None:
+            check_rows(out, q.shape, (q.dtype,), self.device, "out")
+            if not out.is_contiguous() or out.data_ptr() % 16:
+                raise ValueError("out must be contiguous and 16-byte aligned")
+        most = cols * self.page_size
+        need = 0
+        if tokens and seqs and cols:
+            need = _attend_bytes(self.lib, tokens, seqs, int(starts is None), heads, self.kv_heads, self.head_dim, most)
+            if need < 0:
+                _lib.check(need, "mqh_attend_workspace_bytes")
+        qt, qh, _ = q.stride()
+
+        def call(handle):
+            y = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype, device=self.device) if out is None else out
+            if tokens == 0 or seqs == 0:
+                return y
+            if cols == 0:
+                raise ValueError("page_table has no columns")
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            _lib.check(self.lib.mqh_attend_words(_ATTEND_WORDS.pack(
+                q.data_ptr(), qt, qh, self._types[q.dtype], tokens, starts.data_ptr() if starts is not None else 0,
+                seqs, heads, *self._words, page_table.data_ptr(), page_table.stride(0) if seqs > 1 else cols, cols,
+                lengths.data_ptr(), scale, y.data_ptr(), ws.data_ptr() if need else 0, need, self._flags.data_ptr(),
+                handle)), "mqh_attend")
+            return y
+
+        return self._run(stream, call)
+
+    def status(self, stream=None) -> int:
+        """Synchronizes; 0, -4 (a value that is not finite) or -9 (a slot, page,
+        length or start out of range) since the last call."""
+        import torch
+
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        return int(self.lib.mqh_status(self._flags.data_ptr(), stream.cuda_stream))

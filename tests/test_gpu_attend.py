@@ -1,0 +1,283 @@
+"""Attention over the paged cache on the GPU against a plain form in 64 bits,
+with the bounds of mixer_reference.attend."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import mixer_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.int8, torch.bfloat16),
+         (torch.int8, torch.float16)]
+
+
+def problem(new, lengths, heads, kv_heads, dim, page, cache, qt, seed=0, k_scale=1.0, v_scale=1.0):
+    """Queries, a shuffled paged cache with stale places, its tables, and the values it stands for."""
+    g = torch.Generator().manual_seed(seed)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g)
+
+    counts = [-(-n // page) for n in lengths]
+    pages = sum(counts) + 3
+    order = torch.randperm(pages, generator=g).to(torch.int32)
+    cols = max(max(counts), 1) + 1
+    table, used = torch.full((len(lengths), cols), -7, dtype=torch.int32), 0   # (columns past a sequence's end hold anything)
+    for b, c in enumerate(counts):
+        table[b, :c] = order[used:used + c]
+        used += c
+    k = [randn(n, kv_heads, dim) * k_scale for n in lengths]
+    v = [randn(n, kv_heads, dim) * torch.exp(randn(n, kv_heads, 1)) * v_scale for n in lengths]
+    kc, ks, kv = ref.paged(k, table, page, pages, cache)
+    vc, vs, vv = ref.paged(v, table, page, pages, cache)
+    q = randn(sum(new), heads, dim).to(qt)
+    starts = torch.tensor([0] + new).cumsum(0).to(torch.int32)
+    return dict(q=q, table=table, lengths=torch.tensor(lengths, dtype=torch.int32), starts=starts, k=kv, v=vv,
+                cache=[None if t is None else t.cuda() for t in (kc, vc, ks, vs)], new=new)
+
+
+def cache_of(p):
+    from flash_moe_hip.kv_cache import PagedCache
+
+    return PagedCache(*p["cache"])
+
+
+def call(c, p, single=False, **kw):
+    return c.attend(p["q"].cuda(), p["table"].cuda(), p["lengths"].cuda(),
+                    starts=None if single else p["starts"].cuda(), **kw)
+
+
+def check(got, p, scale, cache):
+    at = 0
+    for b, n in enumerate(p["new"]):
+        want, bound = ref.attend(p["q"][at:at + n], p["k"][b], p["v"][b], scale, cache)
+        err = (got[at:at + n].cpu().double() - want).abs()
+        assert (err <= bound).all(), f"sequence {b}: {float((err / bound).max()):.3g} of the bound"
+        at += n
+
+
+SHAPES = [   # new, lengths, heads, kv_heads, dim, page
+    ([1], [1], 1, 1, 64, 16),
+    ([5], [5], 4, 2, 128, 16),
+    ([3, 0, 17, 1], [3, 0, 40, 65], 8, 2, 64, 32),
+    ([70, 33], [70, 161], 5, 1, 128, 16),
+    ([40], [300], 6, 6, 64, 1024),
+    ([129, 2, 31], [129, 1027, 500], 16, 2, 256, 64),
+    ([9, 9], [777, 64], 128, 1, 64, 64),
+    ([300], [2300], 4, 1, 128, 128),
+]
+
+
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_chunks(shape, cache, qt):
+    print(shape, cache, qt, flush=True)
+    p = problem(*shape, cache, qt, seed=sum(shape[1]))
+    c = cache_of(p)
+    check(call(c, p), p, shape[4] ** -0.5, cache)
+    assert c.status() == 0
+
+
+SINGLE = [   # lengths, heads, kv_heads, dim, page
+    ([1], 1, 1, 64, 16),
+    ([31, 32, 33], 8, 8, 128, 16),
+    ([0, 5, 1000], 16, 2, 256, 64),
+    ([4099], 16, 1, 128, 64),
+    ([2049, 129], 6, 2, 64, 32),
+    ([100, 515], 40, 2, 128, 16),       # 20 heads a kv head
+    ([20000, 3], 8, 4, 64, 128),
+    ([70000], 4, 2, 256, 16),
+]
+
+
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+@pytest.mark.parametrize("shape", SINGLE, ids=str)
+def test_single_tokens(shape, cache, qt):
+    print(shape, cache, qt, flush=True)
+    lengths, heads, kv_heads, dim, page = shape
+    p = problem([1] * len(lengths), lengths, heads, kv_heads, dim, page, cache, qt, seed=sum(lengths))
+    c = cache_of(p)
+    got = call(c, p, single=True)
+    check(got, p, dim ** -0.5, cache)
+    # the same through starts
+    check(call(c, p), p, dim ** -0.5, cache)
+    assert c.status() == 0
+
+
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+def test_queries_before_the_first_key_are_zeros(cache, qt):
+    """More new tokens than cached ones: the first see nothing."""
+    p = problem([6, 200], [4, 0], 4, 2, 64, 16, cache, qt)
+    c = cache_of(p)
+    got = call(c, p).cpu()
+    assert not got[:2].any() and not got[6:].any() and c.status() == 0
+    p["q"], p["new"] = p["q"][2:6], [4]
+    check(got[2:6], p, 64 ** -0.5, cache)
+
+
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+@pytest.mark.parametrize("single", [False, True])
+def test_scales_far_from_one(cache, qt, single):
+    """Sharp and flat softmaxes, large and small values."""
+    n = 1 if single else 37
+    for k_scale, v_scale, scale in ((8.0, 1.0, 0.3), (1.0, 200.0, 0.125), (0.01, 2e-3, 0.05), (1.0, 1.0, 1e-6)):
+        p = problem([n], [700], 4, 2, 128, 32, cache, qt, seed=5, k_scale=k_scale, v_scale=v_scale)
+        c = cache_of(p)
+        check(call(c, p, single=single, scale=scale), p, scale, cache)
+        assert c.status() == 0
+
+
+@pytest.mark.parametrize("single", [False, True])
+def test_long_rows_and_growing_scores(single):
+    """Scores that grow with the position move the reference exponent at every step."""
+    n = 1 if single else 20
+    p = problem([n], [3000], 2, 1, 64, 64, torch.float16, torch.float16, seed=8)
+    ramp = torch.linspace(0.01, 4, 3000).view(-1, 1, 1)
+    k = [torch.sign(p["q"][-1:, :1].float()) * ramp]
+    kc, _, kv = ref.paged(k, p["table"], 64, p["cache"][0].shape[0], torch.float16)
+    p["cache"][0], p["k"] = kc.cuda(), kv
+    c = cache_of(p)
+    check(call(c, p, single=single), p, 64 ** -0.5, torch.float16)
+
+
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+def test_values_of_later_tokens_do_not_matter(cache, qt):
+    """Infinities and NaN in keys and values reach the rows that see them, and no other."""
+    lengths, new, page = [150], [100], 16
+    p = problem(new, lengths, 4, 2, 64, page, cache, qt, seed=3)
+    clean = call(cache_of(p), p).cpu()
+    at = {60: math.nan, 90: math.inf, 120: -math.inf}
+
+    def put(t, s, i, x):
+        page_, off = int(p["table"][0, i // page]), i % page
+        if cache == torch.int8:
+            s[page_, 1, off] = math.nan
+        else:
+            t[page_, 1, off, 11] = x
+
+    for what in (1, 0):   # values, then keys as well
+        for i, x in at.items():
+            put(p["cache"][what], p["cache"][2 + (what == 1)], i, x)
+        c = cache_of(p)
+        got = call(c, p).cpu()
+        assert c.status() == -4
+        first = 60 - 50   # the row of position 60
+        torch.testing.assert_close(got[:first], clean[:first], rtol=0, atol=0)
+        torch.testing.assert_close(got[:, :2], clean[:, :2], rtol=0, atol=0)   # the other kv head
+        assert got[first:, 2:, 11].isnan().all()
+        if what == 1 and cache != torch.int8:
+            others = [d for d in range(64) if d != 11]
+            torch.testing.assert_close(got[:, :, others], clean[:, :, others], rtol=0, atol=0)
+
+
+def test_an_infinite_value_that_is_seen_is_infinite():
+    p = problem([100], [100], 2, 2, 64, 16, torch.bfloat16, torch.bfloat16, seed=3)
+    page_, off = int(p["table"][0, 70 // 16]), 70 % 16
+    p["cache"][1][page_, 0, off, 5] = -math.inf
+    got = call(cache_of(p), p).cpu()
+    assert got[:70].isfinite().all() and (got[70:, 0, 5] == -math.inf).all() and got[70:, 1].isfinite().all()
+
+
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+def test_strided_queries_and_tables_rows_of_no_sequence(cache, qt):
+    new, lengths = [7, 20], [90, 33]
+    p = problem(new, lengths, 4, 2, 128, 16, cache, qt, seed=6)
+    c = cache_of(p)
+    wide = torch.zeros(40, 4 * 128 + 9, dtype=qt)
+    wide[3:30, 5:5 + 512] = p["q"].flatten(1)
+    q = wide.cuda()[:, 5:5 + 512].unflatten(1, (4, 128))
+    starts = (p["starts"] + 3).cuda()
+    table = torch.nn.functional.pad(p["table"], (0, 5)).cuda()[:, :p["table"].shape[1]]
+    out = torch.full((40, 4, 128), 7.0, dtype=qt, device="cuda")
+    got = c.attend(q, table, p["lengths"].cuda(), starts=starts, out=out)
+    assert got is out and (out[:3] == 7).all() and (out[30:] == 7).all()
+    check(out[3:30], p, 128 ** -0.5, cache)
+    # the same with the keys split over workgroups
+    p = problem([5, 2], [9000, 4000], 4, 2, 128, 16, cache, qt, seed=6)
+    c = cache_of(p)
+    q = torch.zeros(12, 4, 128, dtype=qt)
+    q[2:9] = p["q"]
+    out = torch.full((12, 4, 128), 7.0, dtype=qt, device="cuda")
+    c.attend(q.cuda(), p["table"].cuda(), p["lengths"].cuda(), starts=(p["starts"] + 2).cuda(), out=out)
+    assert (out[:2] == 7).all() and (out[9:] == 7).all()
+    check(out[2:9], p, 128 ** -0.5, cache)
+    assert c.status() == 0
+
+
+@pytest.mark.parametrize("single", [False, True])
+def test_bad_pages_lengths_and_starts_are_reported(single):
+    def fresh():
+        return problem([1, 1], [300, 40], 4, 2, 64, 16, torch.float16, torch.float16)
+
+    p = fresh()
+    p["table"][0, 3] = 10 ** 6
+    c = cache_of(p)
+    call(c, p, single=single)
+    assert c.status() == -9
+    p = fresh()
+    p["lengths"][1] = 10 ** 6
+    p["table"].clamp_(min=0)
+    c = cache_of(p)
+    call(c, p, single=single)
+    assert c.status() in (-9, -4)
+    if not single:
+        for starts in ([0, 5, 2], [-3, 1, 2], [0, 1, 9]):
+            p = fresh()
+            p["starts"] = torch.tensor(starts, dtype=torch.int32)
+            c = cache_of(p)
+            call(c, p)
+            assert c.status() == -9, starts
+
+
+def test_many_sequences():
+    """More sequences than a wavefront has lanes, some without queries, some without keys."""
+    new = [i % 4 for i in range(150)]
+    lengths = [n + (i * 37) % 200 if i % 7 else n for i, n in enumerate(new)]
+    p = problem(new, lengths, 2, 1, 64, 16, torch.bfloat16, torch.bfloat16, seed=2)
+    c = cache_of(p)
+    check(call(c, p), p, 64 ** -0.5, torch.bfloat16)
+    p = problem([1] * 150, [n + 1 for n in lengths], 2, 1, 64, 16, torch.bfloat16, torch.bfloat16, seed=2)
+    c = cache_of(p)
+    check(call(c, p, single=True), p, 64 ** -0.5, torch.bfloat16)
+    assert c.status() == 0
+
+
+def test_no_queries():
+    p = problem([0], [30], 4, 2, 64, 16, torch.float16, torch.float16)
+    c = cache_of(p)
+    assert call(c, p).shape == (0, 4, 64)
+    assert c.status() == 0
+
+
+@pytest.mark.parametrize("single", [False, True])
+def test_captured_replayed_and_other_streams(single):
+    """Two captured calls on one cache, replayed in turn with eager work between, and a side stream."""
+    n = 1 if single else 6
+    p = problem([n, n], [5000, 700], 8, 2, 128, 64, torch.int8, torch.bfloat16, seed=4)
+    c = cache_of(p)
+    q, table, lengths, starts = (t.cuda() for t in (p["q"], p["table"], p["lengths"], p["starts"]))
+    kw = dict(starts=None if single else starts)
+    other = torch.randn_like(q.float()).to(q.dtype)
+    want, want2 = c.attend(q, table, lengths, **kw), c.attend(other, table, lengths, **kw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = c.attend(q, table, lengths, stream=side, **kw)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graphs = []
+    for x in (q, other):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = c.attend(x, table, lengths, **kw)
+        graphs.append((graph, y))
+    for _ in range(4):
+        for (graph, y), w in zip(graphs, (want, want2)):
+            y.zero_()
+            graph.replay()
+            assert torch.equal(c.attend(other, table, lengths, **kw), want2)
+            assert torch.equal(y, w)
+    assert c.status() == 0

@@ -1,0 +1,103 @@
+"""What the token mixers' calls refuse (CPU only: every check precedes any HIP call)."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from flash_moe_hip import _lib
+
+    return _lib.load()
+
+
+P = C.c_void_p(4096)
+
+
+def test_cache_constructor():
+    from flash_moe_hip.kv_cache import PagedCache
+
+    def make(shape=(2, 2, 16, 64), dtype=torch.float16, **kw):
+        return PagedCache(torch.zeros(shape, dtype=dtype), torch.zeros(shape, dtype=dtype), **kw)
+
+    with pytest.raises(ValueError, match="CUDA device"):
+        make()
+    with pytest.raises(ValueError, match="head_dim"):
+        make((2, 2, 16, 96))
+    with pytest.raises(ValueError, match="page_size"):
+        make((2, 2, 24, 64))
+    with pytest.raises(ValueError, match="page_size"):
+        make((2, 2, 8, 64))
+    with pytest.raises(ValueError, match="int8"):
+        make(dtype=torch.float32)
+    with pytest.raises(ValueError, match="k_scale"):
+        make(dtype=torch.int8)
+    with pytest.raises(ValueError, match="scales must be"):
+        make(dtype=torch.int8, k_scale=torch.zeros(2, 2, 8), v_scale=torch.zeros(2, 2, 16))
+    with pytest.raises(ValueError, match="only int8"):
+        make(k_scale=torch.zeros(2, 2, 16), v_scale=torch.zeros(2, 2, 16))
+    with pytest.raises(ValueError, match="one type"):
+        PagedCache(torch.zeros(2, 2, 16, 64, dtype=torch.float16), torch.zeros(2, 2, 16, 64, dtype=torch.bfloat16))
+
+
+def kv_write(lib, **kw):
+    a = dict(k=P, kt=256, kh=64, v=P, vt=256, vh=64, type=1, slots=P, tokens=4, kc=P, vc=P, ks=None, vs=None, ct=1,
+             pages=4, heads=2, page=16, dim=64, flags=P, stream=None)
+    a.update(kw)
+    return lib.mqh_kv_write(*a.values())
+
+
+def test_write_codes(lib):
+    for bad in (dict(k=None), dict(v=None), dict(slots=None), dict(kc=None), dict(vc=None), dict(flags=None),
+                dict(tokens=0), dict(pages=0), dict(heads=0), dict(heads=1025), dict(page=24), dict(page=8),
+                dict(page=2048), dict(kc=C.c_void_p(4098)), dict(ct=3), dict(ct=3, ks=P, vs=C.c_void_p(4100)),
+                dict(k=C.c_void_p(4097)), dict(type=0, v=C.c_void_p(4098)), dict(pages=2 ** 31)):
+        assert kv_write(lib, **bad) == -1, bad
+    for bad in (dict(type=3), dict(type=7), dict(ct=0), dict(dim=96), dict(dim=32)):
+        assert kv_write(lib, **bad) == -2, bad
+    assert lib.mqh_kv_write_words(None) == -1 and lib.mqh_kv_read_words(None) == -1
+    assert lib.mqh_attend_words(None) == -1
+
+
+def test_read_codes(lib):
+    def read(**kw):
+        a = dict(slots=P, tokens=4, kc=P, vc=P, ks=None, vs=None, ct=1, pages=4, heads=2, page=16, dim=64, k=P, v=P,
+                 type=1, flags=P, stream=None)
+        a.update(kw)
+        return lib.mqh_kv_read(*a.values())
+
+    for bad in (dict(slots=None), dict(k=None), dict(v=C.c_void_p(4104)), dict(tokens=-1), dict(flags=None)):
+        assert read(**bad) == -1, bad
+    assert read(type=3) == -2 and read(ct=4) == -2 and read(dim=100) == -2
+
+
+def attend(lib, **kw):
+    a = dict(q=P, qt=512, qh=64, q_type=1, tokens=4, starts=P, seqs=2, heads=8, kc=P, vc=P, ks=None, vs=None, ct=1,
+             pages=4, kv=2, page=16, dim=64, table=P, stride=4, cols=4, lengths=P, scale=0.125, out=P, ws=P,
+             bytes=1 << 30, flags=P, stream=None)
+    a.update(kw)
+    return lib.mqh_attend(*a.values())
+
+
+def test_attend_codes(lib):
+    for bad in (dict(q=None), dict(table=None), dict(lengths=None), dict(out=None), dict(flags=None), dict(tokens=0),
+                dict(seqs=0), dict(heads=7), dict(heads=0), dict(heads=258), dict(starts=None), dict(scale=0.0),
+                dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(out=C.c_void_p(4098)),
+                dict(q=C.c_void_p(4097)), dict(cols=0), dict(stride=3), dict(kc=None), dict(page=17)):
+        assert attend(lib, **bad) == -1, bad
+    for bad in (dict(q_type=2), dict(q_type=0), dict(ct=2), dict(dim=80), dict(ct=0)):
+        assert attend(lib, **bad) == -2, bad
+    # a split call needs its workspace
+    long = dict(cols=4096, stride=4096)
+    need = lib.mqh_attend_workspace_bytes(4, 2, 0, 8, 2, 64, 4096 * 16)
+    assert need > 0 and need % 256 == 0
+    assert attend(lib, bytes=need - 1, **long) == -6
+    assert attend(lib, ws=None, **long) == -1
+    assert attend(lib, ws=C.c_void_p(4096 + 16), **long) == -1
+    assert lib.mqh_attend_workspace_bytes(4, 2, 1, 8, 2, 64, 64) == -1
+    assert lib.mqh_attend_workspace_bytes(4, 2, 0, 8, 3, 64, 64) == -1
+    assert lib.mqh_attend_workspace_bytes(4096, 1, 0, 32, 8, 128, 4096) >= 0
