@@ -317,7 +317,7 @@ int mqh_workspace_init(void* workspace, int64_t workspace_bytes, void* stream);
 int mqh_status(void* workspace, void* stream);
 
 /* ------------------------------------------------------------------------ */
-/* 3. Token mixers: paged key/value cache and attention over it              */
+/* 3. Token mixers: paged key/value cache, attention, linear attention        */
 /* ------------------------------------------------------------------------ */
 
 /* What a full-attention layer keeps between calls, and the attention that
@@ -382,12 +382,49 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
                int table_cols, const int32_t* lengths, float scale, void* out, void* workspace,
                int64_t workspace_bytes, int32_t* flags, void* stream);
 
-/* mqh_kv_write, mqh_kv_read and mqh_attend with their arguments, in order, as
- * 64-bit words (20, 16 and 27; pointers as integers, the scale as the bits of
- * a double). */
+/* One token of each of `seqs` sequences through linear attention with a decay
+ * per head (the gated recurrence of mqh_delta_heads for many sequences, other
+ * types and shared key heads, and the same without the delta rule):
+ *   S <- e^gate S;  u = beta (v - S k), or v where beta is NULL;
+ *   S <- S + u k^T;  out = S q
+ * state [seqs x heads x value_dim x key_dim] FP32 (16-byte aligned), updated in
+ * place; q, k [seqs x key_heads x key_dim] and v [seqs x heads x value_dim] of
+ * `type` (F32, F16 or BF16; element strides *_token and *_head, the last
+ * dimension contiguous); value head h uses key head h / (heads / key_heads);
+ * beta, gate [seqs x heads] FP32 with row strides; out [seqs x heads x
+ * value_dim] contiguous.  key_dim a multiple of 4 up to 256, value_dim one up
+ * to 1024.  Sums are FP32; their order is this library's own, not that of
+ * moe_delta_heads.  An output that is not finite latches -4 in `flags`.
+ * Returns 0, -1, -2 or -5. */
+int mqh_linear_step(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                    const void* v, int64_t v_token, int64_t v_head, int type, const float* beta, int64_t beta_token,
+                    const float* gate, int64_t gate_token, float* state, void* out, int seqs, int heads, int key_heads,
+                    int key_dim, int value_dim, int32_t* flags, void* stream);
+
+/* Bytes of workspace mqh_linear_prefill needs (delta: 1 with beta, 0 without). */
+int64_t mqh_linear_prefill_workspace_bytes(int tokens, int seqs, int heads, int key_dim, int value_dim, int delta);
+
+/* Prompts through the same recurrence, `tokens` rows in all: sequence b's are
+ * starts[b] .. starts[b + 1] - 1 (starts [seqs + 1] int32; NULL: one sequence,
+ * all rows), its state is row b of `state`, read and updated.  The same result
+ * as mqh_linear_step token by token up to FP32 rounding.  Rows of no sequence
+ * are left as they were; starts out of range latch -9.  A value that is not
+ * finite makes outputs of its 64-token chunk, and everything after, not finite.
+ * The workspace (256-byte aligned) is the call's own until its kernels have
+ * run.  Returns 0, -1, -2, -5 or -6. */
+int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                       const void* v, int64_t v_token, int64_t v_head, int type, const float* beta, int64_t beta_token,
+                       const float* gate, int64_t gate_token, float* state, void* out, const int32_t* starts,
+                       int tokens, int seqs, int heads, int key_heads, int key_dim, int value_dim, void* workspace,
+                       int64_t workspace_bytes, int32_t* flags, void* stream);
+
+/* The calls of this group with their arguments, in order, as 64-bit words (20,
+ * 16, 27, 23 and 27; pointers as integers, the scale as the bits of a double). */
 int mqh_kv_write_words(const int64_t* args);
 int mqh_kv_read_words(const int64_t* args);
 int mqh_attend_words(const int64_t* args);
+int mqh_linear_step_words(const int64_t* args);
+int mqh_linear_prefill_words(const int64_t* args);
 
 #ifdef __cplusplus
 }

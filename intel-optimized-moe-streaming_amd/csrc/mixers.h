@@ -65,12 +65,33 @@ struct LinearParams {
     const int32_t* starts;      // [seqs + 1]
     float* state;               // [seqs x heads x value_dim x key_dim]
     void* out;                  // [tokens x heads x value_dim] contiguous
-    float* work;                // prompts: the workspace
     int type;
     int tokens, seqs, heads, key_heads, key_dim, value_dim;
     int* flags;
+    // prompts: the workspace (a chunk of 64 tokens of a head at a time, indexed
+    // [chunk - chunk0][head]), and the chunks of this pass
+    float* w;                   // [64 x KP] T diag(beta e^G) K            (delta rule)
+    float* u;                   // [VP x 64] T diag(beta) V, then the writes U, transposed (delta rule)
+    float* s0;                  // [VP x KP] the state before the chunk
+    double* g;                  // [64] running sums of the gate
+    float* e;                   // [64] e^(G_end - G), and [64] e^(G_end) from 64 on
+    int chunk0, chunks;
 };
 
+constexpr int LINEAR_CHUNK = 64;
+// key dims are padded to 64, 128 or 256, value dims to a multiple of 16
+inline int linear_kp(int key_dim) { return key_dim <= 64 ? 64 : key_dim <= 128 ? 128 : 256; }
+inline int linear_vp(int value_dim) { return (value_dim + 15) & ~15; }
+// chunks of sequence b begin at starts[b] / 64 + b: room for its partial chunk
+// without a prefix sum
+inline int64_t linear_chunks(int64_t tokens, int64_t seqs) { return tokens / LINEAR_CHUNK + seqs; }
+// floats of one chunk of one head
+inline int64_t linear_chunk_floats(int kp, int vp, bool delta) {
+    return (delta ? 64 * kp + 64 * vp : 0) + (int64_t)vp * kp + 128 + 128;
+}
+
+hipError_t launch_linear_step(const LinearParams& p, hipStream_t s);
+hipError_t launch_linear_prompt(const LinearParams& p, hipStream_t s);
 hipError_t launch_kv_write(const KvParams& p, hipStream_t s);
 hipError_t launch_kv_read(const KvParams& p, hipStream_t s);
 
@@ -121,6 +142,33 @@ __device__ __forceinline__ void load8(const void* base, int64_t at, float (&x)[8
             x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
         }
     }
+}
+
+// one element, four consecutive elements as FP32
+template <int TYPE>
+__device__ __forceinline__ float load1(const void* base, int64_t at) {
+    if constexpr (TYPE == MIX_F32) return ((const float*)base)[at];
+    else if constexpr (TYPE == MIX_F16) return (float)((const _Float16*)base)[at];
+    else return __uint_as_float((uint32_t)((const uint16_t*)base)[at] << 16);
+}
+template <int TYPE>
+__device__ __forceinline__ floatx4 load4(const void* base, int64_t at) {
+    if constexpr (TYPE == MIX_F32) {
+        return load_any<floatx4>((const float*)base + at);
+    } else if constexpr (TYPE == MIX_F16) {
+        const half4 a = load_any<half4>((const _Float16*)base + at);
+        return floatx4{(float)a[0], (float)a[1], (float)a[2], (float)a[3]};
+    } else {
+        const uintx2 a = load_any<uintx2>((const uint16_t*)base + at);
+        return floatx4{__uint_as_float(a[0] << 16), __uint_as_float(a[0] & 0xffff0000u),
+                       __uint_as_float(a[1] << 16), __uint_as_float(a[1] & 0xffff0000u)};
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ void store1(void* base, int64_t at, float x) {
+    if constexpr (TYPE == MIX_F32) ((float*)base)[at] = x;
+    else if constexpr (TYPE == MIX_F16) ((_Float16*)base)[at] = (_Float16)x;
+    else ((__bf16*)base)[at] = (__bf16)x;
 }
 
 // eight FP32 values to a row, each rounded once (to nearest, ties to even)

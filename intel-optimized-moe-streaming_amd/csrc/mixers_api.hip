@@ -69,6 +69,31 @@ bool attend_sizes(int tokens, int seqs, int single, int heads, int kv_heads, int
     return ((int64_t)tokens + seqs) * kv_heads < (int64_t)1 << 31 && (int64_t)tokens * heads * dim < (int64_t)1 << 40;
 }
 
+// what both linear calls have to hold
+int check_linear(const void* q, const void* k, const void* v, int type, const float* gate, const float* state,
+                 const void* out, int tokens, int seqs, int heads, int key_heads, int key_dim, int value_dim,
+                 const int32_t* flags) {
+    if (!q || !k || !v || !gate || !state || !out || !flags) return ST_ARG;
+    if (!row_type(type)) return ST_TYPE;
+    if (tokens <= 0 || seqs <= 0 || heads <= 0 || key_heads <= 0 || heads % key_heads || heads > 4096) return ST_ARG;
+    if (key_dim <= 0 || key_dim > 256 || key_dim % 4 || value_dim <= 0 || value_dim > 1024 || value_dim % 4)
+        return ST_TYPE;
+    const int size = mix_bytes(type);
+    if (unaligned(q, size) || unaligned(k, size) || unaligned(v, size) || unaligned(out, size)) return ST_ARG;
+    if (unaligned(state, 16) || unaligned(gate, 4)) return ST_ARG;
+    return tokens > 1 << 24 || seqs > 1 << 20 || (int64_t)seqs * heads >= (int64_t)1 << 24 ? ST_ARG : ST_OK;
+}
+
+// Chunks a pass of the prompt kernels takes: all of them up to a workspace of
+// 1 GiB, at least 64 (a pass costs three launches and breaks the scans of other
+// sequences off).
+constexpr int64_t LINEAR_PASS_BYTES = (int64_t)1 << 30;
+int64_t linear_pass_chunks(int tokens, int seqs, int heads, int key_dim, int value_dim, bool delta) {
+    const int64_t all = linear_chunks(tokens, seqs);
+    const int64_t one = heads * linear_chunk_floats(linear_kp(key_dim), linear_vp(value_dim), delta) * 4;
+    return std::min(all, std::max<int64_t>(64, LINEAR_PASS_BYTES / one));
+}
+
 }  // namespace
 
 extern "C" {
@@ -153,8 +178,88 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
     return status(e);
 }
 
+int mqh_linear_step(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                    const void* v, int64_t v_token, int64_t v_head, int type, const float* beta, int64_t beta_token,
+                    const float* gate, int64_t gate_token, float* state, void* out, int seqs, int heads, int key_heads,
+                    int key_dim, int value_dim, int32_t* flags, void* stream) {
+    const int st = check_linear(q, k, v, type, gate, state, out, seqs, seqs, heads, key_heads, key_dim, value_dim, flags);
+    if (st) return st;
+    LinearParams p{};
+    p.q = q; p.k = k; p.v = v;
+    p.q_token = q_token; p.q_head = q_head; p.k_token = k_token; p.k_head = k_head;
+    p.v_token = v_token; p.v_head = v_head;
+    p.beta = beta; p.beta_token = beta_token; p.gate = gate; p.gate_token = gate_token;
+    p.state = state; p.out = out; p.type = type;
+    p.tokens = seqs; p.seqs = seqs; p.heads = heads; p.key_heads = key_heads;
+    p.key_dim = key_dim; p.value_dim = value_dim; p.flags = flags;
+    return status(launch_linear_step(p, (hipStream_t)stream));
+}
+
+int64_t mqh_linear_prefill_workspace_bytes(int tokens, int seqs, int heads, int key_dim, int value_dim, int delta) {
+    if (tokens <= 0 || seqs <= 0 || heads <= 0 || heads > 4096 || key_dim <= 0 || key_dim > 256 || key_dim % 4 ||
+        value_dim <= 0 || value_dim > 1024 || value_dim % 4 || (delta != 0 && delta != 1) || tokens > 1 << 24 ||
+        seqs > 1 << 20)
+        return ST_ARG;
+    return linear_pass_chunks(tokens, seqs, heads, key_dim, value_dim, delta) * heads *
+           linear_chunk_floats(linear_kp(key_dim), linear_vp(value_dim), delta) * 4;
+}
+
+int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                       const void* v, int64_t v_token, int64_t v_head, int type, const float* beta, int64_t beta_token,
+                       const float* gate, int64_t gate_token, float* state, void* out, const int32_t* starts,
+                       int tokens, int seqs, int heads, int key_heads, int key_dim, int value_dim, void* workspace,
+                       int64_t workspace_bytes, int32_t* flags, void* stream) {
+    const int st = check_linear(q, k, v, type, gate, state, out, tokens, seqs, heads, key_heads, key_dim, value_dim, flags);
+    if (st) return st;
+    if (!starts && seqs != 1) return ST_ARG;
+    const bool delta = beta != nullptr;
+    const int64_t pass = linear_pass_chunks(tokens, seqs, heads, key_dim, value_dim, delta), units = pass * heads;
+    const int kp = linear_kp(key_dim), vp = linear_vp(value_dim);
+    if (workspace_bytes < units * linear_chunk_floats(kp, vp, delta) * 4) return ST_WORKSPACE;
+    if (!workspace || unaligned(workspace, 256)) return ST_ARG;
+    LinearParams p{};
+    p.q = q; p.k = k; p.v = v;
+    p.q_token = q_token; p.q_head = q_head; p.k_token = k_token; p.k_head = k_head;
+    p.v_token = v_token; p.v_head = v_head;
+    p.beta = beta; p.beta_token = beta_token; p.gate = gate; p.gate_token = gate_token;
+    p.state = state; p.out = out; p.starts = starts; p.type = type;
+    p.tokens = tokens; p.seqs = seqs; p.heads = heads; p.key_heads = key_heads;
+    p.key_dim = key_dim; p.value_dim = value_dim; p.flags = flags;
+    // (every part is a multiple of 64 floats a unit)
+    p.g = (double*)workspace;
+    p.e = (float*)workspace + units * 128;
+    p.s0 = p.e + units * 128;
+    p.w = p.s0 + units * vp * kp;
+    p.u = p.w + units * 64 * kp;
+    const int64_t all = linear_chunks(tokens, seqs);
+    for (int64_t at = 0; at < all; at += pass) {
+        p.chunk0 = (int)at;
+        p.chunks = (int)std::min(pass, all - at);
+        const hipError_t e = launch_linear_prompt(p, (hipStream_t)stream);
+        if (e != hipSuccess) return ST_HIP;
+    }
+    return ST_OK;
+}
+
 // The calls with their arguments, in order, as 64-bit words (pointers as
 // integers, floats as the bits of a double)
+int mqh_linear_step_words(const int64_t* a) {
+    if (!a) return ST_ARG;
+    const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
+    return mqh_linear_step(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10), a[11],
+                           (const float*)P(12), a[13], (float*)P(14), P(15), (int)a[16], (int)a[17], (int)a[18],
+                           (int)a[19], (int)a[20], (int32_t*)P(21), P(22));
+}
+
+int mqh_linear_prefill_words(const int64_t* a) {
+    if (!a) return ST_ARG;
+    const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
+    return mqh_linear_prefill(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10),
+                              a[11], (const float*)P(12), a[13], (float*)P(14), P(15), (const int32_t*)P(16),
+                              (int)a[17], (int)a[18], (int)a[19], (int)a[20], (int)a[21], (int)a[22], P(23), a[24],
+                              (int32_t*)P(25), P(26));
+}
+
 int mqh_kv_write_words(const int64_t* a) {
     if (!a) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };

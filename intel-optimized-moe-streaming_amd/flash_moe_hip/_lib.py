@@ -50,6 +50,11 @@ EXPORTS = (
     "mqh_kv_write_words",
     "mqh_kv_read_words",
     "mqh_attend_words",
+    "mqh_linear_step",
+    "mqh_linear_prefill_workspace_bytes",
+    "mqh_linear_prefill",
+    "mqh_linear_step_words",
+    "mqh_linear_prefill_words",
 )
 
 STATUS_TEXT = {
@@ -162,7 +167,15 @@ def _declare(lib: C.CDLL) -> C.CDLL:
         _P, _P, _I64, _P, _P,                         # out, workspace, bytes, flags, stream
     ]
     lib.mqh_attend.restype = _I
-    for f in (lib.mqh_kv_write_words, lib.mqh_kv_read_words, lib.mqh_attend_words):
+    rows = [_P, _I64, _I64] * 3 + [_I, _P, _I64, _P, _I64, _P, _P]   # q, k, v with strides, type, beta, gate, state, out
+    lib.mqh_linear_step.argtypes = [*rows, _I, _I, _I, _I, _I, _P, _P]
+    lib.mqh_linear_step.restype = _I
+    lib.mqh_linear_prefill_workspace_bytes.argtypes = [_I, _I, _I, _I, _I, _I]
+    lib.mqh_linear_prefill_workspace_bytes.restype = _I64
+    lib.mqh_linear_prefill.argtypes = [*rows, _P, _I, _I, _I, _I, _I, _I, _P, _I64, _P, _P]
+    lib.mqh_linear_prefill.restype = _I
+    for f in (lib.mqh_kv_write_words, lib.mqh_kv_read_words, lib.mqh_attend_words, lib.mqh_linear_step_words,
+              lib.mqh_linear_prefill_words):
         f.argtypes = [C.c_char_p]
         f.restype = _I
     return lib

@@ -136,6 +136,24 @@ class DeltaState:
         _lib.check(rc, "mqh_delta_heads")
         return out
 
+    def prefill(self, q, k, v, beta, gate, *, out=None, stream=None):
+        """A prompt through the layer (mqh_linear_prefill, the form of the reference's
+        token loop, gated_deltanet.py:264-402, that takes 64 tokens at a time): q, k
+        [tokens, key_heads, key_dim] (key_heads a divisor of heads), v [tokens, heads,
+        value_dim] of one type (FP32, FP16 or BF16), beta and gate [tokens, heads]
+        FP32; the state is updated and [tokens, heads, value_dim] returned.  FP32
+        sums in an order of their own, where ``step`` has the reference's bit for
+        bit.  key_dim a multiple of 4 up to 256, value_dim one up to 1024."""
+        from .kv_cache import OnStream
+        from .linear_attention import check_dims, prefill_states
+
+        nv, dv, dk = self.shape
+        check_dims(dk, dv)
+        if self.state.get_device() < 0:
+            raise ValueError(f"expected a CUDA device, got {self.state.device}")
+        return prefill_states(self.lib, OnStream(self.state.device), self._flags, self.state.view(1, nv, dv, dk), q, k,
+                              v, beta, gate, None, out, stream)
+
     def status(self, stream=None) -> int:
         """Synchronizes; -4 if an output was not finite since the last call."""
         import torch

@@ -88,3 +88,35 @@ def attend(q, k, v, scale, cache_dtype):
     if q.dtype == torch.float16:
         bound += 2.0 ** -25   # subnormal outputs
     return out, bound * 1.01 + 1e-30   # (products of the terms above)
+
+
+def linear(state, q, k, v, beta, gate):
+    """Token by token in float64: state [heads, dv, dk], q, k [n, key_heads, dk], v
+    [n, heads, dv], beta (or None) and gate [n, heads].  Returns (out, state, size)
+    with size [heads, dv]: the largest of |S row| + |v| |k| met on the way."""
+    heads = v.shape[1]
+    s = state.double().clone()
+    q, k = (t.double().repeat_interleave(heads // t.shape[1], 1) for t in (q, k))
+    v, decay = v.double(), torch.exp(gate.double())
+    out = torch.zeros(v.shape, dtype=torch.float64)
+    size = s.norm(dim=2)
+    for t in range(v.shape[0]):
+        s = s * decay[t].view(-1, 1, 1)
+        u = v[t]
+        if beta is not None:
+            u = beta[t].double().unsqueeze(1) * (u - torch.einsum("hvk,hk->hv", s, k[t]))
+        s = s + u.unsqueeze(2) * k[t].unsqueeze(1)
+        out[t] = torch.einsum("hvk,hk->hv", s, q[t])
+        size = torch.maximum(size, s.norm(dim=2) + v[t].abs() * k[t].norm(dim=1, keepdim=True))
+    return out, s, size
+
+
+def linear_bound(size, tokens, key_dim, chunk=64):
+    """How far a row of the state may be off, in 2-norm (and an output, for |q| <= 1),
+    for keys of norm <= 1, gates <= 0 and beta in [0, 1]: a step of the recurrence
+    then never lengthens an error, so those of the chunks add up.  A chunk's error is
+    that of four FP32 products of at most key_dim + 64 terms (W S, the writes, the
+    state, the output), each term off by 2^-24 of |S| + |v| |k|, and its solution
+    of 1 + L doubles them at most (its inverse is a product of such steps)."""
+    chunks = -(-tokens // chunk) + 1
+    return chunks * 8 * (key_dim + chunk) * 2.0 ** -24 * size

@@ -101,3 +101,77 @@ def test_attend_codes(lib):
     assert lib.mqh_attend_workspace_bytes(4, 2, 1, 8, 2, 64, 64) == -1
     assert lib.mqh_attend_workspace_bytes(4, 2, 0, 8, 3, 64, 64) == -1
     assert lib.mqh_attend_workspace_bytes(4096, 1, 0, 32, 8, 128, 4096) >= 0
+
+
+def linear(lib, prompt=False, **kw):
+    a = dict(q=P, qt=64, qh=16, k=P, kt=64, kh=16, v=P, vt=64, vh=16, type=0, beta=P, bt=4, gate=P, gt=4, state=P, out=P)
+    if prompt:
+        a.update(starts=P, tokens=8, seqs=2, heads=4, key_heads=4, key_dim=16, value_dim=16, ws=P, bytes=1 << 30)
+    else:
+        a.update(seqs=2, heads=4, key_heads=4, key_dim=16, value_dim=16)
+    a.update(flags=P, stream=None)
+    a.update(kw)
+    return (lib.mqh_linear_prefill if prompt else lib.mqh_linear_step)(*a.values())
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_linear_codes(lib, prompt):
+    for bad in (dict(q=None), dict(k=None), dict(v=None), dict(gate=None), dict(state=None), dict(out=None),
+                dict(flags=None), dict(seqs=0), dict(heads=0), dict(heads=6), dict(key_heads=0), dict(heads=4100),
+                dict(state=C.c_void_p(4100)), dict(q=C.c_void_p(4098)), dict(out=C.c_void_p(4098))):
+        assert linear(lib, prompt, **bad) == -1, bad
+    for bad in (dict(type=3), dict(key_dim=15), dict(key_dim=260), dict(value_dim=18), dict(value_dim=1028),
+                dict(key_dim=0)):
+        assert linear(lib, prompt, **bad) == -2, bad
+    assert lib.mqh_linear_step_words(None) == -1 and lib.mqh_linear_prefill_words(None) == -1
+
+
+def test_linear_prompt_codes(lib):
+    need = lib.mqh_linear_prefill_workspace_bytes(8, 2, 4, 16, 16, 1)
+    assert need > lib.mqh_linear_prefill_workspace_bytes(8, 2, 4, 16, 16, 0) > 0
+    assert linear(lib, True, bytes=need - 1) == -6
+    assert linear(lib, True, tokens=0) == -1
+    assert linear(lib, True, starts=None) == -1
+    assert linear(lib, True, ws=None) == -1
+    assert linear(lib, True, ws=C.c_void_p(4096 + 64)) == -1
+    assert lib.mqh_linear_prefill_workspace_bytes(8, 2, 4, 18, 16, 1) == -1
+    assert lib.mqh_linear_prefill_workspace_bytes(0, 2, 4, 16, 16, 1) == -1
+
+
+def test_linear_state_constructor():
+    from flash_moe_hip.linear_attention import LinearState
+
+    with pytest.raises(ValueError, match="multiple of 4"):
+        LinearState(1, 2, 16, 18, device="cpu")
+    with pytest.raises(ValueError, match="multiple of 4"):
+        LinearState(1, 2, 16, 260, device="cpu")
+    with pytest.raises(ValueError, match="at least 1"):
+        LinearState(0, 2, 16, 16, device="cpu")
+    with pytest.raises(ValueError, match="CUDA device"):
+        LinearState(1, 2, 16, 16, device="cpu")
+    with pytest.raises(ValueError, match="shape"):
+        LinearState(1, 2, 16, 16, state=torch.zeros(1, 2, 16, 8))
+    with pytest.raises(ValueError, match="no backward"):
+        LinearState(1, 2, 16, 16, state=torch.zeros(1, 2, 16, 16, requires_grad=True))
+
+
+def test_row_checks():
+    from flash_moe_hip.kv_cache import check_index, check_rows
+
+    cpu, types = torch.device("cpu"), (torch.float32, torch.float16)
+    x = torch.zeros(4, 2, 64)
+    check_rows(x, (4, 2, 64), types, cpu, "x")
+    check_rows(torch.zeros(4, 200)[:, 3:131].unflatten(1, (2, 64)), (4, 2, 64), types, cpu, "x")
+    for bad, why in ((x[:3], "shape"), (x.double(), "expected one of"), (x.transpose(0, 2), "shape"),
+                     (torch.zeros(4, 64, 2).transpose(1, 2), "contiguous"), (x.clone().requires_grad_(), "backward")):
+        with pytest.raises(ValueError, match=why):
+            check_rows(bad, (4, 2, 64), types, cpu, "x")
+    with pytest.raises(ValueError, match="on cpu"):
+        check_rows(x, (4, 2, 64), types, torch.device("cuda", 0), "x")
+    i = torch.zeros(6, dtype=torch.int32)
+    check_index(i, (6,), torch.int32, cpu, "i")
+    for bad in (i[:5], i.long(), torch.zeros(12, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="contiguous"):
+            check_index(bad, (6,), torch.int32, cpu, "i")
+    with pytest.raises(ValueError, match="on cpu"):
+        check_index(i, (6,), torch.int32, torch.device("cuda", 0), "i")
