@@ -390,7 +390,7 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
  * state [seqs x heads x value_dim x key_dim] FP32 (16-byte aligned), updated in
  * place; q, k [seqs x key_heads x key_dim] and v [seqs x heads x value_dim] of
  * `type` (F32, F16 or BF16; element strides *_token and *_head, the last
- * dimension contiguous); value head h uses key head h / (heads / key_heads);
+ * dimension contiguous, strides at most 2^22); value head h uses key head h / (heads / key_heads);
  * beta, gate [seqs x heads] FP32 with row strides; out [seqs x heads x
  * value_dim] contiguous.  key_dim a multiple of 4 up to 256, value_dim one up
  * to 1024.  Sums are FP32; their order is this library's own, not that of

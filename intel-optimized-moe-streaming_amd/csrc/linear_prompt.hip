@@ -7,8 +7,8 @@
 //   S1 = e^(G_C) S0 + (diag(e^(G_C - G)) U)^T K
 // (U = V without the delta rule).  Only U and S1 need the chunks in order, so
 // three launches share the work:
-//   1 k_linear_solve   chunks in parallel: W = (1 + L)^-1 diag(beta e^G) K and
-//                      (1 + L)^-1 diag(beta) V
+//   1 k_linear_solve   chunks in parallel: W = (1 + L)^-1 diag(beta e^G) K,
+//                      (1 + L)^-1 diag(beta) V and diag(e^(G_C - G)) K
 //   2 k_linear_scan    chunk after chunk, 16 value rows of a head a workgroup:
 //                      U = (1 + L)^-1 diag(beta) V - W S0^T, then S1
 //   3 k_linear_out     chunks in parallel: O
@@ -25,6 +25,10 @@
 // elements in one 16-byte load and, for the right one, register j of a result as
 // it stands.  So U goes from result to operand without moving, and so does the
 // state: S^T tiles are both the accumulators of S1 and the operand of W S0^T.
+//
+// What one kernel leaves for another lies in the workspace in operand order, 16
+// bytes a lane, a 16 x 16 tile's 1 KiB in one run (rows 256 bytes and more apart
+// cost the address unit 64 cycles a load: the scan took 4 us a chunk so).
 
 #include "mixers.h"
 
@@ -92,39 +96,110 @@ __device__ __forceinline__ double gate_sums(const LinearParams& p, const ChunkRa
     return g;
 }
 
-// what the other two kernels read of the gate, by one wave
-__device__ __forceinline__ void store_gates(const LinearParams& p, int64_t ch, double g) {
+// what the other two kernels read of the gate, by one wave; returns e^(G_end - G)
+__device__ __forceinline__ float store_gates(const LinearParams& p, int64_t ch, double g) {
     const int lane = threadIdx.x & 63;
     const double end = __shfl(g, 63);
     p.g[ch * C + lane] = g;
-    p.e[ch * 128 + lane] = expf((float)(end - g));
+    const float to_end = expf((float)(end - g));
+    p.e[ch * 128 + lane] = to_end;
     if (lane == 63) p.e[ch * 128 + 64] = expf((float)end);
+    return to_end;
 }
 
-// without the delta rule: the gates are all there is to prepare
-__global__ __launch_bounds__(256) void k_linear_gates(LinearParams p) {
-    const int64_t ch = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (ch >= (int64_t)p.chunks * p.heads) return;
-    const ChunkRange c = chunk_range(p, (int)(ch / p.heads));
-    if (!c.count) return;
-    store_gates(p, ch, gate_sums(p, c, (int)(ch % p.heads)));
-}
+constexpr int THREADS = 512;   // of the kernels that take chunks in parallel
 
-// rows of a chunk into LDS as FP32 [64][KP + 4], zeros past its end and key_dim
-template <int KP, int TYPE>
-__device__ __forceinline__ void stage_rows(const LinearParams& p, const ChunkRange& c, const void* x, int64_t token,
-                                           int64_t head_at, float* to) {
-    constexpr int PIECES = KP / 4;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < C * PIECES; i += 256) {
-        const int t = i / PIECES, col = (i % PIECES) * 4;
-        floatx4 v = {0, 0, 0, 0};
-        if (t < c.count && col < p.key_dim) v = load4<TYPE>(x, (int64_t)(c.first + t) * token + head_at + col);
-        *(floatx4*)(to + t * (KP + 4) + col) = v;
+// A chunk's rows of q, k or v of one head as a buffer: lane offsets of 32 bits
+// from a uniform base (64-bit products per load cost the scan more than its
+// matrix instructions), and a read past the last row's end gives 0.  (Strides are
+// at most 2^22 elements, so a chunk's offsets stay below 2^31.)
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+template <int TYPE>
+constexpr int TYPE_BYTES = TYPE == MIX_F32 ? 4 : 2;
+
+__device__ __forceinline__ Rsrc buffer_of(const void* base, int64_t bytes, uint32_t size) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const uint8_t*)base + bytes), 0, size, 0x00027000);
+}
+template <int TYPE>
+__device__ __forceinline__ Rsrc rows_buffer(const void* x, int first, int count, int64_t token, int64_t head_at, int dim) {
+    constexpr int B = TYPE_BYTES<TYPE>;
+    return buffer_of(x, ((int64_t)first * token + head_at) * B, (uint32_t)(((count - 1) * (int)token + dim) * B));
+}
+__device__ __forceinline__ floatx4 buffer4(Rsrc r, uint32_t at, uint32_t uniform = 0) {
+    return __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, at, uniform, 0));
+}
+// one element as it lies, and its value; four as FP32
+template <int TYPE>
+__device__ __forceinline__ uint32_t buffer_raw(Rsrc r, uint32_t at) {
+    if constexpr (TYPE == MIX_F32) return __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
+}
+template <int TYPE>
+__device__ __forceinline__ float raw_value(uint32_t v) {
+    if constexpr (TYPE == MIX_F32) return __uint_as_float(v);
+    else if constexpr (TYPE == MIX_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)v);
+    else return __uint_as_float(v << 16);
+}
+template <int TYPE>
+__device__ __forceinline__ floatx4 buffer_values4(Rsrc r, uint32_t at) {
+    if constexpr (TYPE == MIX_F32) {
+        return buffer4(r, at);
+    } else {
+        const uintx2 a = __builtin_bit_cast(uintx2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0));
+        return floatx4{raw_value<TYPE>(a[0] & 0xffffu), raw_value<TYPE>(a[0] >> 16), raw_value<TYPE>(a[1] & 0xffffu),
+                       raw_value<TYPE>(a[1] >> 16)};
     }
 }
 
-// tiles (i, j <= i) of a 4 x 4 block triangle, wave w taking the w-th of every four
+// rows of a chunk for LDS as FP32 [64][KP + 4], zeros past its end and key_dim:
+// every load of a thread in flight before its first store
+template <int KP, int TYPE>
+struct StagedRows {
+    static constexpr int PIECES = KP / 4, N = C * PIECES / THREADS;
+    floatx4 v[N];
+    __device__ __forceinline__ void load(const LinearParams& p, const ChunkRange& c, const void* x, int64_t token,
+                                         int64_t head_at) {
+        constexpr int B = TYPE_BYTES<TYPE>;
+        const Rsrc r = rows_buffer<TYPE>(x, c.first, c.count, token, head_at, p.key_dim);
+        const uint32_t step = (uint32_t)token * (THREADS / PIECES) * B;
+        uint32_t at = (uint32_t)token * (threadIdx.x / PIECES) * B + (threadIdx.x % PIECES) * 4 * B;
+#pragma unroll
+        for (int n = 0; n < N; ++n, at += step) v[n] = buffer_values4<TYPE>(r, at);
+    }
+    __device__ __forceinline__ void store(const LinearParams& p, const ChunkRange& c, float* to) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = threadIdx.x + n * THREADS, t = i / PIECES, col = (i % PIECES) * 4;
+            const bool there = t < c.count && col < p.key_dim;
+            *(floatx4*)(to + t * (KP + 4) + col) = there ? v[n] : floatx4{0, 0, 0, 0};
+        }
+    }
+};
+
+// column `row` of a value tile, 16 i + 4 g + r of the chunk's tokens in v[i][r]:
+// as read, and with what is past the end as zeros
+template <int TYPE>
+__device__ __forceinline__ void load_values(const LinearParams& p, const ChunkRange& c, int head, int row, floatx4 (&v)[4]) {
+    constexpr int B = TYPE_BYTES<TYPE>;
+    const int g = (threadIdx.x & 63) >> 4;
+    const Rsrc b = rows_buffer<TYPE>(p.v, c.first, c.count, p.v_token, head * p.v_head, p.value_dim);
+    const uint32_t token = (uint32_t)p.v_token * B;
+    uint32_t at = token * 4 * g + (row < p.value_dim ? row : 0) * B;
+#pragma unroll
+    for (int i = 0; i < 4; ++i, at += token * 16)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[i][r] = raw_value<TYPE>(buffer_raw<TYPE>(b, at + token * r));
+}
+__device__ __forceinline__ void mask_values(const LinearParams& p, const ChunkRange& c, int row, floatx4 (&v)[4]) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            v[i][r] = 16 * i + 4 * g + r < c.count && row < p.value_dim ? v[i][r] : 0.0f;
+}
+
+// tile n of the ten (i, j <= i) of a 4 x 4 block triangle
 __device__ __forceinline__ void triangle_tile(int n, int& i, int& j) {
     i = n >= 6 ? 3 : n >= 3 ? 2 : n >= 1 ? 1 : 0;
     j = n - i * (i + 1) / 2;
@@ -144,34 +219,72 @@ __device__ __forceinline__ floatx4 tile_product(const float* a, const float* b, 
 
 constexpr int LS = C + 4;   // row stride of the 64 x 64 matrices in LDS
 
-// ---- 1: W and (1 + L)^-1 diag(beta) V of a chunk of a head
-template <int KP, int TYPE>
-__global__ __launch_bounds__(256) void k_linear_solve(LinearParams p) {
+// ---- 1: W, (1 + L)^-1 diag(beta) V and K scaled to the chunk's end, of a chunk
+// of a head (without the delta rule V as it is, and no W)
+template <int KP, int TYPE, bool DELTA>
+__global__ __launch_bounds__(THREADS) void k_linear_solve(LinearParams p) {
     extern __shared__ __align__(16) float lds[];
     float* sk = lds;                       // [64][KP + 4]
-    float* sl = sk + C * (KP + 4);         // [64][LS]: -L
+    float* sl = sk + C * (KP + 4);         // [64][LS]: -L; later 1 KiB a wave to turn W's tiles in
     float* st = sl + C * LS;               // [4][16][20]: inverses of the diagonal blocks of 1 + L
     __shared__ double s_g[C];
-    __shared__ __align__(16) float s_beta[C], s_through[C];   // beta, beta e^G
+    __shared__ __align__(16) float s_beta[C], s_through[C], s_end[C];   // beta, beta e^G, e^(G_end - G)
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t ch = blockIdx.x;
     const int head = (int)(ch % p.heads), key_head = head / (p.heads / p.key_heads);
     const ChunkRange c = chunk_range(p, (int)(ch / p.heads));
     if (!c.count) return;
 
-    stage_rows<KP, TYPE>(p, c, p.k, p.k_token, key_head * p.k_head, sk);
-    if (wave == 0) {
-        const double sum = gate_sums(p, c, head);
-        const float beta = lane < c.count ? p.beta[(int64_t)(c.first + lane) * p.beta_token + head] : 0.0f;
-        s_g[lane] = sum;
-        s_beta[lane] = beta;
-        s_through[lane] = beta * expf((float)sum);
-        store_gates(p, ch, sum);
+    const int vp = (p.value_dim + 15) & ~15;
+    // the first value tile of a wave is read ahead of everything
+    floatx4 x[4];
+    const int v_waves = DELTA ? KP / 16 : 0;   // tiles of W go before those of V
+    const int first_v = v_waves + (wave + 8 - v_waves % 8) % 8;
+    if (first_v < v_waves + vp / 16) load_values<TYPE>(p, c, head, 16 * (first_v - v_waves) + l16, x);
+    {
+        StagedRows<KP, TYPE> rows;
+        rows.load(p, c, p.k, p.k_token, key_head * p.k_head);
+        if (wave == 0) {
+            const double sum = gate_sums(p, c, head);
+            s_g[lane] = sum;
+            s_end[lane] = store_gates(p, ch, sum);
+            if constexpr (DELTA) {
+                const float beta = lane < c.count ? p.beta[(int64_t)(c.first + lane) * p.beta_token + head] : 0.0f;
+                s_beta[lane] = beta;
+                s_through[lane] = beta * expf((float)sum);
+            }
+        }
+        rows.store(p, c, sk);
     }
     __syncthreads();
 
-    for (int n = wave; n < 10; n += 4) {
+    // K scaled to the chunk's end, tile (i, n): column 16 n + l16, tokens 16 i + 4 g + j
+    {
+        floatx4* ke = (floatx4*)(p.k_end + ch * C * KP);
+        const floatx4 f = *(const floatx4*)(s_end + 16 * (wave & 3) + 4 * g);
+#pragma unroll
+        for (int n = 0; n < KP / 32; ++n) {
+            const float* at = sk + (16 * (wave & 3) + 4 * g) * (KP + 4) + 16 * (2 * n + (wave >> 2)) + l16;
+            floatx4 v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = at[r * (KP + 4)] * f[r];
+            ke[((2 * n + (wave >> 2)) * 4 + (wave & 3)) * 64 + lane] = v;
+        }
+    }
+    floatx4* u = (floatx4*)(p.u + ch * C * vp);
+    if constexpr (!DELTA) {
+        for (int n = wave; n < vp / 16; n += 8) {
+            if (n != wave) load_values<TYPE>(p, c, head, 16 * n + l16, x);
+            mask_values(p, c, 16 * n + l16, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[(n * 4 + i) * 64 + lane] = x[i];
+        }
+        return;
+    }
+
+    for (int n = wave; n < 10; n += 8) {
         int i, j;
         triangle_tile(n, i, j);
         const floatx4 d = tile_product<KP>(sk, sk, i, j);
@@ -185,7 +298,7 @@ __global__ __launch_bounds__(256) void k_linear_solve(LinearParams p) {
     __syncthreads();
 
     // column l16 of the inverse of diagonal block `wave`, by substitution
-    {
+    if (wave < 4) {
         float x[16];
         const float* rows = sl + 16 * wave * LS + 16 * wave;
 #pragma unroll
@@ -207,54 +320,73 @@ __global__ __launch_bounds__(256) void k_linear_solve(LinearParams p) {
         for (int j = 0; j < i; ++j)
             lo[i * (i - 1) / 2 + j] = *(const floatx4*)(sl + (16 * i + l16) * LS + 16 * j + 4 * g);
     }
-    const int vp = (p.value_dim + 15) & ~15;
-    float* w = p.w + ch * C * KP;
-    float* u = p.u + ch * C * vp;
-    for (int n = wave; n < KP / 16 + vp / 16; n += 4) {
-        const bool is_v = n >= KP / 16;
-        const int col = 16 * (is_v ? n - KP / 16 : n) + l16;
-        floatx4 x[4];
+    __syncthreads();   // (-L is in registers: its place turns tiles from here)
+    // W tile (i, n): token 16 i + l16, columns 16 n + 4 g + j of lane 16 g + l16; the
+    // solution's tiles have their columns across the lanes and are turned in LDS
+    floatx4* w = (floatx4*)(p.w + ch * C * KP);
+    float* turn = sl + wave * 256;
+    for (int n = wave; n < v_waves + vp / 16; n += 8) {
+        const bool is_v = n >= v_waves;
+        const int col = 16 * (is_v ? n - v_waves : n) + l16;
+        floatx4 y[4];
+        if (is_v) {
+            if (n != first_v) load_values<TYPE>(p, c, head, col, x);
+            mask_values(p, c, col, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const floatx4 f = *(const floatx4*)((is_v ? s_beta : s_through) + 16 * i + 4 * g);
+            for (int i = 0; i < 4; ++i) y[i] = x[i] * *(const floatx4*)(s_beta + 16 * i + 4 * g);
+        } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * i + 4 * g + r;
-                float v = 0.0f;
-                if (!is_v) v = sk[t * (KP + 4) + col];
-                else if (t < c.count && col < p.value_dim)
-                    v = load1<TYPE>(p.v, (int64_t)(c.first + t) * p.v_token + head * p.v_head + col);
-                x[i][r] = v * f[r];
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[i][r] = sk[(16 * i + 4 * g + r) * (KP + 4) + col];
+                y[i] *= *(const floatx4*)(s_through + 16 * i + 4 * g);
             }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            floatx4 acc = x[i];
 #pragma unroll
-            for (int j = 0; j < i; ++j) acc = mfma4(lo[i * (i - 1) / 2 + j], x[j], acc);
-            x[i] = mfma4(inv[i], acc, floatx4{0, 0, 0, 0});
-            if (is_v) *(floatx4*)(u + (int64_t)col * C + 16 * i + 4 * g) = x[i];
-            else
+            for (int j = 0; j < i; ++j) y[i] = mfma4(lo[i * (i - 1) / 2 + j], y[j], y[i]);
+            y[i] = mfma4(inv[i], y[i], floatx4{0, 0, 0, 0});
+            if (is_v) {
+                u[((n - v_waves) * 4 + i) * 64 + lane] = y[i];
+            } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) w[(16 * i + 4 * g + r) * KP + col] = x[i][r];
+                for (int r = 0; r < 4; ++r) turn[(16 * (l16 >> 2) + 4 * g + r) * 4 + (l16 & 3)] = y[i][r];
+                // (a wave's LDS accesses are in order; the fence is the compiler's)
+                asm volatile("" ::: "memory");
+                w[(n * 4 + i) * 64 + lane] = *(const floatx4*)(turn + 4 * lane);
+                asm volatile("" ::: "memory");
+            }
         }
     }
 }
 
 // ---- 2: the state from chunk to chunk, 16 value rows of a head
-template <int KP, int TYPE, bool DELTA>
+// one chunk's operands of a wave of the scan
+template <int NB, bool DELTA>
+struct ScanStage {
+    floatx4 w[DELTA ? 4 : 1][NB], ke[4][NB], u[4];
+    float end;
+};
+
+template <int KP, bool DELTA>
 __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
     constexpr int KW = KP / 4;       // key columns of a wave
     constexpr int NB = KW / 16;
+    // chunks in flight, the one in work among them: without the delta rule a chunk
+    // is short work beside the latency of its loads
+    constexpr int DEPTH = DELTA ? 2 : 4;
+    using Stage = ScanStage<NB, DELTA>;
     __shared__ __align__(16) floatx4 part[2][4][4][64];   // W S0^T over each wave's columns, by turns
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the value tiles of a head run on one XCD (workgroups go round the eight), so
     // that its W and K are read into one L2
     const int vt = (p.value_dim + 15) / 16;
     const int sh = blockIdx.x / (8 * vt) * 8 + (blockIdx.x & 7), tile = (blockIdx.x / 8) % vt;
     if (sh >= p.seqs * p.heads) return;
-    const int b = sh / p.heads, head = sh % p.heads, key_head = head / (p.heads / p.key_heads);
+    const int b = sh / p.heads, head = sh % p.heads;
     int s0, s1;
     sequence_bounds(p, b, s0, s1, tid == 0);
     // this pass's chunks of the sequence
@@ -273,79 +405,99 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
         s[n] = row_live && col < p.key_dim ? *(const floatx4*)(state + col) : floatx4{0, 0, 0, 0};
     }
 
-    floatx4 w[DELTA ? 4 : 1][NB], k[4][NB], u[4], e[4];
-    float end;
-    auto load = [&](int n) {
-        const int64_t ch = (int64_t)(base + n) * p.heads + head;
-        const int first = s0 + n * C, left = min(s1 - first, C);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            e[i] = *(const floatx4*)(p.e + ch * 128 + 16 * i + 4 * g);
-            if constexpr (DELTA) {
-                u[i] = *(const floatx4*)(p.u + (ch * vp + row) * C + 16 * i + 4 * g);
-#pragma unroll
-                for (int m = 0; m < NB; ++m)
-                    w[i][m] = *(const floatx4*)(p.w + (ch * C + 16 * i + l16) * KP + kc + 16 * m + 4 * g);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * i + 4 * g + r;
-                const bool there = t < left;
-                const int64_t token = first + (there ? t : 0);
-                if constexpr (!DELTA) {
-                    const float v = load1<TYPE>(p.v, token * p.v_token + head * p.v_head + (row_live ? row : 0));
-                    u[i][r] = there && row_live ? v : 0.0f;
-                }
-#pragma unroll
-                for (int m = 0; m < NB; ++m) {
-                    const int col = kc + 16 * m + l16;
-                    const float v = load1<TYPE>(p.k, token * p.k_token + key_head * p.k_head + (col < p.key_dim ? col : 0));
-                    k[i][m][r] = there && col < p.key_dim ? v : 0.0f;
-                }
-            }
-        }
-        end = p.e[ch * 128 + 64];
+    // A chunk's tiles, 1 KiB each: 4 n + i of the wave's columns, i of the value tile
+    struct Buffers {
+        Rsrc w, ke, u;
     };
-    load(n0);
-    for (int n = n0; n < n1; ++n) {
+    auto buffers = [&](int n) {
         const int64_t ch = (int64_t)(base + n) * p.heads + head;
-        float* kept = p.s0 + (ch * vp + row) * KP + kc + 4 * g;
+        Buffers r;
+        r.w = buffer_of(p.w, (ch * KP + kc) * (C * 4), DELTA ? C * KW * 4 : 0);
+        r.ke = buffer_of(p.k_end, (ch * KP + kc) * (C * 4), C * KW * 4);
+        r.u = buffer_of(p.u, (ch * vp + 16 * tile) * (C * 4), C * 16 * 4);
+        return r;
+    };
+    auto load_w = [&](Stage& d, const Buffers& r, int i) {
 #pragma unroll
-        for (int m = 0; m < NB; ++m) *(floatx4*)(kept + 16 * m) = s[m];
+        for (int m = 0; m < NB; ++m) d.w[i][m] = buffer4(r.w, 16 * lane, 1024 * (4 * m + i));
+    };
+    auto load_rest = [&](Stage& d, const Buffers& r, int i) {
+        d.u[i] = buffer4(r.u, 16 * lane, 1024 * i);
+#pragma unroll
+        for (int m = 0; m < NB; ++m) d.ke[i][m] = buffer4(r.ke, 16 * lane, 1024 * (4 * m + i));
+    };
+    auto load_end = [&](Stage& d, int n) { d.end = p.e[((int64_t)(base + n) * p.heads + head) * 128 + 64]; };
+
+    // One chunk from `d`, while chunk `next`'s operands are read into `f`: a few
+    // loads before each group of products.  (All of them at once held the waves at
+    // the address unit for as long as half a chunk's products.)
+    auto process = [&](Stage& d, int n, Stage& f, int next) {
+        const int64_t ch = (int64_t)(base + n) * p.heads + head;
+        const bool more = next < n1;
+        const Buffers r = buffers(more ? next : n);
+        // (tile (value tile, n): row l16, columns 16 n + 4 g + j)
+        floatx4* kept = (floatx4*)(p.s0 + ch * vp * KP + 16 * (tile * KP + kc)) + lane;
+#pragma unroll
+        for (int m = 0; m < NB; ++m) kept[64 * m] = s[m];
+        floatx4 u[4];
         if constexpr (DELTA) {
             floatx4(*mine)[64] = part[n & 1][wave];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                floatx4 x = {0, 0, 0, 0};
+                if (more) load_w(f, r, i);
+                u[i] = floatx4{0, 0, 0, 0};
 #pragma unroll
-                for (int m = 0; m < NB; ++m) x = mfma4(w[i][m], s[m], x);
-                mine[i][lane] = x;
+                for (int m = 0; m < NB; ++m) u[i] = mfma4(d.w[i][m], s[m], u[i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine[i][lane] = u[i];
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 floatx4 x = part[n & 1][0][i][lane];
 #pragma unroll
                 for (int v = 1; v < 4; ++v) x += part[n & 1][v][i][lane];
-                u[i] -= x;
+                u[i] = d.u[i] - x;
             }
             // (the waves share the writing of U: 16 tokens each)
             floatx4 own = u[0];
 #pragma unroll
             for (int i = 1; i < 4; ++i) own = wave == i ? u[i] : own;
-            *(floatx4*)(p.u + (ch * vp + row) * C + 16 * wave + 4 * g) = own;
+            ((floatx4*)(p.u + (ch * vp + 16 * tile) * C))[wave * 64 + lane] = own;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = d.u[i];
         }
-        floatx4 ue[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ue[i] = u[i] * e[i];
+        for (int m = 0; m < NB; ++m) s[m] *= d.end;
+        if (more) load_end(f, next);
 #pragma unroll
-        for (int m = 0; m < NB; ++m) s[m] *= end;
-        // (the next chunk's loads go out behind this one's last use of each register)
+        for (int i = 0; i < 4; ++i) {
+            if (more) load_rest(f, r, i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int m = 0; m < NB; ++m) s[m] = mfma4(d.ke[i][m], u[i], s[m]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    Stage st[DEPTH];
 #pragma unroll
-            for (int m = 0; m < NB; ++m) s[m] = mfma4(k[i][m], ue[i], s[m]);
-        if (n + 1 < n1) load(n + 1);
+    for (int d = 0; d < DEPTH - 1; ++d)
+        if (n0 + d < n1) {
+            const Buffers r = buffers(n0 + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (DELTA) load_w(st[d], r, i);
+                load_rest(st[d], r, i);
+            }
+            load_end(st[d], n0 + d);
+        }
+    for (int n = n0; n < n1; n += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (n + d >= n1) break;
+            process(st[d], n + d, st[(d + DEPTH - 1) % DEPTH], n + d + DEPTH - 1);
+        }
     }
     if (row_live)
 #pragma unroll
@@ -356,8 +508,8 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
 }
 
 // ---- 3: the outputs of a chunk of a head
-template <int KP, int TYPE, bool DELTA>
-__global__ __launch_bounds__(256) void k_linear_out(LinearParams p) {
+template <int KP, int TYPE>
+__global__ __launch_bounds__(THREADS, KP == 256 ? 2 : 4) void k_linear_out(LinearParams p) {
     extern __shared__ __align__(16) float lds[];
     float* sq = lds;                    // [64][KP + 4]
     float* sk = sq + C * (KP + 4);      // [64][KP + 4], then M [64][LS]
@@ -369,28 +521,45 @@ __global__ __launch_bounds__(256) void k_linear_out(LinearParams p) {
     const int head = (int)(ch % p.heads), key_head = head / (p.heads / p.key_heads);
     const ChunkRange c = chunk_range(p, (int)(ch / p.heads));
     if (!c.count) return;
-    stage_rows<KP, TYPE>(p, c, p.q, p.q_token, key_head * p.q_head, sq);
-    stage_rows<KP, TYPE>(p, c, p.k, p.k_token, key_head * p.k_head, sk);
-    if (wave == 0) {
+    const int vp = (p.value_dim + 15) & ~15;
+    const floatx4* state = (const floatx4*)(p.s0 + ch * vp * KP) + lane;
+    const floatx4* writes = (const floatx4*)(p.u + ch * vp * C) + lane;
+    // value tile `wave` first: its state rows and writes are read ahead of everything
+    floatx4 s4[KP / 16], u[4];
+    auto load_tile = [&](int n) {
+#pragma unroll
+        for (int k = 0; k < KP / 16; ++k) s4[k] = state[(n * (KP / 16) + k) * 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = writes[(n * 4 + i) * 64];
+    };
+    {
+        StagedRows<KP, TYPE> q, k;
+        q.load(p, c, p.q, p.q_token, key_head * p.q_head);
+        k.load(p, c, p.k, p.k_token, key_head * p.k_head);
         const double sum = p.g[ch * C + lane];
-        s_g[lane] = sum;
-        s_from[lane] = expf((float)sum);
+        if (wave < vp / 16) load_tile(wave);
+        q.store(p, c, sq);
+        k.store(p, c, sk);
+        if (wave == 0) {
+            s_g[lane] = sum;
+            s_from[lane] = expf((float)sum);
+        }
     }
     __syncthreads();
-    floatx4 m[3];
+    floatx4 m[2];
 #pragma unroll
-    for (int n = 0; n < 3; ++n) {
+    for (int n = 0; n < 2; ++n) {
         int i, j;
-        if (wave + 4 * n >= 10) break;
-        triangle_tile(wave + 4 * n, i, j);
+        if (wave + 8 * n >= 10) break;
+        triangle_tile(wave + 8 * n, i, j);
         m[n] = tile_product<KP>(sq, sk, i, j);
     }
     __syncthreads();   // (M goes where K was)
 #pragma unroll
-    for (int n = 0; n < 3; ++n) {
+    for (int n = 0; n < 2; ++n) {
         int i, j;
-        if (wave + 4 * n >= 10) break;
-        triangle_tile(wave + 4 * n, i, j);
+        if (wave + 8 * n >= 10) break;
+        triangle_tile(wave + 8 * n, i, j);
         const int tj = 16 * j + l16;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -400,37 +569,27 @@ __global__ __launch_bounds__(256) void k_linear_out(LinearParams p) {
     }
     __syncthreads();
 
-    const int vp = (p.value_dim + 15) & ~15;
-    const float* state = p.s0 + ch * vp * KP;
     bool finite = true;
-    for (int n = wave; n < vp / 16; n += 4) {
+    for (int n = wave; n < vp / 16; n += 8) {
         const int row = 16 * n + l16;
         const bool row_live = row < p.value_dim;
+        if (n != wave) load_tile(n);
         floatx4 acc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = floatx4{0, 0, 0, 0};
-        const float* srow = state + (int64_t)row * KP + 4 * g;
-#pragma unroll 4
-        for (int k = 0; k < KP; k += 16) {
-            const floatx4 s4 = *(const floatx4*)(srow + k);
+        // (the query operands one step ahead, and no further: registers)
+        floatx4 a[2][4];
+        auto load_q = [&](int k) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                acc[i] = mfma4(*(const floatx4*)(sq + (16 * i + l16) * (KP + 4) + k + 4 * g), s4, acc[i]);
-        }
-        floatx4 u[4];
+            for (int i = 0; i < 4; ++i) a[k & 1][i] = *(const floatx4*)(sq + (16 * i + l16) * (KP + 4) + 16 * k + 4 * g);
+        };
+        load_q(0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (DELTA) {
-                u[i] = *(const floatx4*)(p.u + (ch * vp + row) * C + 16 * i + 4 * g);
-            } else {
+        for (int k = 0; k < KP / 16; ++k) {
+            if (k + 1 < KP / 16) load_q(k + 1);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int t = 16 * i + 4 * g + r;
-                    u[i][r] = t < c.count && row_live
-                                  ? load1<TYPE>(p.v, (int64_t)(c.first + t) * p.v_token + head * p.v_head + row)
-                                  : 0.0f;
-                }
-            }
+            for (int i = 0; i < 4; ++i) acc[i] = mfma4(a[k & 1][i], s4[k], acc[i]);
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -454,19 +613,15 @@ __global__ __launch_bounds__(256) void k_linear_out(LinearParams p) {
 template <int KP, int TYPE, bool DELTA>
 static hipError_t launch_prompt_of(const LinearParams& p, hipStream_t s) {
     const unsigned units = (unsigned)((int64_t)p.chunks * p.heads);
-    if constexpr (DELTA) {
-        constexpr int bytes = (C * (KP + 4) + C * LS + 4 * 16 * 20) * 4;
-        hipLaunchKernelGGL((k_linear_solve<KP, TYPE>), dim3(units), dim3(256), bytes, s, p);
-    } else {
-        hipLaunchKernelGGL(k_linear_gates, dim3((units + 3) / 4), dim3(256), 0, s, p);
-    }
+    constexpr int solve_bytes = (C * (KP + 4) + (DELTA ? C * LS + 4 * 16 * 20 : 0)) * 4;
+    hipLaunchKernelGGL((k_linear_solve<KP, TYPE, DELTA>), dim3(units), dim3(THREADS), solve_bytes, s, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const unsigned vt = (unsigned)(p.value_dim + 15) / 16, sh = (unsigned)(p.seqs * p.heads);
-    hipLaunchKernelGGL((k_linear_scan<KP, TYPE, DELTA>), dim3((sh + 7) / 8 * 8 * vt), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((k_linear_scan<KP, DELTA>), dim3((sh + 7) / 8 * 8 * vt), dim3(256), 0, s, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     constexpr int bytes = 2 * C * (KP + 4) * 4;
-    hipLaunchKernelGGL((k_linear_out<KP, TYPE, DELTA>), dim3(units), dim3(256), bytes, s, p);
+    hipLaunchKernelGGL((k_linear_out<KP, TYPE>), dim3(units), dim3(THREADS), bytes, s, p);
     return hipGetLastError();
 }
 

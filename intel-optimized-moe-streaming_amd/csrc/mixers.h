@@ -70,11 +70,12 @@ struct LinearParams {
     int* flags;
     // prompts: the workspace (a chunk of 64 tokens of a head at a time, indexed
     // [chunk - chunk0][head]), and the chunks of this pass
-    float* w;                   // [64 x KP] T diag(beta e^G) K            (delta rule)
-    float* u;                   // [VP x 64] T diag(beta) V, then the writes U, transposed (delta rule)
-    float* s0;                  // [VP x KP] the state before the chunk
+    float* w;                   // T diag(beta e^G) K (delta rule)
+    float* k_end;               // diag(e^(G_end - G)) K
+    float* u;                   // T diag(beta) V, then the writes U (without the delta rule V)
+    float* s0;                  // the state before the chunk
     double* g;                  // [64] running sums of the gate
-    float* e;                   // [64] e^(G_end - G), and [64] e^(G_end) from 64 on
+    float* e;                   // e^(G_end) at 64
     int chunk0, chunks;
 };
 
@@ -87,7 +88,7 @@ inline int linear_vp(int value_dim) { return (value_dim + 15) & ~15; }
 inline int64_t linear_chunks(int64_t tokens, int64_t seqs) { return tokens / LINEAR_CHUNK + seqs; }
 // floats of one chunk of one head
 inline int64_t linear_chunk_floats(int kp, int vp, bool delta) {
-    return (delta ? 64 * kp + 64 * vp : 0) + (int64_t)vp * kp + 128 + 128;
+    return (delta ? 2 : 1) * 64 * kp + 64 * vp + (int64_t)vp * kp + 128 + 128;
 }
 
 hipError_t launch_linear_step(const LinearParams& p, hipStream_t s);

@@ -2,6 +2,8 @@
 // include/moe_quant_hip.h): the paged key/value cache, attention over it and
 // linear attention.  They validate and enqueue only; nothing is allocated, and
 // no state is kept between calls.
+#include <initializer_list>
+
 #include "../../include/moe_quant_hip.h"
 #include "attend.h"
 #include "mixers.h"
@@ -72,7 +74,7 @@ bool attend_sizes(int tokens, int seqs, int single, int heads, int kv_heads, int
 // what both linear calls have to hold
 int check_linear(const void* q, const void* k, const void* v, int type, const float* gate, const float* state,
                  const void* out, int tokens, int seqs, int heads, int key_heads, int key_dim, int value_dim,
-                 const int32_t* flags) {
+                 const int32_t* flags, std::initializer_list<int64_t> strides) {
     if (!q || !k || !v || !gate || !state || !out || !flags) return ST_ARG;
     if (!row_type(type)) return ST_TYPE;
     if (tokens <= 0 || seqs <= 0 || heads <= 0 || key_heads <= 0 || heads % key_heads || heads > 4096) return ST_ARG;
@@ -81,6 +83,8 @@ int check_linear(const void* q, const void* k, const void* v, int type, const fl
     const int size = mix_bytes(type);
     if (unaligned(q, size) || unaligned(k, size) || unaligned(v, size) || unaligned(out, size)) return ST_ARG;
     if (unaligned(state, 16) || unaligned(gate, 4)) return ST_ARG;
+    for (int64_t stride : strides)
+        if (stride < 0 || stride > (int64_t)1 << 22) return ST_ARG;   // (a chunk's offsets are 32-bit)
     return tokens > 1 << 24 || seqs > 1 << 20 || (int64_t)seqs * heads >= (int64_t)1 << 24 ? ST_ARG : ST_OK;
 }
 
@@ -182,7 +186,8 @@ int mqh_linear_step(const void* q, int64_t q_token, int64_t q_head, const void* 
                     const void* v, int64_t v_token, int64_t v_head, int type, const float* beta, int64_t beta_token,
                     const float* gate, int64_t gate_token, float* state, void* out, int seqs, int heads, int key_heads,
                     int key_dim, int value_dim, int32_t* flags, void* stream) {
-    const int st = check_linear(q, k, v, type, gate, state, out, seqs, seqs, heads, key_heads, key_dim, value_dim, flags);
+    const int st = check_linear(q, k, v, type, gate, state, out, seqs, seqs, heads, key_heads, key_dim, value_dim, flags,
+                                {q_token, q_head, k_token, k_head, v_token, v_head, beta_token, gate_token});
     if (st) return st;
     LinearParams p{};
     p.q = q; p.k = k; p.v = v;
@@ -209,7 +214,8 @@ int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const voi
                        const float* gate, int64_t gate_token, float* state, void* out, const int32_t* starts,
                        int tokens, int seqs, int heads, int key_heads, int key_dim, int value_dim, void* workspace,
                        int64_t workspace_bytes, int32_t* flags, void* stream) {
-    const int st = check_linear(q, k, v, type, gate, state, out, tokens, seqs, heads, key_heads, key_dim, value_dim, flags);
+    const int st = check_linear(q, k, v, type, gate, state, out, tokens, seqs, heads, key_heads, key_dim, value_dim, flags,
+                                {q_token, q_head, k_token, k_head, v_token, v_head, beta_token, gate_token});
     if (st) return st;
     if (!starts && seqs != 1) return ST_ARG;
     const bool delta = beta != nullptr;
@@ -229,8 +235,9 @@ int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const voi
     p.g = (double*)workspace;
     p.e = (float*)workspace + units * 128;
     p.s0 = p.e + units * 128;
-    p.w = p.s0 + units * vp * kp;
-    p.u = p.w + units * 64 * kp;
+    p.k_end = p.s0 + units * vp * kp;
+    p.u = p.k_end + units * 64 * kp;
+    p.w = p.u + units * 64 * vp;
     const int64_t all = linear_chunks(tokens, seqs);
     for (int64_t at = 0; at < all; at += pass) {
         p.chunk0 = (int)at;
