@@ -13,9 +13,19 @@ constexpr float ATTEND_GROWTH = 8.0f;   // how far (in log2) a row's probabiliti
 hipError_t launch_attend(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_token(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_join(const AttendParams& p, hipStream_t s);
-// query rows of a workgroup of launch_attend; keys of one of its steps
-constexpr int ATTEND_ROWS = 128;
+// threads and query rows (32 a wave) of a workgroup of launch_attend, keys of one
+// of its steps, and the workgroups a CU holds
+constexpr int attend_threads(int dim) { return dim == 256 ? 512 : 256; }
+constexpr int attend_rows(int dim) { return attend_threads(dim) / 2; }
 constexpr int attend_step(int dim) { return dim == 256 ? 32 : 64; }
+constexpr int ATTEND_GROUP_MAX = 128;
+// Bytes of a row of K and V in LDS.  16 bytes of padding put the same piece of 16
+// keys into 16 places of a 256-byte bank line (the operand loads of K); 64 bytes put
+// the 64-byte pieces of 4 keys into its four quarters (the transposing loads of V).
+// Padding, not exchanged pieces: every load of a tile is then one register and an
+// offset.
+constexpr int attend_krow(int dim) { return 2 * dim + 16; }
+constexpr int attend_vrow(int dim) { return 2 * dim + 64; }
 // query heads a kv head may have in launch_attend_token; keys of a step
 constexpr int TOKEN_ROWS = 16;
 constexpr int TOKEN_STEP = 128;

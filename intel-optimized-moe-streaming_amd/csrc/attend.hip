@@ -7,8 +7,8 @@
 // in one pass over the keys with a running reference exponent m and sum; zeros
 // where p < 0.  Query head h reads kv head h / group.
 //
-// A workgroup takes 128 query rows of one kv head (all heads of its group, so a
-// key tile serves them all), four waves of 32 rows.  Both products are computed
+// A workgroup takes 128 query rows (256 at dim 256) of one kv head (all heads of
+// its group, so a key tile serves them all), 32 rows a wave.  Both products are computed
 // transposed, S^T = K Q^T and O^T = V^T P^T, on 32x32x16 matrix instructions: a
 // lane then holds scores of ONE query row, so maximum, exponential and sum need
 // no lane exchange, and the probabilities already lie in the second product's
@@ -18,10 +18,9 @@
 //
 // Keys go by in steps of 64 (32 at dim 256) through two LDS buffers: the next
 // step's rows are loaded into registers while this one is multiplied, converted
-// (8-bit codes to FP16) and stored behind it; one barrier a step.  16-byte pieces
-// of a row are exchanged by bits of the key so that neither the operand loads of
-// K (16 keys, one piece) nor the transposing loads of V (4 keys, four pieces)
-// meet in a bank.
+// (8-bit codes to FP16) and stored behind it; one barrier a step.  Rows are padded
+// in LDS so that neither the operand loads of K nor the transposing ones of V meet
+// in a bank.
 //
 // The reference exponent moves only when a score passes it by 2^8: the sums are
 // rescaled a few times a row instead of once a step.  8-bit caches: a key's scale
@@ -34,25 +33,31 @@
 // that do not see the key) and put back per channel at the end for the rows that
 // see them.
 
+#include <type_traits>
+
 #include "attend.h"
 
 namespace mqh {
 
 template <int DIM, int CACHE, int QT>
-__global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void k_attend(AttendParams p) {
+__global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams p) {
     using M = MixMath<CACHE>;
     typedef typename M::vec8 vec8;
     typedef typename M::vec4 vec4;
     constexpr bool Q8 = CACHE == MIX_Q8;
     constexpr int STEP = attend_step(DIM);
-    constexpr int ROW = DIM * 2;                       // bytes of an LDS row
-    constexpr int TILE = STEP * ROW;
+    constexpr int KROW = attend_krow(DIM), VROW = attend_vrow(DIM);
+    constexpr int KTILE = STEP * KROW, BUFFER = KTILE + STEP * VROW;
     constexpr int PIECES = Q8 ? DIM / 16 : DIM / 8;    // 16-byte pieces of a cache row
-    constexpr int PASS = 256 / PIECES;                 // keys of one load of every thread
+    constexpr int THREADS = attend_threads(DIM);
+    constexpr int PASS = THREADS / PIECES;             // keys of one load of every thread
     constexpr int LOADS = STEP / PASS;
     constexpr int KB = STEP / 32, DB = DIM / 32, KK = DIM / 16;
+    // at dim 256 the queries' second half stays in LDS: a wave then fits 256
+    // registers and a SIMD holds two
+    constexpr int KR = DIM == 256 ? KK / 2 : KK;
 
-    extern __shared__ __align__(16) uint8_t lds[];     // [2][K tile | V tile]
+    extern __shared__ __align__(16) uint8_t lds[];     // [2][K tile | V tile], then the waves' query operands
     __shared__ __align__(16) float s_kscale[2][STEP];  // 8-bit caches
     __shared__ __align__(16) float s_vlog[2][STEP];    // log2(vs)
     __shared__ __align__(16) float s_vinv[2][STEP];    // 1 / vs
@@ -95,15 +100,16 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void k_attend(AttendParams
     const int keys = max(before + i0 + n_tok, 0);          // keys any row sees
     const int full = before + i0 + 1;                      // keys every row sees
     const int n_steps = (keys + STEP - 1) / STEP;
-    const int per = (n_steps + p.splits - 1) / p.splits;
+    const int per = max((n_steps + p.splits - 1) / p.splits, 512 / STEP);   // (short sequences: fewer splits)
     const int step0 = split * per, step1 = min(step0 + per, n_steps);
     const bool wave_live = wave * 32 < n_tok * p.group;
 
     if (tid == 0) s_any_bad = 0;
-    for (int i = tid; i < 3 * DIM; i += 256) (&s_bad[0][0])[i] = 0x7fffffff;
+    for (int i = tid; i < 3 * DIM; i += THREADS) (&s_bad[0][0])[i] = 0x7fffffff;
 
     // ---- the query rows as operands: column `col`, d = 16 kk + 8 half + e
-    vec8 qf[KK];
+    vec8 qf[KR];
+    uintx4* q_rest = (uintx4*)(lds + 2 * BUFFER) + wave * (KK - KR) * 64 + lane;
     float q_scale = 1.0f;   // 8-bit caches with BF16 queries: what the FP16 operands were multiplied by, inverted
     {
         const int64_t at = (int64_t)(seq.first + i0 + (row_live ? r_tok : 0)) * p.q_token +
@@ -125,16 +131,23 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void k_attend(AttendParams
             const float down = __uint_as_float((uint32_t)(254 - e) << 23);
             q_scale = __uint_as_float((uint32_t)e << 23);
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
+            for (int kk = 0; kk < KK; ++kk) {
+                vec8 v;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    qf[kk][2 * i] = (_Float16)(__uint_as_float(raw[kk][i] << 16) * down);
-                    qf[kk][2 * i + 1] = (_Float16)(__uint_as_float(raw[kk][i] & 0xffff0000u) * down);
+                    v[2 * i] = (_Float16)(__uint_as_float(raw[kk][i] << 16) * down);
+                    v[2 * i + 1] = (_Float16)(__uint_as_float(raw[kk][i] & 0xffff0000u) * down);
                 }
+                if (kk < KR) qf[kk] = v;
+                else q_rest[(kk - KR) * 64] = __builtin_bit_cast(uintx4, v);
+            }
         } else {
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
-                qf[kk] = bits_as<vec8>(load_any<uintx4>((const uint16_t*)p.q + at + 16 * kk + 8 * half));
+            for (int kk = 0; kk < KK; ++kk) {
+                const uintx4 v = load_any<uintx4>((const uint16_t*)p.q + at + 16 * kk + 8 * half);
+                if (kk < KR) qf[kk] = bits_as<vec8>(v);
+                else q_rest[(kk - KR) * 64] = v;
+            }
         }
     }
 
@@ -183,26 +196,25 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void k_attend(AttendParams
     auto store_step = [&](int step, int buf) {
         const int base = step * STEP;
         const bool edge = base + STEP > full;
-        uint8_t* kt = lds + buf * 2 * TILE;
-        uint8_t* vt = kt + TILE;
+        uint8_t* kt = lds + buf * BUFFER;
+        uint8_t* vt = kt + KTILE;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int key = key_in + PASS * i;
-            const int sw = swizzle<DIM>(key);
             if constexpr (Q8) {
                 // (codes are finite, and a key past the end has probability 0)
                 const uintx2 a = codes_to_half(kr[i][0]), b2 = codes_to_half(kr[i][1]);
                 const uintx2 c = codes_to_half(kr[i][2]), d = codes_to_half(kr[i][3]);
                 const uintx2 e = codes_to_half(vr[i][0]), f = codes_to_half(vr[i][1]);
                 const uintx2 g = codes_to_half(vr[i][2]), h = codes_to_half(vr[i][3]);
-                const int o0 = key * ROW + ((2 * piece) ^ sw) * 16, o1 = key * ROW + ((2 * piece + 1) ^ sw) * 16;
-                *(uintx4*)(kt + o0) = uintx4{a[0], a[1], b2[0], b2[1]};
-                *(uintx4*)(kt + o1) = uintx4{c[0], c[1], d[0], d[1]};
-                *(uintx4*)(vt + o0) = uintx4{e[0], e[1], f[0], f[1]};
-                *(uintx4*)(vt + o1) = uintx4{g[0], g[1], h[0], h[1]};
+                uint8_t* ko = kt + key * KROW + piece * 32;
+                uint8_t* vo = vt + key * VROW + piece * 32;
+                *(uintx4*)ko = uintx4{a[0], a[1], b2[0], b2[1]};
+                *(uintx4*)(ko + 16) = uintx4{c[0], c[1], d[0], d[1]};
+                *(uintx4*)vo = uintx4{e[0], e[1], f[0], f[1]};
+                *(uintx4*)(vo + 16) = uintx4{g[0], g[1], h[0], h[1]};
             } else {
-                const int o = key * ROW + (piece ^ sw) * 16;
-                *(uintx4*)(kt + o) = kr[i];
+                *(uintx4*)(kt + key * KROW + piece * 16) = kr[i];
                 if (edge) {
                     const bool there = base + key < keys;
 #pragma unroll
@@ -221,7 +233,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void k_attend(AttendParams
                         vr[i][w] = x;
                     }
                 }
-                *(uintx4*)(vt + o) = vr[i];
+                *(uintx4*)(vt + key * VROW + piece * 16) = vr[i];
             }
         }
         if constexpr (Q8) {
@@ -248,50 +260,60 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void k_attend(AttendParams
     if (step0 < step1) store_step(step0, 0);
     __syncthreads();
 
-    for (int step = step0; step < step1; ++step) {
-        const int buf = (step - step0) & 1;
+    // where this lane points for the transposing loads: key 4 half + i / 4, channels
+    // 16 (lane / 16 % 2) + 4 (i % 4) of 32
+    const int v_at = (4 * half + ((lane & 15) >> 2)) * VROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+    // Operand addresses of a buffer: with the buffer a constant they are offsets
+    auto compute = [&](int step, auto which) {
+        constexpr int buf = decltype(which)::value;
         const bool more = step + 1 < step1;
         if (more) load_step(step + 1);
         if (wave_live) {
-            const uint8_t* kt = lds + buf * 2 * TILE;
-            const uint8_t* vt = kt + TILE;
+            const uint8_t* kt = lds + buf * BUFFER + col * KROW + half * 16;
+            const uint8_t* vt = lds + buf * BUFFER + KTILE + v_at;
             // S^T = K Q^T
             floatx16 s[KB];
 #pragma unroll
             for (int j = 0; j < KB; ++j) {
                 s[j] = floatx16{0};
-                const uint8_t* kp = kt + (32 * j + col) * ROW;
-                const int sw = swizzle<DIM>(col);
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
-                    const vec8 a = bits_as<vec8>(*(const uintx4*)(kp + ((2 * kk + half) ^ sw) * 16));
-                    s[j] = M::mfma32(a, qf[kk], s[j]);
+                    const vec8 a = bits_as<vec8>(*(const uintx4*)(kt + 32 * j * KROW + 32 * kk));
+                    const vec8 q = kk < KR ? qf[kk < KR ? kk : 0] : bits_as<vec8>(q_rest[(kk - KR) * 64]);
+                    s[j] = M::mfma32(a, q, s[j]);
                 }
             }
-            // scores in log2 (8-bit caches: with log2(vs))
+            // 8-bit caches: scores in log2 with the keys' scales and log2(vs) (else the
+            // softmax scale goes into the exponential's argument)
             const int base = step * STEP;
-            const bool edge = base + STEP > full;
+            const float c = Q8 ? 1.0f : p.scale_log2;
+            if constexpr (Q8) {
+#pragma unroll
+                for (int j = 0; j < KB; ++j)
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4) {
+                        const int k0 = 32 * j + 8 * r4 + 4 * half;
+                        const floatx4 ks4 = *(const floatx4*)&s_kscale[buf][k0], vl4 = *(const floatx4*)&s_vlog[buf][k0];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float t = QT == MIX_BF16 ? s[j][4 * r4 + e] * q_scale : s[j][4 * r4 + e];
+                            s[j][4 * r4 + e] = fmaf(t, ks4[e], vl4[e]);
+                        }
+                    }
+            }
+            if (base + STEP > full) {
+#pragma unroll
+                for (int j = 0; j < KB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (base + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3) > seen) s[j][r] = -INFINITY;
+            }
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < KB; ++j)
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    const int k0 = 32 * j + 8 * r4 + 4 * half;
-                    floatx4 ks4, vl4;
-                    if constexpr (Q8) {
-                        ks4 = *(const floatx4*)&s_kscale[buf][k0];
-                        vl4 = *(const floatx4*)&s_vlog[buf][k0];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float t = s[j][4 * r4 + e];
-                        if constexpr (Q8) t = fmaf(t * ks4[e], q_scale, vl4[e]);
-                        else t = t * p.scale_log2;
-                        if (edge && base + k0 + e > seen) t = -INFINITY;
-                        s[j][4 * r4 + e] = t;
-                        mx = fmaxf(mx, t);
-                    }
-                }
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
+            mx *= c;
             if (__any(mx > m + ATTEND_GROWTH)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
                 const float mn = fmaxf(m, mx);
@@ -314,22 +336,17 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void k_attend(AttendParams
                     if constexpr (Q8) vi4 = *(const floatx4*)&s_vinv[buf][k0];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float pr = __builtin_amdgcn_exp2f(s[t / 2][8 * (t & 1) + 4 * e4 + e] - ref);
+                        const float pr = __builtin_amdgcn_exp2f(fmaf(s[t / 2][8 * (t & 1) + 4 * e4 + e], c, -ref));
                         if constexpr (Q8) l = fmaf(pr, vi4[e], l);
                         else l += pr;
                         pb[4 * e4 + e] = (typename M::elem)pr;
                     }
                 }
                 // O^T += V^T P^T
-                const int i = lane & 15, dsub = ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
-                const int ka = 16 * t + 4 * half + (i >> 2), kb = ka + 8;
-                const uint8_t* pa = vt + ka * ROW + (i & 1) * 8;
-                const uint8_t* pc = vt + kb * ROW + (i & 1) * 8;
-                const int swa = swizzle<DIM>(ka), swb = swizzle<DIM>(kb);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    const vec4 lo = lds_transposed<vec4>(pa + ((4 * d + dsub) ^ swa) * 16);
-                    const vec4 hi = lds_transposed<vec4>(pc + ((4 * d + dsub) ^ swb) * 16);
+                    const vec4 lo = lds_transposed<vec4>(vt + 16 * t * VROW + 64 * d);
+                    const vec4 hi = lds_transposed<vec4>(vt + (16 * t + 8) * VROW + 64 * d);
                     const vec8 va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                     o[d] = M::mfma32(va, pb, o[d]);
                 }
@@ -337,6 +354,10 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void k_attend(AttendParams
         }
         if (more) store_step(step + 1, buf ^ 1);
         __syncthreads();
+    };
+    for (int step = step0; step < step1; step += 2) {
+        compute(step, std::integral_constant<int, 0>());
+        if (step + 1 < step1) compute(step + 1, std::integral_constant<int, 1>());
     }
 
     // ---- the rows out: this lane's channels 32 d + 8 r4 + 4 half + e
@@ -437,9 +458,10 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendParams p) {
 
 template <int DIM, int CACHE, int QT>
 static hipError_t launch_attend_of(const AttendParams& p, hipStream_t s) {
-    constexpr int bytes = 4 * attend_step(DIM) * DIM * 2;
+    constexpr int threads = attend_threads(DIM);
+    constexpr int bytes = 2 * attend_step(DIM) * (attend_krow(DIM) + attend_vrow(DIM)) + (DIM == 256 ? threads / 64 * 8 * 1024 : 0);
     hipLaunchKernelGGL((k_attend<DIM, CACHE, QT>), dim3((unsigned)(p.tiles * p.kv_heads), (unsigned)p.splits),
-                       dim3(256), bytes, s, p);
+                       dim3(threads), bytes, s, p);
     return hipGetLastError();
 }
 

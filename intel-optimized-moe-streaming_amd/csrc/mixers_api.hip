@@ -36,20 +36,21 @@ int check_cache(const void* kc, const void* vc, const float* ks, const float* vs
 }
 
 // Workgroups of the many-row kernel, their query tokens, and the splits of
-// their keys: as many as give every CU two workgroups, none of under 512 keys
-// (below that the splits' sums cost more traffic than the keys).
+// their keys: enough for four workgroups a CU (what is left over when the longest
+// end), none of under 512 keys (below that the splits' sums cost more traffic than
+// the keys).
 struct AttendPlan {
     bool token;
     int tile_tokens, tiles, splits;
 };
 
-AttendPlan attend_plan(int tokens, int seqs, bool single, int heads, int kv_heads, int64_t most_keys) {
+AttendPlan attend_plan(int tokens, int seqs, bool single, int heads, int kv_heads, int dim, int64_t most_keys) {
     AttendPlan a;
     const int group = heads / kv_heads;
     a.token = single && group <= TOKEN_ROWS;
-    a.tile_tokens = ATTEND_ROWS / group;
+    a.tile_tokens = attend_rows(dim) / group;
     a.tiles = a.token ? seqs : tokens / a.tile_tokens + seqs;
-    const int64_t groups = (int64_t)a.tiles * kv_heads, want = a.token ? 1024 : 512, least = a.token ? 256 : 512;
+    const int64_t groups = (int64_t)a.tiles * kv_heads, want = a.token ? 1024 : dim == 256 ? 512 : 1024, least = a.token ? 256 : 512;
     int64_t splits = (want + groups - 1) / groups;
     splits = std::min(splits, std::max<int64_t>(1, most_keys / least));
     a.splits = (int)std::min<int64_t>(splits, 128);
@@ -64,7 +65,7 @@ int64_t attend_workspace(const AttendPlan& a, int tokens, int heads, int dim) {
 
 // sizes both the query call and the attention call have to hold
 bool attend_sizes(int tokens, int seqs, int single, int heads, int kv_heads, int dim, int64_t most_keys) {
-    if (tokens <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > ATTEND_ROWS)
+    if (tokens <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > ATTEND_GROUP_MAX)
         return false;
     if (single && tokens != seqs) return false;
     if (tokens > 1 << 24 || seqs > 1 << 20 || most_keys <= 0 || most_keys > 1 << 30) return false;
@@ -144,7 +145,7 @@ int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc
 int64_t mqh_attend_workspace_bytes(int tokens, int seqs, int single, int heads, int kv_heads, int dim,
                                    int64_t most_keys) {
     if (!attend_sizes(tokens, seqs, single, heads, kv_heads, dim, most_keys)) return ST_ARG;
-    return attend_workspace(attend_plan(tokens, seqs, single, heads, kv_heads, most_keys), tokens, heads, dim);
+    return attend_workspace(attend_plan(tokens, seqs, single, heads, kv_heads, dim, most_keys), tokens, heads, dim);
 }
 
 int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int tokens, const int32_t* starts,
@@ -162,7 +163,7 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
     const int64_t most = (int64_t)table_cols * page_size;
     if (!attend_sizes(tokens, seqs, single, heads, kv_heads, dim, most)) return ST_ARG;
     if (!(scale > 0.0f) || !(scale < INFINITY) || unaligned(q, 2) || unaligned(out, 16)) return ST_ARG;
-    const AttendPlan a = attend_plan(tokens, seqs, single, heads, kv_heads, most);
+    const AttendPlan a = attend_plan(tokens, seqs, single, heads, kv_heads, dim, most);
     if (workspace_bytes < attend_workspace(a, tokens, heads, dim)) return ST_WORKSPACE;
     if (a.splits > 1 && (!workspace || unaligned(workspace, 256))) return ST_ARG;
     AttendParams p{};
