@@ -414,45 +414,63 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
 }
 
 // The splits of a row joined: the sums brought to the largest reference exponent
-// and added in split order.  A wave takes a row, 4 channels a lane.
+// and added in split order.  A wave takes a row: lane i first reads split i's
+// exponent and sum (one round trip for all of them), then every lane its channels
+// of eight splits at a time.
 template <int DIM, int QT>
 __global__ __launch_bounds__(256) void k_attend_join(AttendParams p) {
-    constexpr int LANES = DIM / 4;
+    constexpr int N = DIM / 64;   // channels of a lane
+    typedef float vec __attribute__((ext_vector_type(N)));
     const int64_t rows = (int64_t)p.tokens * p.heads;
-    const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const int c = (threadIdx.x % LANES) * 4;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
     if (row >= rows) return;
     if (p.starts) {   // rows of no sequence stay as they were
         const int t = (int)(row / p.heads);
         if (t < p.starts[0] || t >= p.starts[p.seqs]) return;
     }
-    float top = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[2 * (s * rows + row)]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    floatx4 sum = {0, 0, 0, 0};
-    float l = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-        const int64_t at = s * rows + row;
-        const float ms = p.part_ml[2 * at];
-        if (ms == -INFINITY && p.part_ml[2 * at + 1] == 0.0f) continue;   // a split without keys for this row
-        const float w = __builtin_amdgcn_exp2f(ms - ref);
-        const floatx4 v = *(const floatx4*)(p.part_o + at * DIM + c);
-        l = fmaf(w, p.part_ml[2 * at + 1], l);
+    const float2* ml = (const float2*)p.part_ml + row;
+    const float2 none = {-INFINITY, 0.0f};
+    const float2 a = lane < p.splits ? ml[lane * rows] : none, b = lane + 64 < p.splits ? ml[(lane + 64) * rows] : none;
+    float top = fmaxf(a.x, b.x);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = fmaf(w, v[e], sum[e]);
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    // (a split without keys for this row weighs nothing, whatever lies in its place)
+    const float wa = a.x == -INFINITY && a.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(a.x - ref);
+    const float wb = b.x == -INFINITY && b.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(b.x - ref);
+    float l = fmaf(wa, a.y, wb * b.y);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+
+    const vec* part = (const vec*)(p.part_o + row * DIM) + lane;
+    const int64_t step = rows * 64;   // of a split, in vecs
+    vec sum = {};
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {
+        vec v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = part[min(s0 + i, p.splits - 1) * step];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int s = s0 + i;
+            const float w = __shfl(s < 64 ? wa : wb, s & 63);
+            if (s < p.splits && w != 0.0f)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[e] = fmaf(w, v[i][e], sum[e]);
+        }
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     bool finite = true;
+    uint16_t* out = (uint16_t*)p.out + row * DIM + lane * N;
+    uint16_t y[N];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        sum[e] *= inv;
-        finite &= __builtin_isfinite(sum[e]);
+    for (int e = 0; e < N; ++e) {
+        const float x = sum[e] * inv;
+        finite &= __builtin_isfinite(x);
+        if constexpr (QT == MIX_F16) y[e] = __builtin_bit_cast(uint16_t, (_Float16)x);
+        else y[e] = __builtin_bit_cast(uint16_t, (__bf16)x);
     }
-    uint16_t* out = (uint16_t*)p.out + row * DIM + c;
-    if constexpr (QT == MIX_F16)
-        *(half4*)out = half4{(_Float16)sum[0], (_Float16)sum[1], (_Float16)sum[2], (_Float16)sum[3]};
-    else
-        *(bfloat4*)out = bfloat4{(__bf16)sum[0], (__bf16)sum[1], (__bf16)sum[2], (__bf16)sum[3]};
+    __builtin_memcpy(__builtin_assume_aligned(out, 2 * N), y, 2 * N);
     if (!finite) atomicOr(&p.flags[FLAG_NONFINITE], 1);
 }
 
@@ -484,8 +502,7 @@ hipError_t launch_attend(const AttendParams& p, hipStream_t s) {
 
 template <int DIM>
 static hipError_t launch_join_dim(const AttendParams& p, hipStream_t s) {
-    constexpr int ROWS = 256 / (DIM / 4);
-    const dim3 grid((unsigned)(((int64_t)p.tokens * p.heads + ROWS - 1) / ROWS));
+    const dim3 grid((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4));
     if (p.q_type == MIX_F16) hipLaunchKernelGGL((k_attend_join<DIM, MIX_F16>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((k_attend_join<DIM, MIX_BF16>), grid, dim3(256), 0, s, p);
     return hipGetLastError();

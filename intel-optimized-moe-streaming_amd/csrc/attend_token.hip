@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
     const SeqRange seq = sequence_range(p, b, tid == 0);
     const int keys = seq.length;
     const int blocks = (keys + 31) >> 5;
-    const int per = (blocks + p.splits - 1) / p.splits;
+    const int per = max((blocks + p.splits - 1) / p.splits, 8);   // (short sequences: fewer splits)
     const int block0 = split * per, block1 = min(block0 + per, blocks);
     const int page_mask = (1 << p.page_shift) - 1;
 

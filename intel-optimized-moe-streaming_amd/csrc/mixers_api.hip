@@ -50,7 +50,7 @@ AttendPlan attend_plan(int tokens, int seqs, bool single, int heads, int kv_head
     a.token = single && group <= TOKEN_ROWS;
     a.tile_tokens = attend_rows(dim) / group;
     a.tiles = a.token ? seqs : tokens / a.tile_tokens + seqs;
-    const int64_t groups = (int64_t)a.tiles * kv_heads, want = a.token ? 1024 : dim == 256 ? 512 : 1024, least = a.token ? 256 : 512;
+    const int64_t groups = (int64_t)a.tiles * kv_heads, want = a.token ? 4096 : dim == 256 ? 512 : 1024, least = a.token ? 256 : 512;
     int64_t splits = (want + groups - 1) / groups;
     splits = std::min(splits, std::max<int64_t>(1, most_keys / least));
     a.splits = (int)std::min<int64_t>(splits, 128);

@@ -40,50 +40,58 @@ def _attend_bytes(lib, tokens, seqs, single, heads, kv_heads, dim, most):
     return int(lib.mqh_attend_workspace_bytes(tokens, seqs, single, heads, kv_heads, dim, most))
 
 
-def check_rows(t, shape, types, device, what):
-    """A tensor of rows as the kernels take it: shape, a type of `types`, on
-    `device`, its last dimension contiguous (other strides are free)."""
-    if tuple(t.shape) != tuple(shape):
+def check_rows(t, shape, types, index, what):
+    """The strides of a tensor of rows as the kernels take it: of `shape` and a type
+    of `types`, on CUDA device `index`, its last dimension contiguous (other strides
+    are free).  (A small call's time is the host's: one test where all is well.)"""
+    strides = t.stride()
+    if t.shape == shape and t.dtype in types and t.get_device() == index and not t.requires_grad and (
+            strides[-1] == 1 or shape[-1] == 1):
+        return strides
+    if t.shape != shape:
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype not in types:
         raise ValueError(f"{what} is {t.dtype}, expected one of {[str(d) for d in types]}")
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
+    if strides[-1] != 1 and shape[-1] != 1:
         raise ValueError(f"{what} must be contiguous in its last dimension")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, expected {device}")
-    if t.requires_grad:
-        raise ValueError(f"{what} requires grad; these calls have no backward")
+    if t.get_device() != index:
+        raise ValueError(f"{what} is on {t.device}, expected {_device_name(index)}")
+    raise ValueError(f"{what} requires grad; these calls have no backward")
 
 
-def check_index(t, shape, dtype, device, what):
-    """An index tensor: exact shape and type, contiguous, on `device`."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+def _device_name(index):
+    return f"cuda:{index}" if index >= 0 else "cpu"
+
+
+def check_index(t, shape, dtype, index, what):
+    """An index tensor: exact shape and type, contiguous, on CUDA device `index`."""
+    if t.shape == shape and t.dtype == dtype and t.get_device() == index and t.is_contiguous():
+        return
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, expected {device}")
+    raise ValueError(f"{what} is on {t.device}, expected {_device_name(index)}")
 
 
 class OnStream:
-    """The device and stream of a call: makes the device current and, where a
-    stream is given, has the call's tensors allocated on it."""
+    """Runs a call on a device: with it current and the handle of its current
+    stream, or of the stream given, which the call's tensors are then allocated on."""
 
     def __init__(self, device):
         import torch
 
-        self.device = device
         self.index = device.index
         self._torch = torch
+        self._current = torch.cuda.current_device
         self._stream_of = _lib.stream_accessor()
 
-    def __call__(self, stream, call):
-        torch = self._torch
+    def __call__(self, stream, call, *args):
         if stream is not None:
-            with torch.cuda.stream(stream):
-                return call(stream.cuda_stream)
-        if torch.cuda.current_device() != self.index:
-            with torch.cuda.device(self.index):
-                return call(self._stream_of(self.index))
-        return call(self._stream_of(self.index))
+            with self._torch.cuda.stream(stream):
+                return call(stream.cuda_stream, *args)
+        if self._current() != self.index:
+            with self._torch.cuda.device(self.index):
+                return call(self._stream_of(self.index), *args)
+        return call(self._stream_of(self.index), *args)
 
 
 class PagedCache:
@@ -129,11 +137,15 @@ class PagedCache:
         self.device = k.device
         self.lib = _lib.load()
         self._run = OnStream(k.device)
+        self._index = k.device.index
         self._types = _types()
-        self._cache_type = types[k.dtype]
+        self._empty, self._int32, self._int64, self._uint8 = torch.empty, torch.int32, torch.int64, torch.uint8
+        int8 = k.dtype == torch.int8
+        self._q_types = (torch.float16, torch.bfloat16) if int8 else (k.dtype,)
+        self._read_type = torch.float32 if int8 else k.dtype
         self._flags = torch.zeros(64, dtype=torch.int32, device=k.device)
         scales = (k_scale.data_ptr(), v_scale.data_ptr()) if len(held) == 4 else (0, 0)
-        self._words = (k.data_ptr(), v.data_ptr(), *scales, self._cache_type, pages, kv_heads, page_size, dim)
+        self._words = (k.data_ptr(), v.data_ptr(), *scales, types[k.dtype], pages, kv_heads, page_size, dim)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dtype=None, device="cuda"):
@@ -161,51 +173,45 @@ class PagedCache:
         round(x / s), s = max|x| / 127 of the row.  A value that is not finite (or
         that an FP16 cache cannot hold) latches -4; in an int8 cache its row then
         reads back as NaN."""
-        import torch
-
-        n = slots.shape[0] if slots.dim() == 1 else -1
-        check_index(slots, (n,), torch.int64, self.device, "slots")
+        n = self._tokens(slots)
         shape = (n, self.kv_heads, self.head_dim)
-        check_rows(k, shape, self._types, self.device, "k")
-        check_rows(v, shape, (k.dtype,), self.device, "v")
-        if n == 0:
-            return
-        kt, kh, _ = k.stride()
-        vt, vh, _ = v.stride()
+        kt, kh, _ = check_rows(k, shape, self._types, self._index, "k")
+        vt, vh, _ = check_rows(v, shape, (k.dtype,), self._index, "v")
+        if n:
+            self._run(stream, self._write, (k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, self._types[k.dtype],
+                                            slots.data_ptr(), n, *self._words, self._flags.data_ptr()))
 
-        def call(handle):
-            return self.lib.mqh_kv_write_words(_WRITE_WORDS.pack(
-                k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, self._types[k.dtype], slots.data_ptr(), n, *self._words,
-                self._flags.data_ptr(), handle))
+    def _write(self, handle, words):
+        rc = self.lib.mqh_kv_write_words(_WRITE_WORDS.pack(*words, handle))
+        if rc:
+            _lib.check(rc, "mqh_kv_write")
 
-        _lib.check(self._run(stream, call), "mqh_kv_write")
+    def _tokens(self, slots):
+        n = slots.shape[0] if slots.dim() == 1 else -1
+        check_index(slots, (n,), self._int64, self._index, "slots")
+        return n
 
     def read(self, slots, dtype=None, *, stream=None):
         """(k, v) [tokens, kv_heads, head_dim] at `slots` [tokens] int64 as `dtype`
         (the cache's own, FP32 for int8); rows of negative slots are zeros, so are
         those past the cache, which latch -9."""
-        import torch
-
-        n = slots.shape[0] if slots.dim() == 1 else -1
-        check_index(slots, (n,), torch.int64, self.device, "slots")
+        n = self._tokens(slots)
         if dtype is None:
-            dtype = torch.float32 if self._cache_type == Q8 else self.k.dtype
+            dtype = self._read_type
         if dtype not in self._types:
             raise ValueError(f"rows are read as FP32, FP16 or BF16, not {dtype}")
-        shape = (n, self.kv_heads, self.head_dim)
+        return self._run(stream, self._read, slots, n, dtype)
 
-        def call(handle):
-            k = torch.empty(shape, dtype=dtype, device=self.device)
-            v = torch.empty(shape, dtype=dtype, device=self.device)
-            rc = 0
-            if n:
-                rc = self.lib.mqh_kv_read_words(_READ_WORDS.pack(
-                    slots.data_ptr(), n, *self._words, k.data_ptr(), v.data_ptr(), self._types[dtype],
-                    self._flags.data_ptr(), handle))
-            _lib.check(rc, "mqh_kv_read")
-            return k, v
-
-        return self._run(stream, call)
+    def _read(self, handle, slots, n, dtype):
+        rows = self._empty((2, n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        k, v = rows.unbind()
+        if n:
+            rc = self.lib.mqh_kv_read_words(_READ_WORDS.pack(
+                slots.data_ptr(), n, *self._words, k.data_ptr(), v.data_ptr(), self._types[dtype],
+                self._flags.data_ptr(), handle))
+            if rc:
+                _lib.check(rc, "mqh_kv_read")
+        return k, v
 
     def attend(self, q, page_table, lengths, starts=None, *, scale=None, out=None, stream=None):
         """Attention of new tokens, whose rows are already written, over the cache.
@@ -222,55 +228,53 @@ class PagedCache:
         (default head_dim ** -0.5).  Returns out [tokens, heads, head_dim] of q's
         type.  Page numbers, lengths and starts out of range latch -9 (the
         rows concerned are then undefined), outputs that are not finite -4."""
-        import torch
-
         if q.dim() != 3 or page_table.dim() != 2:
             raise ValueError("q must be [tokens, heads, head_dim] and page_table [sequences, columns]")
-        tokens, heads, _ = q.shape
+        tokens, heads, _ = shape = q.shape
         seqs, cols = page_table.shape
-        types = (torch.float16, torch.bfloat16) if self._cache_type == Q8 else (self.k.dtype,)
-        check_rows(q, (tokens, heads, self.head_dim), types, self.device, "q")
+        index = self._index
+        qt, qh, _ = check_rows(q, (tokens, heads, self.head_dim), self._q_types, index, "q")
         group = heads // self.kv_heads
         if group * self.kv_heads != heads or not 1 <= group <= 128:
             raise ValueError(f"heads must be 1 to 128 times the cache's {self.kv_heads}, got {heads}")
-        if page_table.dtype != torch.int32 or page_table.device != self.device or (
-                cols and page_table.stride(1) != 1 and cols != 1) or (seqs > 1 and page_table.stride(0) < cols):
+        row, step = page_table.stride()
+        if page_table.dtype != self._int32 or page_table.get_device() != index or (step != 1 and cols > 1) or (
+                row < cols and seqs > 1):
             raise ValueError(f"page_table must be int32 rows on {self.device}")
-        check_index(lengths, (seqs,), torch.int32, self.device, "lengths")
+        check_index(lengths, (seqs,), self._int32, index, "lengths")
         if starts is not None:
-            check_index(starts, (seqs + 1,), torch.int32, self.device, "starts")
+            check_index(starts, (seqs + 1,), self._int32, index, "starts")
         elif tokens != seqs:
             raise ValueError("without starts there is one query a sequence")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
         if not 0 < scale < float("inf"):
             raise ValueError("scale must be positive and finite")
         if out is not None:
-            check_rows(out, q.shape, (q.dtype,), self.device, "out")
+            check_rows(out, shape, (q.dtype,), index, "out")
             if not out.is_contiguous() or out.data_ptr() % 16:
                 raise ValueError("out must be contiguous and 16-byte aligned")
-        most = cols * self.page_size
         need = 0
-        if tokens and seqs and cols:
-            need = _attend_bytes(self.lib, tokens, seqs, int(starts is None), heads, self.kv_heads, self.head_dim, most)
-            if need < 0:
-                _lib.check(need, "mqh_attend_workspace_bytes")
-        qt, qh, _ = q.stride()
-
-        def call(handle):
-            y = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype, device=self.device) if out is None else out
-            if tokens == 0 or seqs == 0:
-                return y
+        if tokens and seqs:
             if cols == 0:
                 raise ValueError("page_table has no columns")
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            _lib.check(self.lib.mqh_attend_words(_ATTEND_WORDS.pack(
-                q.data_ptr(), qt, qh, self._types[q.dtype], tokens, starts.data_ptr() if starts is not None else 0,
-                seqs, heads, *self._words, page_table.data_ptr(), page_table.stride(0) if seqs > 1 else cols, cols,
-                lengths.data_ptr(), scale, y.data_ptr(), ws.data_ptr() if need else 0, need, self._flags.data_ptr(),
-                handle)), "mqh_attend")
-            return y
+            need = _attend_bytes(self.lib, tokens, seqs, int(starts is None), heads, self.kv_heads, self.head_dim,
+                                 cols * self.page_size)
+            if need < 0:
+                _lib.check(need, "mqh_attend_workspace_bytes")
+        return self._run(stream, self._attend, q, out, need, (
+            q.data_ptr(), qt, qh, self._types[q.dtype], tokens, starts.data_ptr() if starts is not None else 0, seqs,
+            heads, *self._words, page_table.data_ptr(), row if seqs > 1 else cols, cols, lengths.data_ptr(), scale))
 
-        return self._run(stream, call)
+    def _attend(self, handle, q, out, need, words):
+        if out is None:
+            out = self._empty(q.shape, dtype=q.dtype, device=self.device)
+        if words[4] and words[6]:
+            ws = self._empty(need, dtype=self._uint8, device=self.device) if need else None
+            rc = self.lib.mqh_attend_words(_ATTEND_WORDS.pack(
+                *words, out.data_ptr(), ws.data_ptr() if need else 0, need, self._flags.data_ptr(), handle))
+            if rc:
+                _lib.check(rc, "mqh_attend")
+        return out
 
     def status(self, stream=None) -> int:
         """Synchronizes; 0, -4 (a value that is not finite) or -9 (a slot, page,

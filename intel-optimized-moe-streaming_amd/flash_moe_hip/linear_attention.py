@@ -39,34 +39,36 @@ def check_dims(key_dim: int, value_dim: int):
                          f"got {key_dim} and {value_dim}")
 
 
-def _inputs(state, n, q, k, v, beta, gate):
+def _inputs(state, n, q, k, v, beta, gate, out):
     """Check one call's rows against the states' shape; the shared argument words."""
-    import torch
-
     _, heads, dv, dk = state.shape
-    device = state.device
+    index, types = state.get_device(), _types()
     key_heads = q.shape[1] if q.dim() == 3 else -1
     if key_heads < 1 or heads % key_heads:
         raise ValueError(f"q must be [tokens, key_heads, key_dim] with key_heads a divisor of {heads}")
-    check_rows(v, (n, heads, dv), _types(), device, "v")
-    check_rows(q, (n, key_heads, dk), (v.dtype,), device, "q")
-    check_rows(k, (n, key_heads, dk), (v.dtype,), device, "k")
-    for t, what in ((beta, "beta"), (gate, "gate")):
-        if t is not None:
-            check_rows(t, (n, heads), (torch.float32,), device, what)
-    qt, qh, _ = q.stride()
-    kt, kh, _ = k.stride()
-    vt, vh, _ = v.stride()
-    return (q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _types()[v.dtype],
-            beta.data_ptr() if beta is not None else 0, beta.stride(0) if beta is not None else 0,
-            gate.data_ptr(), gate.stride(0), state.data_ptr()), key_heads
-
-
-def _out(out, n, like, heads, dv, device):
+    rows = (n, heads, dv)
+    vt, vh, _ = check_rows(v, rows, types, index, "v")
+    like = (v.dtype,)
+    qt, qh, _ = check_rows(q, (n, key_heads, dk), like, index, "q")
+    kt, kh, _ = check_rows(k, (n, key_heads, dk), like, index, "k")
+    gt, _ = check_rows(gate, (n, heads), _FP32(), index, "gate")
+    bp = bt = 0
+    if beta is not None:
+        bt, _ = check_rows(beta, (n, heads), _FP32(), index, "beta")
+        bp = beta.data_ptr()
     if out is not None:
-        check_rows(out, (n, heads, dv), (like.dtype,), device, "out")
+        check_rows(out, rows, like, index, "out")
         if not out.is_contiguous():
             raise ValueError("out must be contiguous")
+    return (q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, types[v.dtype], bp, bt, gate.data_ptr(), gt,
+            state.data_ptr()), key_heads
+
+
+@functools.lru_cache(maxsize=None)
+def _FP32():
+    import torch
+
+    return (torch.float32,)
 
 
 def prefill_states(lib, run, flags, state, q, k, v, beta, gate, starts, out, stream):
@@ -75,12 +77,11 @@ def prefill_states(lib, run, flags, state, q, k, v, beta, gate, starts, out, str
 
     seqs, heads, dv, dk = state.shape
     n = v.shape[0]
-    words, key_heads = _inputs(state, n, q, k, v, beta, gate)
+    words, key_heads = _inputs(state, n, q, k, v, beta, gate, out)
     if starts is not None:
-        check_index(starts, (seqs + 1,), torch.int32, state.device, "starts")
+        check_index(starts, (seqs + 1,), torch.int32, state.get_device(), "starts")
     elif seqs != 1:
         raise ValueError("prompts of several sequences need starts")
-    _out(out, n, v, heads, dv, state.device)
     need = 0
     if n:
         need = _prefill_bytes(lib, n, seqs, heads, dk, dv, int(beta is not None))
@@ -123,7 +124,7 @@ class LinearState:
         if self.state.device.type != "cuda":
             raise ValueError(f"expected a CUDA device, got {self.state.device}")
         self.lib = _lib.load()
-        self._run = OnStream(self.state.device)
+        self._run, self._empty = OnStream(self.state.device), torch.empty
         self._flags = torch.zeros(64, dtype=torch.int32, device=self.state.device)
 
     def reset(self):
@@ -135,20 +136,17 @@ class LinearState:
         strides; value head h uses key head h // (heads // key_heads)), beta (None:
         no delta rule) and gate [sequences, heads] FP32.  Returns out [sequences,
         heads, value_dim] of v's type."""
-        import torch
-
         seqs, heads, dv, dk = self.shape
-        words, key_heads = _inputs(self.state, seqs, q, k, v, beta, gate)
-        _out(out, seqs, v, heads, dv, self.state.device)
+        words, key_heads = _inputs(self.state, seqs, q, k, v, beta, gate, out)
+        return self._run(stream, self._step, v, out, words, (seqs, heads, key_heads, dk, dv))
 
-        def call(handle):
-            y = torch.empty((seqs, heads, dv), dtype=v.dtype, device=self.state.device) if out is None else out
-            _lib.check(self.lib.mqh_linear_step_words(_STEP_WORDS.pack(
-                *words, y.data_ptr(), seqs, heads, key_heads, dk, dv, self._flags.data_ptr(), handle)),
-                "mqh_linear_step")
-            return y
-
-        return self._run(stream, call)
+    def _step(self, handle, v, out, words, sizes):
+        if out is None:
+            out = self._empty(v.shape, dtype=v.dtype, device=self.state.device)
+        rc = self.lib.mqh_linear_step_words(_STEP_WORDS.pack(*words, out.data_ptr(), *sizes, self._flags.data_ptr(), handle))
+        if rc:
+            _lib.check(rc, "mqh_linear_step")
+        return out
 
     def prefill(self, q, k, v, beta, gate, *, starts=None, out=None, stream=None):
         """Prompts: the arguments of ``step`` with [tokens, ...] rows; sequence b's

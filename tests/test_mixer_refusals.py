@@ -158,7 +158,7 @@ def test_linear_state_constructor():
 def test_row_checks():
     from flash_moe_hip.kv_cache import check_index, check_rows
 
-    cpu, types = torch.device("cpu"), (torch.float32, torch.float16)
+    cpu, types = -1, (torch.float32, torch.float16)
     x = torch.zeros(4, 2, 64)
     check_rows(x, (4, 2, 64), types, cpu, "x")
     check_rows(torch.zeros(4, 200)[:, 3:131].unflatten(1, (2, 64)), (4, 2, 64), types, cpu, "x")
@@ -167,11 +167,11 @@ def test_row_checks():
         with pytest.raises(ValueError, match=why):
             check_rows(bad, (4, 2, 64), types, cpu, "x")
     with pytest.raises(ValueError, match="on cpu"):
-        check_rows(x, (4, 2, 64), types, torch.device("cuda", 0), "x")
+        check_rows(x, (4, 2, 64), types, 0, "x")
     i = torch.zeros(6, dtype=torch.int32)
     check_index(i, (6,), torch.int32, cpu, "i")
     for bad in (i[:5], i.long(), torch.zeros(12, dtype=torch.int32)[::2]):
         with pytest.raises(ValueError, match="contiguous"):
             check_index(bad, (6,), torch.int32, cpu, "i")
     with pytest.raises(ValueError, match="on cpu"):
-        check_index(i, (6,), torch.int32, torch.device("cuda", 0), "i")
+        check_index(i, (6,), torch.int32, 0, "i")
