@@ -508,15 +508,84 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
 }
 
 // ---- 3: the outputs of a chunk of a head
+//
+// FP32 instructions would bound this kernel (13,300 cycles a SIMD for a workgroup
+// at 128 x 128), so the long products run on BF16 ones, 16 times as fast, with
+// every operand as the exact sum of BF16 planes of 8 bits each: three of an FP32
+// value, two of an FP16, one of a BF16.  The products of planes a and b with
+// a + b <= 2 are summed; what is left out is below 2^-23 of a term, as FP32's own
+// rounding is.
+//
+// The 16x16x32 instruction contracts slots (g, e): with columns
+// 32 m + 16 (e / 4) + 4 g + e % 4 in them, the right operand is two tiles in
+// operand order as they lie, and a left row is kept in LDS with its columns in that
+// order (16 bytes a lane).
+
+template <int TYPE>
+constexpr int PLANES = TYPE == MIX_F32 ? 3 : TYPE == MIX_F16 ? 2 : 1;
+
+// v as the sum of N BF16 values, packed in pairs: p[plane][i] holds v[2 i], v[2 i + 1]
+template <int N, int COUNT>
+__device__ __forceinline__ void split(const float (&v)[COUNT], uint32_t (&p)[N][COUNT / 2]) {
+#pragma unroll
+    for (int i = 0; i < COUNT / 2; ++i) {
+        float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            p[n][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+            if (n + 1 < N) {
+                a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+                b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+            }
+        }
+    }
+}
+
+struct Planes {
+    bfloat8 p[3];
+};
+__device__ __forceinline__ Planes split_pair(floatx4 a, floatx4 b) {
+    const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    uint32_t q[3][4];
+    split<3, 8>(v, q);
+    Planes r;
+#pragma unroll
+    for (int n = 0; n < 3; ++n) r.p[n] = __builtin_bit_cast(bfloat8, uintx4{q[n][0], q[n][1], q[n][2], q[n][3]});
+    return r;
+}
+
+// place of column `col` (a multiple of 4) in a row in slot order
+__device__ __forceinline__ int slot_of(int col) {
+    return (col & ~31) + 8 * ((col >> 2) & 3) + 4 * ((col >> 4) & 1);
+}
+
+// bytes of a row of `cols` BF16 columns: 16 of padding put one piece of 16 rows into
+// 16 places of a bank line
+constexpr int plane_row(int cols) { return 2 * cols + 16; }
+
+// LDS of the kernel: Q and K as FP32 or planes, then Q's and M's planes
+template <int KP, int TYPE>
+constexpr int out_bytes() {
+    const int q = PLANES<TYPE> * C * plane_row(KP), first = TYPE == MIX_F32 ? 2 * C * (KP + 4) * 4 : 2 * q;
+    const int second = q + 3 * C * plane_row(C);
+    return first > second ? first : second;
+}
+
 template <int KP, int TYPE>
 __global__ __launch_bounds__(THREADS, KP == 256 ? 2 : 4) void k_linear_out(LinearParams p) {
-    extern __shared__ __align__(16) float lds[];
-    float* sq = lds;                    // [64][KP + 4]
-    float* sk = sq + C * (KP + 4);      // [64][KP + 4], then M [64][LS]
+    constexpr int NQ = PLANES<TYPE>, QR = plane_row(KP), MR = plane_row(C);
+    constexpr int QPLANE = C * QR, MPLANE = C * MR;
+    extern __shared__ __align__(16) uint8_t out_lds[];
+    float* sq = (float*)out_lds;            // FP32: Q, K [64][KP + 4] first
+    float* sk = sq + C * (KP + 4);
+    uint8_t* qp = out_lds;                  // Q's planes [NQ][64][QR] (16-bit types: from the start)
+    uint8_t* kp = out_lds + NQ * QPLANE;    // 16-bit types: K's planes first
+    uint8_t* mp = out_lds + NQ * QPLANE;    // M's planes [3][64][MR]
     __shared__ double s_g[C];
     __shared__ __align__(16) float s_from[C];   // e^G
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t ch = blockIdx.x;
     const int head = (int)(ch % p.heads), key_head = head / (p.heads / p.key_heads);
     const ChunkRange c = chunk_range(p, (int)(ch / p.heads));
@@ -532,14 +601,35 @@ __global__ __launch_bounds__(THREADS, KP == 256 ? 2 : 4) void k_linear_out(Linea
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = writes[(n * 4 + i) * 64];
     };
+    using Rows = StagedRows<KP, TYPE>;
+    // rows in planes, in slot order
+    auto store_planes = [&](const Rows& r, uint8_t* to) {
+#pragma unroll
+        for (int n = 0; n < Rows::N; ++n) {
+            const int i = tid + n * THREADS, t = i / Rows::PIECES, col = (i % Rows::PIECES) * 4;
+            const bool there = t < c.count && col < p.key_dim;
+            const float v[4] = {there ? r.v[n][0] : 0.0f, there ? r.v[n][1] : 0.0f, there ? r.v[n][2] : 0.0f,
+                                there ? r.v[n][3] : 0.0f};
+            uint32_t w[NQ][2];
+            split<NQ, 4>(v, w);
+#pragma unroll
+            for (int a = 0; a < NQ; ++a) *(uintx2*)(to + a * QPLANE + t * QR + slot_of(col) * 2) = uintx2{w[a][0], w[a][1]};
+        }
+    };
+    Rows q;
     {
-        StagedRows<KP, TYPE> q, k;
+        Rows k;
         q.load(p, c, p.q, p.q_token, key_head * p.q_head);
         k.load(p, c, p.k, p.k_token, key_head * p.k_head);
         const double sum = p.g[ch * C + lane];
         if (wave < vp / 16) load_tile(wave);
-        q.store(p, c, sq);
-        k.store(p, c, sk);
+        if constexpr (TYPE == MIX_F32) {
+            q.store(p, c, sq);
+            k.store(p, c, sk);
+        } else {
+            store_planes(q, qp);
+            store_planes(k, kp);
+        }
         if (wave == 0) {
             s_g[lane] = sum;
             s_from[lane] = expf((float)sum);
@@ -552,21 +642,46 @@ __global__ __launch_bounds__(THREADS, KP == 256 ? 2 : 4) void k_linear_out(Linea
         int i, j;
         if (wave + 8 * n >= 10) break;
         triangle_tile(wave + 8 * n, i, j);
-        m[n] = tile_product<KP>(sq, sk, i, j);
+        if constexpr (TYPE == MIX_F32) {
+            m[n] = tile_product<KP>(sq, sk, i, j);
+        } else {
+            m[n] = floatx4{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KP / 32; ++k)
+#pragma unroll
+                for (int a = 0; a < NQ; ++a)
+#pragma unroll
+                    for (int b = 0; b < NQ; ++b)
+                        m[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            *(const bfloat8*)(qp + a * QPLANE + (16 * i + l16) * QR + 64 * k + 16 * g),
+                            *(const bfloat8*)(kp + b * QPLANE + (16 * j + l16) * QR + 64 * k + 16 * g), m[n], 0, 0, 0);
+        }
     }
-    __syncthreads();   // (M goes where K was)
+    __syncthreads();   // (M's planes, and Q's of FP32, go where K and Q were)
+    if constexpr (TYPE == MIX_F32) store_planes(q, qp);
+    // M in planes, its columns in slot order: column 16 j + l16 of the result's rows
+    auto store_m = [&](int i, int j, floatx4 v) {
+        const int tj = 16 * j + l16;
+        uint8_t* to = mp + (slot_of(tj & ~3) + (tj & 3)) * 2;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int ti = 16 * i + 4 * g + r;
+            const float x[2] = {tj <= ti ? expf((float)(s_g[ti] - s_g[tj])) * v[r] : 0.0f, 0.0f};
+            uint32_t w[3][1];
+            split<3, 2>(x, w);
+#pragma unroll
+            for (int a = 0; a < 3; ++a) *(uint16_t*)(to + a * MPLANE + ti * MR) = (uint16_t)w[a][0];
+        }
+    };
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
         int i, j;
         if (wave + 8 * n >= 10) break;
         triangle_tile(wave + 8 * n, i, j);
-        const int tj = 16 * j + l16;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int ti = 16 * i + 4 * g + r;
-            sk[ti * LS + tj] = tj <= ti ? expf((float)(s_g[ti] - s_g[tj])) * m[n][r] : 0.0f;
-        }
+        store_m(i, j, m[n]);
     }
+    // (the blocks beside the diagonal that share an instruction with it are zeros)
+    if (wave >= 6) store_m(wave == 6 ? 0 : 2, wave == 6 ? 1 : 3, floatx4{0, 0, 0, 0});
     __syncthreads();
 
     bool finite = true;
@@ -577,26 +692,35 @@ __global__ __launch_bounds__(THREADS, KP == 256 ? 2 : 4) void k_linear_out(Linea
         floatx4 acc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = floatx4{0, 0, 0, 0};
-        // (the query operands one step ahead, and no further: registers)
-        floatx4 a[2][4];
-        auto load_q = [&](int k) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[k & 1][i] = *(const floatx4*)(sq + (16 * i + l16) * (KP + 4) + 16 * k + 4 * g);
-        };
-        load_q(0);
+        for (int k = 0; k < KP / 32; ++k) {
+            const Planes b = split_pair(s4[2 * k], s4[2 * k + 1]);
 #pragma unroll
-        for (int k = 0; k < KP / 16; ++k) {
-            if (k + 1 < KP / 16) load_q(k + 1);
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = mfma4(a[k & 1][i], s4[k], acc[i]);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int a = 0; a < NQ; ++a) {
+                    const bfloat8 x = *(const bfloat8*)(qp + a * QPLANE + (16 * i + l16) * QR + 64 * k + 16 * g);
+#pragma unroll
+                    for (int d = 2 - a; d >= 0; --d) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, b.p[d], acc[i], 0, 0, 0);
+                }
+            __builtin_amdgcn_sched_barrier(0);   // (no further ahead: registers)
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            acc[i] *= *(const floatx4*)(s_from + 16 * i + 4 * g);
+        for (int i = 0; i < 4; ++i) acc[i] *= *(const floatx4*)(s_from + 16 * i + 4 * g);
 #pragma unroll
-            for (int j = 0; j <= i; ++j)
-                acc[i] = mfma4(*(const floatx4*)(sk + (16 * i + l16) * LS + 16 * j + 4 * g), u[j], acc[i]);
+        for (int k = 0; k < 2; ++k) {
+            const Planes b = split_pair(u[2 * k], u[2 * k + 1]);
+#pragma unroll
+            for (int i = 2 * k; i < 4; ++i)
+#pragma unroll
+                for (int a = 0; a < 3; ++a) {
+                    const bfloat8 x = *(const bfloat8*)(mp + a * MPLANE + (16 * i + l16) * MR + 64 * k + 16 * g);
+#pragma unroll
+                    for (int d = 2 - a; d >= 0; --d) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, b.p[d], acc[i], 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int t = 16 * i + 4 * g + r;
@@ -605,7 +729,6 @@ __global__ __launch_bounds__(THREADS, KP == 256 ? 2 : 4) void k_linear_out(Linea
                     finite &= __builtin_isfinite(acc[i][r]);
                 }
             }
-        }
     }
     if (!finite) atomicOr(&p.flags[FLAG_NONFINITE], 1);
 }
@@ -620,7 +743,7 @@ static hipError_t launch_prompt_of(const LinearParams& p, hipStream_t s) {
     const unsigned vt = (unsigned)(p.value_dim + 15) / 16, sh = (unsigned)(p.seqs * p.heads);
     hipLaunchKernelGGL((k_linear_scan<KP, DELTA>), dim3((sh + 7) / 8 * 8 * vt), dim3(256), 0, s, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    constexpr int bytes = 2 * C * (KP + 4) * 4;
+    constexpr int bytes = out_bytes<KP, TYPE>();
     hipLaunchKernelGGL((k_linear_out<KP, TYPE>), dim3(units), dim3(THREADS), bytes, s, p);
     return hipGetLastError();
 }
