@@ -145,10 +145,12 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
         load_k(ra, rb);
         load_v(ra, rb);
         for (int it = 0; block < block1; ++it, block += 4) {
-            const int next = block + 4;
-            const bool more = next < block1;
+            // (past the last block its keys are read once more: with the loads under a
+            // condition the compiler waits for all of them where it needs the oldest)
+            const bool more = block + 4 < block1;
+            const int next = more ? block + 4 : block;
             if (more && ((it + 1) & 63) == 0) load_pages(next);
-            if (more) rows_of(next, it + 1, ra, rb);
+            rows_of(next, more ? it + 1 : it, ra, rb);
             const bool edge = block * 32 + 32 > keys;
             // S^T = K Q^T
             floatx4 s[2];
@@ -188,7 +190,7 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
                     s[j][e] = t;
                     mx = fmaxf(mx, t);
                 }
-            if (more) load_k(ra, rb);
+            load_k(ra, rb);
             // V into LDS (rows past the end as zeros: what is there may be anything)
             {
                 const int piece = lane % PIECES, key = lane / PIECES;
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
                     }
                 }
             }
-            if (more) load_v(ra, rb);
+            load_v(ra, rb);
             if (__any(mx > m + ATTEND_GROWTH)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16));
                 mx = fmaxf(mx, __shfl_xor(mx, 32));

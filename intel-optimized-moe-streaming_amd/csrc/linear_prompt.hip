@@ -433,8 +433,10 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
     // the address unit for as long as half a chunk's products.)
     auto process = [&](Stage& d, int n, Stage& f, int next) {
         const int64_t ch = (int64_t)(base + n) * p.heads + head;
-        const bool more = next < n1;
-        const Buffers r = buffers(more ? next : n);
+        // (past the last chunk its operands are read once more: with the loads under a
+        // condition the compiler waits for all of them where it needs the oldest)
+        next = min(next, n1 - 1);
+        const Buffers r = buffers(next);
         // (tile (value tile, n): row l16, columns 16 n + 4 g + j)
         floatx4* kept = (floatx4*)(p.s0 + ch * vp * KP + 16 * (tile * KP + kc)) + lane;
 #pragma unroll
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
             floatx4(*mine)[64] = part[n & 1][wave];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (more) load_w(f, r, i);
+                load_w(f, r, i);
                 u[i] = floatx4{0, 0, 0, 0};
 #pragma unroll
                 for (int m = 0; m < NB; ++m) u[i] = mfma4(d.w[i][m], s[m], u[i]);
@@ -471,10 +473,10 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
         }
 #pragma unroll
         for (int m = 0; m < NB; ++m) s[m] *= d.end;
-        if (more) load_end(f, next);
+        load_end(f, next);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (more) load_rest(f, r, i);
+            load_rest(f, r, i);
 #pragma unroll
             for (int m = 0; m < NB; ++m) s[m] = mfma4(d.ke[i][m], u[i], s[m]);
             __builtin_amdgcn_sched_barrier(0);
@@ -482,16 +484,16 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
     };
     Stage st[DEPTH];
 #pragma unroll
-    for (int d = 0; d < DEPTH - 1; ++d)
-        if (n0 + d < n1) {
-            const Buffers r = buffers(n0 + d);
+    for (int d = 0; d < DEPTH - 1; ++d) {
+        const int n = min(n0 + d, n1 - 1);
+        const Buffers r = buffers(n);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (DELTA) load_w(st[d], r, i);
-                load_rest(st[d], r, i);
-            }
-            load_end(st[d], n0 + d);
-        }
+        for (int i = 0; i < 4; ++i)
+            if constexpr (DELTA) load_w(st[d], r, i);
+        load_end(st[d], n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_rest(st[d], r, i);
+    }
     for (int n = n0; n < n1; n += DEPTH) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
