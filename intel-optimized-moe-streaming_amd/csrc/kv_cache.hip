@@ -60,10 +60,27 @@ __global__ __launch_bounds__(256) void k_kv_write(KvParams p) {
         if (!finite) scale = __uint_as_float(0x7fc00000u);
         uint32_t w[2] = {0, 0};
         if (finite && scale > 0.0f) {
+            // x / scale, rounded to a whole number: the product with 1 / scale is within
+            // 2^-15 of the quotient (up to 127, three roundings), so it rounds to the same
+            // number unless it is that near to a half; only then are the eight divided.
+            // (Eight divisions a lane bounded the kernel: 27.9 us for 16,384 tokens of
+            // 8 heads of 128.)
+            const float inv = 1.0f / scale;
+            float c[8], nearest = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int c = (int)fminf(fmaxf(rintf(x[i] / scale), -127.0f), 127.0f);
-                w[i >> 2] |= (uint32_t)(c & 0xff) << (8 * (i & 3));
+                const float y = x[i] * inv;
+                c[i] = rintf(y);
+                nearest = fmaxf(nearest, fabsf(y - c[i]));
+            }
+            if (nearest > 0.5f - 0x1p-14f) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) c[i] = rintf(x[i] / scale);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int v = (int)fminf(fmaxf(c[i], -127.0f), 127.0f);
+                w[i >> 2] |= (uint32_t)(v & 0xff) << (8 * (i & 3));
             }
         }
         uintx2 codes = {w[0], w[1]};

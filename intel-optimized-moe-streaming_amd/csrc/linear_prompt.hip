@@ -457,16 +457,15 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                floatx4 x = part[n & 1][0][i][lane];
 #pragma unroll
-                for (int v = 1; v < 4; ++v) x += part[n & 1][v][i][lane];
-                u[i] = d.u[i] - x;
+                for (int v = 1; v < 4; ++v) u[i] += part[n & 1][(wave + v) & 3][i][lane];
+                u[i] = d.u[i] - u[i];
             }
             // (the waves share the writing of U: 16 tokens each)
-            floatx4 own = u[0];
+            floatx4* writes = (floatx4*)(p.u + (ch * vp + 16 * tile) * C) + lane;
 #pragma unroll
-            for (int i = 1; i < 4; ++i) own = wave == i ? u[i] : own;
-            ((floatx4*)(p.u + (ch * vp + 16 * tile) * C))[wave * 64 + lane] = own;
+            for (int i = 0; i < 4; ++i)
+                if (wave == i) writes[i * 64] = u[i];
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) u[i] = d.u[i];
