@@ -13,7 +13,9 @@
 //
 // Bound by memory: a row is read and written once.  dim / 8 lanes own a row of
 // eight values each (16-byte loads of 16-bit rows, 8-byte stores of codes); the
-// row's maximum goes over them by lane exchanges, no LDS.
+// row's maximum goes over them by lane exchanges, no LDS.  A workgroup takes one
+// head of consecutive tokens, whose scales usually share a line: with the heads of
+// a token together, every line of scales was written piecemeal from several XCDs.
 
 #include "mixers.h"
 
@@ -29,29 +31,10 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
     return v;
 }
 
-template <int DIM, int TYPE, int CACHE>
-__global__ __launch_bounds__(256) void k_kv_write(KvParams p) {
-    constexpr int LANES = DIM / 8;   // of a row
-    const int lane = threadIdx.x % LANES;
-    const uint32_t row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const bool live = row < (uint32_t)p.tokens * p.kv_heads;
-    const uint32_t token = live ? row / (uint32_t)p.kv_heads : 0, head = live ? row % (uint32_t)p.kv_heads : 0;
-    const int64_t slot = p.slots[token];
-    const bool is_v = blockIdx.y;
-    const int64_t at = is_v ? token * p.v_token + head * p.v_head : token * p.k_token + head * p.k_head;
-    float x[8];
-    load8<TYPE>(is_v ? p.v : p.k, at + lane * 8, x);
-    uint32_t top = 0;   // of the magnitudes' bits: NaN above infinity above the numbers
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    if constexpr (CACHE == MIX_Q8) top = row_max<LANES>(top);
-    if (!live || slot < 0) return;
-    if (slot >= p.n_slots) {
-        if (lane == 0) atomicOr(&p.flags[FLAG_BAD_ID], 1);
-        return;
-    }
-    const int64_t page = slot >> p.page_shift, off = slot & ((1 << p.page_shift) - 1);
-    const int64_t dst = (((page * p.kv_heads + head) << p.page_shift) + off);
+// one row's store: codes and scale, or the values rounded once
+template <int DIM, int CACHE>
+__device__ __forceinline__ void write_row(const KvParams& p, const float (&x)[8], uint32_t top, int64_t dst, bool is_v,
+                                          int lane) {
     void* cache = is_v ? p.vc : p.kc;
     if constexpr (CACHE == MIX_Q8) {
         const bool finite = top < 0x7f800000u;
@@ -62,9 +45,7 @@ __global__ __launch_bounds__(256) void k_kv_write(KvParams p) {
         if (finite && scale > 0.0f) {
             // x / scale, rounded to a whole number: the product with 1 / scale is within
             // 2^-15 of the quotient (up to 127, three roundings), so it rounds to the same
-            // number unless it is that near to a half; only then are the eight divided.
-            // (Eight divisions a lane bounded the kernel: 27.9 us for 16,384 tokens of
-            // 8 heads of 128.)
+            // number unless it is that near to a half; only then are the eight divided
             const float inv = 1.0f / scale;
             float c[8], nearest = 0.0f;
 #pragma unroll
@@ -83,62 +64,113 @@ __global__ __launch_bounds__(256) void k_kv_write(KvParams p) {
                 w[i >> 2] |= (uint32_t)(v & 0xff) << (8 * (i & 3));
             }
         }
-        uintx2 codes = {w[0], w[1]};
+        const uintx2 codes = {w[0], w[1]};
         *(uintx2*)((int8_t*)cache + dst * DIM + lane * 8) = codes;
         if (lane == 0) {
             (is_v ? p.vs : p.ks)[dst] = scale;
             if (!finite) atomicOr(&p.flags[FLAG_NONFINITE], 1);
         }
     } else {
-        // (an FP32 value past FP16's range becomes infinite: a fault as well)
-        bool bad = top >= 0x7f800000u;
-        if constexpr (CACHE == MIX_F16) bad = top >= 0x477ff000u;
-        else bad = top >= 0x7f7f8000u;
+        // (an FP32 value past the cache's range becomes infinite: a fault as well)
         store8<CACHE>(cache, dst * DIM + lane * 8, x);
-        if (bad) atomicOr(&p.flags[FLAG_NONFINITE], 1);
+        if (top >= (CACHE == MIX_F16 ? 0x477ff000u : 0x7f7f8000u)) atomicOr(&p.flags[FLAG_NONFINITE], 1);
     }
 }
 
-template <int DIM, int TYPE, int CACHE>
-__global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
-    constexpr int LANES = DIM / 8;
+// N rows of a head a lane (tokens 256 / LANES apart), all of their loads in flight
+template <int DIM, int TYPE, int CACHE, int N>
+__global__ __launch_bounds__(256) void k_kv_write(KvParams p) {
+    constexpr int LANES = DIM / 8, ROWS = 256 / LANES;   // lanes of a row, rows of a pass
     const int lane = threadIdx.x % LANES;
-    const uint32_t row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    if (row >= (uint32_t)p.tokens * p.kv_heads) return;
-    const uint32_t token = row / (uint32_t)p.kv_heads, head = row % (uint32_t)p.kv_heads;
-    const int64_t slot = p.slots[token];
+    const int head = blockIdx.x % (uint32_t)p.kv_heads;
+    const int first = blockIdx.x / (uint32_t)p.kv_heads * (N * ROWS) + threadIdx.x / LANES;
     const bool is_v = blockIdx.y;
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};   // no token, no value
-    if (slot >= p.n_slots) {
-        if (lane == 0) atomicOr(&p.flags[FLAG_BAD_ID], 1);
-    } else if (slot >= 0) {
-        const int64_t page = slot >> p.page_shift, off = slot & ((1 << p.page_shift) - 1);
-        const int64_t src = (((page * p.kv_heads + head) << p.page_shift) + off);
-        const void* cache = is_v ? p.vc : p.kc;
+    const void* src = is_v ? p.v : p.k;
+    const int64_t step = is_v ? p.v_token : p.k_token, at = head * (is_v ? p.v_head : p.k_head) + lane * 8;
+    int64_t slot[N];
+    float x[N][8];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int token = min(first + n * ROWS, p.tokens - 1);
+        slot[n] = p.slots[token];
+        load8<TYPE>(src, token * step + at, x[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        uint32_t top = 0;   // of the magnitudes' bits: NaN above infinity above the numbers
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[n][i]) & 0x7fffffffu);
+        if constexpr (CACHE == MIX_Q8) top = row_max<LANES>(top);
+        if (first + n * ROWS >= p.tokens || slot[n] < 0) continue;
+        if (slot[n] >= p.n_slots) {
+            if (lane == 0) atomicOr(&p.flags[FLAG_BAD_ID], 1);
+            continue;
+        }
+        const int64_t page = slot[n] >> p.page_shift, off = slot[n] & ((1 << p.page_shift) - 1);
+        write_row<DIM, CACHE>(p, x[n], top, ((page * p.kv_heads + head) << p.page_shift) + off, is_v, lane);
+    }
+}
+
+template <int DIM, int TYPE, int CACHE, int N>
+__global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
+    constexpr int LANES = DIM / 8, ROWS = 256 / LANES;
+    const int lane = threadIdx.x % LANES;
+    const int head = blockIdx.x % (uint32_t)p.kv_heads;
+    const int first = blockIdx.x / (uint32_t)p.kv_heads * (N * ROWS) + threadIdx.x / LANES;
+    const bool is_v = blockIdx.y;
+    const void* cache = is_v ? p.vc : p.kc;
+    int64_t slot[N];
+    float x[N][8];
+#pragma unroll
+    for (int n = 0; n < N; ++n) slot[n] = p.slots[min(first + n * ROWS, p.tokens - 1)];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        // (a slot that is none reads slot 0 and gives zeros)
+        const int64_t s = slot[n] >= 0 && slot[n] < p.n_slots ? slot[n] : 0;
+        const int64_t page = s >> p.page_shift, off = s & ((1 << p.page_shift) - 1);
+        const int64_t src = ((page * p.kv_heads + head) << p.page_shift) + off;
         if constexpr (CACHE == MIX_Q8) {
             const uintx2 codes = *(const uintx2*)((const int8_t*)cache + src * DIM + lane * 8);
             const float scale = (is_v ? p.vs : p.ks)[src];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = (float)(int8_t)(codes[i >> 2] >> (8 * (i & 3))) * scale;
+            for (int i = 0; i < 8; ++i) x[n][i] = (float)(int8_t)(codes[i >> 2] >> (8 * (i & 3))) * scale;
         } else {
-            load8<CACHE>(cache, src * DIM + lane * 8, x);
+            load8<CACHE>(cache, src * DIM + lane * 8, x[n]);
         }
     }
-    store8<TYPE>((void*)(is_v ? p.v : p.k), (int64_t)row * DIM + lane * 8, x);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int64_t token = first + n * ROWS;
+        if (token >= p.tokens) continue;
+        if (slot[n] < 0 || slot[n] >= p.n_slots) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[n][i] = 0.0f;
+            if (slot[n] >= p.n_slots && lane == 0) atomicOr(&p.flags[FLAG_BAD_ID], 1);
+        }
+        store8<TYPE>((void*)(is_v ? p.v : p.k), (token * p.kv_heads + head) * DIM + lane * 8, x[n]);
+    }
 }
 
-template <int DIM, int TYPE, int CACHE>
+template <int DIM, int TYPE, int CACHE, int N>
 static hipError_t launch_kv(const KvParams& p, bool write, hipStream_t s) {
-    constexpr int ROWS = 256 / (DIM / 8);
-    const dim3 grid((unsigned)(((int64_t)p.tokens * p.kv_heads + ROWS - 1) / ROWS), 2);
-    if (write) hipLaunchKernelGGL((k_kv_write<DIM, TYPE, CACHE>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((k_kv_read<DIM, TYPE, CACHE>), grid, dim3(256), 0, s, p);
+    constexpr int ROWS = N * 256 / (DIM / 8);
+    const dim3 grid((unsigned)((p.tokens + ROWS - 1) / ROWS * p.kv_heads), 2);
+    if (write) hipLaunchKernelGGL((k_kv_write<DIM, TYPE, CACHE, N>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((k_kv_read<DIM, TYPE, CACHE, N>), grid, dim3(256), 0, s, p);
     return hipGetLastError();
+}
+
+// Four rows a lane where that leaves every CU its eight workgroups (16,384 tokens of
+// 8 heads of 128 into codes and back: 46.7 us with one, 44.8 with four), one where there are few rows.
+template <int DIM, int TYPE, int CACHE>
+static hipError_t launch_kv_rows(const KvParams& p, bool write, hipStream_t s) {
+    if ((int64_t)p.tokens * p.kv_heads * 2 * (DIM / 8) / (4 * 256) >= 2048) return launch_kv<DIM, TYPE, CACHE, 4>(p, write, s);
+    return launch_kv<DIM, TYPE, CACHE, 1>(p, write, s);
 }
 
 template <int DIM>
 static hipError_t launch_kv_types(const KvParams& p, bool write, hipStream_t s) {
-#define MQH_KV(T, C) if (p.type == T && p.cache_type == C) return launch_kv<DIM, T, C>(p, write, s)
+#define MQH_KV(T, C) if (p.type == T && p.cache_type == C) return launch_kv_rows<DIM, T, C>(p, write, s)
     MQH_KV(MIX_F32, MIX_F16); MQH_KV(MIX_F32, MIX_BF16); MQH_KV(MIX_F32, MIX_Q8);
     MQH_KV(MIX_F16, MIX_F16); MQH_KV(MIX_F16, MIX_BF16); MQH_KV(MIX_F16, MIX_Q8);
     MQH_KV(MIX_BF16, MIX_F16); MQH_KV(MIX_BF16, MIX_BF16); MQH_KV(MIX_BF16, MIX_Q8);

@@ -90,13 +90,13 @@ int check_linear(const void* q, const void* k, const void* v, int type, const fl
 }
 
 // Chunks a pass of the prompt kernels takes: all of them up to a workspace of
-// 1 GiB, at least 64 (a pass costs three launches and breaks the scans of other
+// 1 GiB, at least 8 (a pass costs three launches and breaks the scans of other
 // sequences off).
 constexpr int64_t LINEAR_PASS_BYTES = (int64_t)1 << 30;
 int64_t linear_pass_chunks(int tokens, int seqs, int heads, int key_dim, int value_dim, bool delta) {
     const int64_t all = linear_chunks(tokens, seqs);
     const int64_t one = heads * linear_chunk_floats(linear_kp(key_dim), linear_vp(value_dim), delta) * 4;
-    return std::min(all, std::max<int64_t>(64, LINEAR_PASS_BYTES / one));
+    return std::min(all, std::max<int64_t>(8, LINEAR_PASS_BYTES / one));
 }
 
 }  // namespace

@@ -67,6 +67,32 @@ def test_write_and_read(tokens, heads, dim, page, dtype, cache, strided):
         assert ((rk.cpu().double()[kept] - x).abs() <= step * (0.5 + 3 * 127 * half_step(torch.float32))).all()
 
 
+@pytest.mark.parametrize("cache", CACHES, ids=str)
+@pytest.mark.parametrize("tokens,heads,dim", [(8195, 8, 128), (32773, 4, 64), (4101, 8, 256)])
+def test_many_rows(tokens, heads, dim, cache):
+    """Enough rows that a lane takes four, and a ragged end."""
+    from flash_moe_hip.kv_cache import PagedCache
+
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    c = PagedCache.empty(-(-tokens // 32) + 1, heads, dim, 32, cache)
+    k, v = (torch.randn(tokens, heads, dim, generator=g, device="cuda").bfloat16() for _ in range(2))
+    slots = torch.randperm(c.pages * 32, generator=g, device="cuda")[:tokens]
+    slots[-5:-1] = -1
+    kept = slots >= 0
+    c.write(k, v, slots)
+    for got, x in zip(c.read(slots, torch.float32), (k, v)):
+        if cache == torch.int8:   # (on the CPU: torch divides by a number on the GPU with its reciprocal)
+            codes, scale = quantized(x.cpu())
+            want = (codes.float() * scale.unsqueeze(-1)).cuda()
+        else:
+            want = x.to(cache).float()
+        assert torch.equal(got[kept], want[kept]) and not got[~kept].any()
+    assert c.status() == 0
+    free = torch.ones(c.pages * 32, dtype=torch.bool, device="cuda")
+    free[slots[kept]] = False
+    assert not c.k.transpose(1, 2).flatten(0, 1)[free].any()
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_edge_rows_of_an_int8_cache(dim):
     from flash_moe_hip.kv_cache import PagedCache
