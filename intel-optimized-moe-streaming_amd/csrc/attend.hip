@@ -71,6 +71,15 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
     // stay in few L2s), tiles with the most keys first
     const int kvh = blockIdx.x % p.kv_heads, split = blockIdx.y;
     const int tile = p.tiles - 1 - blockIdx.x / p.kv_heads;
+    if (p.starts && blockIdx.x == 0 && split == 0) {
+        // (starts out of order may leave a sequence without a workgroup that looks at it)
+        bool bad = false;
+        for (int i = tid; i < p.seqs; i += THREADS) {
+            const int a = p.starts[i], z = p.starts[i + 1];
+            bad |= a < 0 || z < a || z > p.tokens;
+        }
+        if (bad) atomicOr(&p.flags[FLAG_BAD_ID], 1);
+    }
     int b = -1;
     {
         // tiles of sequence b begin at starts[b] / tile_tokens + b, which leaves room

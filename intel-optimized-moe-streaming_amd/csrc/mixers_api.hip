@@ -35,10 +35,13 @@ int check_cache(const void* kc, const void* vc, const float* ks, const float* vs
     return unaligned(kc, 16) || unaligned(vc, 16) ? ST_ARG : ST_OK;
 }
 
-// Workgroups of the many-row kernel, their query tokens, and the splits of
-// their keys: enough for four workgroups a CU (what is left over when the longest
-// end), none of under 512 keys (below that the splits' sums cost more traffic than
-// the keys).
+// Workgroups of an attention call, their query tokens, and the splits of their
+// keys.  Many rows: the splits that make one round of what the chip holds (two
+// workgroups a CU, one at dim 256); more cost their sums' traffic and a second
+// round (512 tokens after 8,000, dim 256, 16 heads: 100 us, 127 with twice the
+// splits).  Single tokens: sixteen a CU, so that long sequences end with short ones
+// (64 ragged ones of up to 8,192 keys: 204 us, 221 with four).  No split of under
+// 512 keys (single tokens 256).
 struct AttendPlan {
     bool token;
     int tile_tokens, tiles, splits;
@@ -50,7 +53,7 @@ AttendPlan attend_plan(int tokens, int seqs, bool single, int heads, int kv_head
     a.token = single && group <= TOKEN_ROWS;
     a.tile_tokens = attend_rows(dim) / group;
     a.tiles = a.token ? seqs : tokens / a.tile_tokens + seqs;
-    const int64_t groups = (int64_t)a.tiles * kv_heads, want = a.token ? 4096 : dim == 256 ? 512 : 1024, least = a.token ? 256 : 512;
+    const int64_t groups = (int64_t)a.tiles * kv_heads, want = a.token ? 4096 : dim == 256 ? 256 : 512, least = a.token ? 256 : 512;
     int64_t splits = (want + groups - 1) / groups;
     splits = std::min(splits, std::max<int64_t>(1, most_keys / least));
     a.splits = (int)std::min<int64_t>(splits, 128);
@@ -250,9 +253,10 @@ int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const voi
 }
 
 // The calls with their arguments, in order, as 64-bit words (pointers as
-// integers, floats as the bits of a double)
+// integers, floats as the bits of a double).  A count that an int does not hold is
+// refused, not cut.
 int mqh_linear_step_words(const int64_t* a) {
-    if (!a) return ST_ARG;
+    if (!a || a[16] != (int)a[16]) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     return mqh_linear_step(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10), a[11],
                            (const float*)P(12), a[13], (float*)P(14), P(15), (int)a[16], (int)a[17], (int)a[18],
@@ -260,7 +264,7 @@ int mqh_linear_step_words(const int64_t* a) {
 }
 
 int mqh_linear_prefill_words(const int64_t* a) {
-    if (!a) return ST_ARG;
+    if (!a || a[17] != (int)a[17] || a[18] != (int)a[18]) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     return mqh_linear_prefill(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10),
                               a[11], (const float*)P(12), a[13], (float*)P(14), P(15), (const int32_t*)P(16),
@@ -269,7 +273,7 @@ int mqh_linear_prefill_words(const int64_t* a) {
 }
 
 int mqh_kv_write_words(const int64_t* a) {
-    if (!a) return ST_ARG;
+    if (!a || a[8] != (int)a[8]) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     return mqh_kv_write(P(0), a[1], a[2], P(3), a[4], a[5], (int)a[6], (const int64_t*)P(7), (int)a[8], P(9), P(10),
                         (float*)P(11), (float*)P(12), (int)a[13], a[14], (int)a[15], (int)a[16], (int)a[17],
@@ -277,14 +281,14 @@ int mqh_kv_write_words(const int64_t* a) {
 }
 
 int mqh_kv_read_words(const int64_t* a) {
-    if (!a) return ST_ARG;
+    if (!a || a[1] != (int)a[1]) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     return mqh_kv_read((const int64_t*)P(0), (int)a[1], P(2), P(3), (const float*)P(4), (const float*)P(5), (int)a[6],
                        a[7], (int)a[8], (int)a[9], (int)a[10], P(11), P(12), (int)a[13], (int32_t*)P(14), P(15));
 }
 
 int mqh_attend_words(const int64_t* a) {
-    if (!a) return ST_ARG;
+    if (!a || a[4] != (int)a[4] || a[6] != (int)a[6] || a[19] != (int)a[19]) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     double scale;
     __builtin_memcpy(&scale, &a[21], 8);

@@ -224,7 +224,8 @@ class PagedCache:
         last of its tokens; without it every sequence has one.  Query head h reads
         kv head h // (heads // kv_heads).  Each query sees the keys up to its own
         position; a row that sees none (a length below its queries) is zeros; rows
-        of `out` that belong to no sequence are left as they were.  scale > 0
+        of `out` that belong to no sequence are left as they were (without `out`
+        they hold anything).  scale > 0
         (default head_dim ** -0.5).  Returns out [tokens, heads, head_dim] of q's
         type.  Page numbers, lengths and starts out of range latch -9 (the
         rows concerned are then undefined), outputs that are not finite -4."""

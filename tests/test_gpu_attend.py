@@ -225,7 +225,7 @@ def test_bad_pages_lengths_and_starts_are_reported(single):
     call(c, p, single=single)
     assert c.status() in (-9, -4)
     if not single:
-        for starts in ([0, 5, 2], [-3, 1, 2], [0, 1, 9]):
+        for starts in ([0, 5, 2], [-3, 1, 2], [0, 1, 9], [2, 0, 1]):
             p = fresh()
             p["starts"] = torch.tensor(starts, dtype=torch.int32)
             c = cache_of(p)

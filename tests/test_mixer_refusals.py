@@ -126,6 +126,30 @@ def test_linear_codes(lib, prompt):
     assert lib.mqh_linear_step_words(None) == -1 and lib.mqh_linear_prefill_words(None) == -1
 
 
+def test_counts_past_32_bits_are_refused(lib):
+    """The word forms: 2^32 + 4 tokens are not 4."""
+    import struct
+
+    p, n = 4096, 2 ** 32 + 4
+    cache = [p, p, 0, 0, 1, 4, 2, 16, 64]
+    assert lib.mqh_kv_write_words(struct.pack("20q", p, 128, 64, p, 128, 64, 1, p, n, *cache, p, 0)) == -1
+    assert lib.mqh_kv_read_words(struct.pack("16q", p, n, *cache, p, p, 1, p, 0)) == -1
+    for tokens, seqs, cols in ((n, 2, 4), (4, n, 4), (4, 2, n)):
+        assert lib.mqh_attend_words(struct.pack("21qd5q", p, 512, 64, 1, tokens, p, seqs, 8, *cache, p, cols, cols, p,
+                                                0.125, p, p, 1 << 30, p, 0)) == -1
+    rows = [p, 64, 16, p, 64, 16, p, 64, 16, 0, p, 4, p, 4, p, p]
+    assert lib.mqh_linear_step_words(struct.pack("23q", *rows, n, 4, 4, 16, 16, p, 0)) == -1
+    for tokens, seqs in ((n, 2), (8, n)):
+        assert lib.mqh_linear_prefill_words(struct.pack("27q", *rows, p, tokens, seqs, 4, 4, 16, 16, p, 1 << 30, p, 0)) == -1
+
+
+def test_strides_past_a_chunk_are_refused(lib):
+    for name in ("qt", "qh", "kt", "kh", "vt", "vh", "bt", "gt"):
+        for prompt in (False, True):
+            assert linear(lib, prompt, **{name: 2 ** 22 + 1}) == -1
+            assert linear(lib, prompt, **{name: -1}) == -1
+
+
 def test_linear_prompt_codes(lib):
     need = lib.mqh_linear_prefill_workspace_bytes(8, 2, 4, 16, 16, 1)
     assert need > lib.mqh_linear_prefill_workspace_bytes(8, 2, 4, 16, 16, 0) > 0
