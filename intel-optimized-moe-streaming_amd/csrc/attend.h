@@ -26,9 +26,8 @@ constexpr int ATTEND_GROUP_MAX = 128;
 // offset.
 constexpr int attend_krow(int dim) { return 2 * dim + 16; }
 constexpr int attend_vrow(int dim) { return 2 * dim + 64; }
-// query heads a kv head may have in launch_attend_token; keys of a step
+// query heads a kv head may have in launch_attend_token
 constexpr int TOKEN_ROWS = 16;
-constexpr int TOKEN_STEP = 128;
 
 // the 16-bit type the matrix instructions take: BF16 for BF16 caches, else FP16
 // (8-bit codes are exact in it, and so are FP16 values)

@@ -12,8 +12,8 @@
 //   2 k_linear_scan    chunk after chunk, 16 value rows of a head a workgroup:
 //                      U = (1 + L)^-1 diag(beta) V - W S0^T, then S1
 //   3 k_linear_out     chunks in parallel: O
-// Everything is FP32 on FP32 matrix instructions (16x16x4); the sums G are taken
-// in double, so that differences of far gates keep their digits, and a gate
+// Everything is FP32, on FP32 matrix instructions (16x16x4; the outputs on BF16 ones
+// over exact planes, below); the sums G are taken in double, so that differences of far gates keep their digits, and a gate
 // below -1e4 counts as that (its exponential is 0 either way).  The triangular
 // system is solved by substitution, block by block of 16 rows: powers of L would
 // cancel where keys repeat.
@@ -29,6 +29,11 @@
 // What one kernel leaves for another lies in the workspace in operand order, 16
 // bytes a lane, a 16 x 16 tile's 1 KiB in one run (rows 256 bytes and more apart
 // cost the address unit 64 cycles a load: the scan took 4 us a chunk so).
+//
+// 4096 FP32 tokens, 32 heads over 16 key heads, 128 x 128: 80 + 153 + 82 us.  The
+// first and last are bound by memory (160 and 192 KB a chunk and head, 4.2 and 4.9
+// TB/s), the scan by its chain (2.4 us a chunk: products 0.7, the waves' exchange of
+// W S0^T 0.9, loads and stores the rest).
 
 #include "mixers.h"
 
@@ -101,10 +106,8 @@ __device__ __forceinline__ float store_gates(const LinearParams& p, int64_t ch, 
     const int lane = threadIdx.x & 63;
     const double end = __shfl(g, 63);
     p.g[ch * C + lane] = g;
-    const float to_end = expf((float)(end - g));
-    p.e[ch * 128 + lane] = to_end;
-    if (lane == 63) p.e[ch * 128 + 64] = expf((float)end);
-    return to_end;
+    if (lane == 63) p.e[ch * 4] = expf((float)end);
+    return expf((float)(end - g));
 }
 
 constexpr int THREADS = 512;   // of the kernels that take chunks in parallel
@@ -426,7 +429,7 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
 #pragma unroll
         for (int m = 0; m < NB; ++m) d.ke[i][m] = buffer4(r.ke, 16 * lane, 1024 * (4 * m + i));
     };
-    auto load_end = [&](Stage& d, int n) { d.end = p.e[((int64_t)(base + n) * p.heads + head) * 128 + 64]; };
+    auto load_end = [&](Stage& d, int n) { d.end = p.e[((int64_t)(base + n) * p.heads + head) * 4]; };
 
     // One chunk from `d`, while chunk `next`'s operands are read into `f`: a few
     // loads before each group of products.  (All of them at once held the waves at

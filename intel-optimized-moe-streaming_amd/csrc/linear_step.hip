@@ -8,7 +8,8 @@
 // 16-byte pieces and the row stays in registers between.  Both dot products are
 // taken of the state as read, S q = e^gate (S q) + u (k q), so one pass of lane
 // sums serves them.  A wave takes 16 rows of one head and has all their loads in
-// flight.  Everything is FP32; 16-bit q, k and v are exact in it.
+// flight.  Everything is FP32; 16-bit q, k and v are exact in it.  64 sequences of 32
+// x 128 x 128, FP32: 57 us over changing states, 4.8 TB/s (a large copy: 4.9).
 
 #include "mixers.h"
 

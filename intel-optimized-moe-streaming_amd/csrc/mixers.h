@@ -75,7 +75,7 @@ struct LinearParams {
     float* u;                   // T diag(beta) V, then the writes U (without the delta rule V)
     float* s0;                  // the state before the chunk
     double* g;                  // [64] running sums of the gate
-    float* e;                   // e^(G_end) at 64
+    float* e;                   // e^(G_end), 16 bytes a unit
     int chunk0, chunks;
 };
 
@@ -88,7 +88,7 @@ inline int linear_vp(int value_dim) { return (value_dim + 15) & ~15; }
 inline int64_t linear_chunks(int64_t tokens, int64_t seqs) { return tokens / LINEAR_CHUNK + seqs; }
 // floats of one chunk of one head
 inline int64_t linear_chunk_floats(int kp, int vp, bool delta) {
-    return (delta ? 2 : 1) * 64 * kp + 64 * vp + (int64_t)vp * kp + 128 + 128;
+    return (delta ? 2 : 1) * 64 * kp + 64 * vp + (int64_t)vp * kp + 128 + 4;
 }
 
 hipError_t launch_linear_step(const LinearParams& p, hipStream_t s);

@@ -235,10 +235,10 @@ int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const voi
     p.state = state; p.out = out; p.starts = starts; p.type = type;
     p.tokens = tokens; p.seqs = seqs; p.heads = heads; p.key_heads = key_heads;
     p.key_dim = key_dim; p.value_dim = value_dim; p.flags = flags;
-    // (every part is a multiple of 64 floats a unit)
+    // (every part is a multiple of 16 bytes a unit)
     p.g = (double*)workspace;
     p.e = (float*)workspace + units * 128;
-    p.s0 = p.e + units * 128;
+    p.s0 = p.e + units * 4;
     p.k_end = p.s0 + units * vp * kp;
     p.u = p.k_end + units * 64 * kp;
     p.w = p.u + units * 64 * vp;

@@ -13,6 +13,8 @@ mirrors the reference's ``flash_moe`` interface for this path:
   shared_expert   SharedExpert
   layer_store     ExpertLayer (stacked GGUF expert tensors in HBM)
   moe_gpu         MoeRunner (device-tensor fused calls)
+  kv_cache        PagedCache (paged key/value cache, attention over it)
+  linear_attention  LinearState (recurrent states of many sequences: prompts and steps)
 
 Importing the package does not load the library; the first call does, and
 raises if it is missing.
