@@ -281,3 +281,97 @@ def test_captured_replayed_and_other_streams(single):
             assert torch.equal(c.attend(other, table, lengths, **kw), want2)
             assert torch.equal(y, w)
     assert c.status() == 0
+
+
+@pytest.mark.parametrize("cache,qt,heads,kv_heads,dim", [
+    (torch.float16, torch.float16, 32, 4, 64), (torch.int8, torch.bfloat16, 32, 4, 64),
+    (torch.bfloat16, torch.bfloat16, 24, 8, 128), (torch.int8, torch.float16, 32, 4, 256)], ids=str)
+def test_a_prompt_of_thousands_of_keys_a_workgroup(cache, qt, heads, kv_heads, dim):
+    """Enough rows that the keys are not split: a workgroup goes through more pages than a wavefront has lanes."""
+    p = problem([2311], [2400], heads, kv_heads, dim, 16, cache, qt, seed=1)
+    c = cache_of(p)
+    got = call(c, p)
+    assert c.status() == 0
+    # some of the rows, the first and the last among them
+    keep = torch.tensor([0, 1, 700, 1023, 1024, 1500, 2048, 2309, 2310])
+    for i in keep.tolist():
+        n = 2400 - 2310 + i
+        want, bound = ref.attend(p["q"][i:i + 1], p["k"][0][:n], p["v"][0][:n], dim ** -0.5, cache)
+        assert ((got[i:i + 1].cpu().double() - want).abs() <= bound).all(), i
+
+
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+def test_single_tokens_of_thousands_of_keys_a_workgroup(cache, qt):
+    """Enough sequences that the keys are not split (they share pages): a wavefront goes through more blocks than it has
+    lanes."""
+    p = problem([1], [9001], 8, 8, 64, 16, cache, qt, seed=2)
+    c = cache_of(p)
+    seqs = 600
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(seqs, 8, 64, generator=g).to(qt)
+    lengths = torch.full((seqs,), 9001, dtype=torch.int32)
+    lengths[5], lengths[77], lengths[599] = 8193, 0, 8190
+    table = p["table"].expand(seqs, -1).contiguous()
+    got = c.attend(q.cuda(), table.cuda(), lengths.cuda()).cpu()
+    assert c.status() == 0 and not got[77].any()
+    for b in (0, 5, 300, 599):
+        n = int(lengths[b])
+        want, bound = ref.attend(q[b:b + 1], p["k"][0][:n], p["v"][0][:n], 64 ** -0.5, cache)
+        assert ((got[b:b + 1].double() - want).abs() <= bound).all(), b
+
+
+@pytest.mark.parametrize("single", [False, True])
+def test_pages_past_32_bits_of_offset(single):
+    from flash_moe_hip.kv_cache import PagedCache
+
+    pages = 2 ** 32 // (64 * 128) + 9   # elements past 2^32
+    n = 1 if single else 7
+    p = problem([n], [200], 2, 1, 128, 64, torch.int8, torch.bfloat16, seed=3)
+    k = torch.empty(pages, 1, 64, 128, dtype=torch.int8, device="cuda")
+    scale = torch.empty(pages, 1, 64, device="cuda")
+    big = PagedCache(k, torch.empty_like(k), scale, torch.empty_like(scale))
+    far = torch.tensor([[pages - 1, pages - 3, 0, pages // 2]], dtype=torch.int32)
+    for b in range(4):
+        for t, s in zip((big.k, big.v, big.k_scale, big.v_scale), p["cache"]):
+            t[int(far[0, b])] = s[int(p["table"][0, b])]
+    p["table"] = far
+    check(call(big, p, single=single), p, 128 ** -0.5, torch.int8)
+    assert big.status() == 0
+
+
+def test_refusals():
+    """Arguments the Python call refuses before anything is enqueued."""
+    p = problem([2, 3], [30, 40], 4, 2, 64, 16, torch.float16, torch.float16)
+    c = cache_of(p)
+    q, table, lengths, starts = (t.cuda() for t in (p["q"], p["table"], p["lengths"], p["starts"]))
+    bad = [
+        ((q.float(), table, lengths, starts), {}, "expected one of"),
+        ((q.bfloat16(), table, lengths, starts), {}, "expected one of"),
+        ((q[:, :3], table, lengths, starts), {}, "times the cache"),
+        ((q[:, :, :32], table, lengths, starts), {}, "shape"),
+        ((q.cpu(), table, lengths, starts), {}, "is on cpu"),
+        ((q, table.long(), lengths, starts), {}, "page_table"),
+        ((q, table.cpu(), lengths, starts), {}, "page_table"),
+        ((q, table[:, :0], lengths, starts), {}, "no columns"),
+        ((q, table, lengths.long(), starts), {}, "lengths"),
+        ((q, table, lengths, starts[:2]), {}, "starts"),
+        ((q, table, lengths, None), {}, "one query a sequence"),
+        ((q, table, lengths, starts), dict(scale=0.0), "scale"),
+        ((q, table, lengths, starts), dict(scale=math.nan), "scale"),
+        ((q, table, lengths, starts), dict(out=torch.empty_like(q).float()), "expected one of"),
+        ((q, table, lengths, starts), dict(out=torch.empty(5, 4, 128, dtype=q.dtype, device="cuda")[:, :, :64]),
+         "contiguous"),
+        ((q.clone().requires_grad_(), table, lengths, starts), {}, "no backward"),
+    ]
+    for args, kw, why in bad:
+        with pytest.raises(ValueError, match=why):
+            c.attend(*args, **kw)
+    rows, slots = torch.zeros(3, 2, 64, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    for args, why in (((rows, rows.half(), slots), "expected one of"), ((rows, rows[:2], slots), "shape"),
+                      ((rows, rows, slots.int()), "slots"), ((rows.double(), rows.double(), slots), "expected one of"),
+                      ((rows.transpose(0, 2), rows, slots), "shape"), ((rows, rows, slots.cpu()), "is on cpu")):
+        with pytest.raises(ValueError, match=why):
+            c.write(*args)
+    with pytest.raises(ValueError, match="rows are read"):
+        c.read(slots, dtype=torch.int8)
+    assert c.status() == 0
