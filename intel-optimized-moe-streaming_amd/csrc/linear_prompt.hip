@@ -13,10 +13,10 @@
 //                      U = (1 + L)^-1 diag(beta) V - W S0^T, then S1
 //   3 k_linear_out     chunks in parallel: O
 // Everything is FP32, on FP32 matrix instructions (16x16x4; the outputs on BF16 ones
-// over exact planes, below); the sums G are taken in double, so that differences of far gates keep their digits, and a gate
-// below -1e4 counts as that (its exponential is 0 either way).  The triangular
-// system is solved by substitution, block by block of 16 rows: powers of L would
-// cancel where keys repeat.
+// over exact planes, below).  The sums G are taken in double, so that differences of
+// far gates keep their digits, and a gate below -1e4 counts as that (its exponential
+// is 0 either way).  The triangular system is solved by substitution, block by block
+// of 16 rows: powers of L would cancel where keys repeat.
 //
 // Operand layout.  The 16x16x4 instruction leaves row 4 g + r, column l % 16 of
 // its result in register r of lane l = 16 g + l % 16, and takes element (row or

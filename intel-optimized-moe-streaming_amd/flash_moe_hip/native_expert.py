@@ -143,7 +143,8 @@ class DeltaState:
         value_dim] of one type (FP32, FP16 or BF16), beta and gate [tokens, heads]
         FP32; the state is updated and [tokens, heads, value_dim] returned.  FP32
         sums in an order of their own, where ``step`` has the reference's bit for
-        bit.  key_dim a multiple of 4 up to 256, value_dim one up to 1024."""
+        bit.  key_dim a multiple of 4 up to 256, value_dim one up to 1024.  A call
+        takes a workspace from torch's allocator, about 1 GiB for the longest."""
         from .kv_cache import OnStream
         from .linear_attention import check_dims, prefill_states
 
