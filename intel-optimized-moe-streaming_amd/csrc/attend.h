@@ -10,6 +10,15 @@ namespace mqh {
 constexpr float ATTEND_GROWTH = 8.0f;   // how far (in log2) a row's probabilities may grow past 1 before the
                                         // reference exponent moves and the sums are scaled down
 
+// 8-bit caches: what stands for the scale of a value row of zeros.  Its codes add
+// nothing, so any number gives the right products, but its logarithm takes part in the
+// reference exponent, by which all products are rounded (with 1 values of 1e-3 beside a
+// zero row whose score leads by 10 were off by a fifth), and its probability comes back
+// by the reciprocal.  At 2^-80 a zero row leads only where its weight leaves nothing of
+// the others, for values from 1e-22 on, and its own weight is lost only below 2^-46 vs
+// of the largest, vs the largest product's scale.
+constexpr float ATTEND_ZERO_SCALE = 0x1p-80f;
+
 hipError_t launch_attend(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_token(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_join(const AttendParams& p, hipStream_t s);

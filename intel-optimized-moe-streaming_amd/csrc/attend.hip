@@ -252,7 +252,7 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
         }
         if constexpr (Q8) {
             if (wave == 0 && lane < STEP) {
-                const float vs = sv > 0.0f ? sv : 1.0f;   // (codes of a zero row are zero; NaN: the logarithm stays NaN)
+                const float vs = sv >= KV_MIN_SCALE ? sv : ATTEND_ZERO_SCALE;   // (NaN: the logarithm stays NaN)
                 s_kscale[buf][lane] = sk * p.scale_log2;
                 s_vlog[buf][lane] = sv != sv ? sv : __builtin_log2f(vs);
                 s_vinv[buf][lane] = 1.0f / vs;

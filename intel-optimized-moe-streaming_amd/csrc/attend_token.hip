@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
                 for (int e = 0; e < 4; ++e) {
                     float t;
                     if constexpr (Q8) {
-                        const float sv = vs4[j][e], vs = sv > 0.0f ? sv : 1.0f;
+                        const float sv = vs4[j][e], vs = sv >= KV_MIN_SCALE ? sv : ATTEND_ZERO_SCALE;
                         t = fmaf(s[j][e] * ks4[j][e], q_scale, sv != sv ? sv : __builtin_amdgcn_logf(vs));
                         vinv[j][e] = __builtin_amdgcn_rcpf(vs);
                     } else {

@@ -23,8 +23,6 @@
 
 namespace mqh {
 
-constexpr float KV_MIN_SCALE = 0x1p-100f;
-
 // the largest of `v` over the GROUP neighbouring lanes of this lane's row
 template <int GROUP>
 __device__ __forceinline__ uint32_t row_max(uint32_t v) {

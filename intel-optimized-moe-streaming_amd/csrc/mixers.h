@@ -13,6 +13,9 @@ namespace mqh {
 // (MQH_MIX_F32, _F16, _BF16, _Q8)
 enum : int { MIX_F32 = 0, MIX_F16 = 1, MIX_BF16 = 2, MIX_Q8 = 3 };
 
+// the least scale of an 8-bit cache's row; a row below it is stored as zeros, its scale 0
+constexpr float KV_MIN_SCALE = 0x1p-100f;
+
 inline int mix_bytes(int t) { return t == MIX_F32 ? 4 : t == MIX_Q8 ? 1 : 2; }
 
 struct KvParams {

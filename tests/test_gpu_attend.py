@@ -375,3 +375,50 @@ def test_refusals():
     with pytest.raises(ValueError, match="rows are read"):
         c.read(slots, dtype=torch.int8)
     assert c.status() == 0
+
+
+def with_zero_rows(p, rows, lead, zeros, scale, page):
+    """The problem's int8 cache anew from `rows` (keys and values of one sequence), the value rows `zeros` all
+    zero and their keys ahead of the others by `lead` in every score: channel 0 of every query is 8, and of
+    these keys alone it is not 0."""
+    k, v = rows
+    k[:, :, 0] = 0
+    k[zeros], v[zeros] = 0, 0
+    k[zeros, :, 0] = lead / (8 * scale)
+    p["q"][:, :, 0] = 8
+    pages = p["cache"][0].shape[0]
+    kc, ks, p["k"] = ref.paged([k], p["table"], page, pages, torch.int8)
+    vc, vs, p["v"] = ref.paged([v], p["table"], page, pages, torch.int8)
+    p["cache"] = [t.cuda() for t in (kc, vc, ks, vs)]
+
+
+@pytest.mark.parametrize("qt", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("new,length,dim", [(1, 700, 64), (1, 5000, 128), (1, 300, 256), (37, 700, 64), (20, 1024, 128),
+                                            (3, 5000, 256)])
+def test_zero_value_rows_weigh_in_the_softmax_only(new, length, dim, qt):
+    """Value rows of zeros in an int8 cache, with scores level with the others' and ahead of them, beside small and
+    large values: the other rows' products keep their bits."""
+    scale = dim ** -0.5
+    g = torch.Generator().manual_seed(length)
+    for v_scale in (1.0, 0.05, 1e-3, 1e-5, 1e-8, 1e-12, 1e3):
+        for lead in (0.0, 5.0, 15.0):
+            print(new, length, dim, qt, v_scale, lead, flush=True)
+            p = problem([new], [length], 4, 2, dim, 32, torch.int8, qt, seed=length)
+            k, v = (torch.randn(length, 2, dim, generator=g) for _ in range(2))
+            zeros = torch.tensor([0, 1, length // 2, length - new])
+            with_zero_rows(p, (k, v * v_scale), lead, zeros, scale, 32)
+            c = cache_of(p)
+            got = call(c, p, single=new == 1)
+            if qt == torch.float16 and v_scale < 1e-6:   # (FP16 outputs are zeros then: nothing to see)
+                continue
+            check(got, p, scale, torch.int8)
+            assert c.status() == 0
+
+
+@pytest.mark.parametrize("new", [1, 9])
+def test_values_of_zero_alone(new):
+    p = problem([new], [3000], 4, 2, 64, 32, torch.int8, torch.bfloat16, seed=1)
+    g = torch.Generator().manual_seed(1)
+    with_zero_rows(p, [torch.randn(3000, 2, 64, generator=g) for _ in range(2)], 1.0, torch.arange(3000), 0.125, 32)
+    c = cache_of(p)
+    assert not call(c, p, single=new == 1).any() and c.status() == 0
