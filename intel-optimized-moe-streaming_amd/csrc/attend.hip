@@ -424,7 +424,7 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 y[e] = o[d][4 * r4 + e] * inv;
-                finite &= __builtin_isfinite(y[e]);
+                finite &= fits<QT>(y[e]);
             }
             const int c = 32 * d + 8 * r4 + 4 * half;
             if constexpr (QT == MIX_F16)
@@ -488,7 +488,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendParams p) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         const float x = sum[e] * inv;
-        finite &= __builtin_isfinite(x);
+        finite &= fits<QT>(x);
         if constexpr (QT == MIX_F16) y[e] = __builtin_bit_cast(uint16_t, (_Float16)x);
         else y[e] = __builtin_bit_cast(uint16_t, (__bf16)x);
     }

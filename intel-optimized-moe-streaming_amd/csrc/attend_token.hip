@@ -298,7 +298,7 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             sum[e] *= inv;
-            finite &= __builtin_isfinite(sum[e]);
+            finite &= fits<QT>(sum[e]);
         }
         uint16_t* out = (uint16_t*)p.out + out_row * DIM + c;
         if constexpr (QT == MIX_F16)

@@ -73,7 +73,7 @@ __device__ __forceinline__ void write_row(const KvParams& p, const float (&x)[8]
     } else {
         // (an FP32 value past the cache's range becomes infinite: a fault as well)
         store8<CACHE>(cache, dst * DIM + lane * 8, x);
-        if (top >= (CACHE == MIX_F16 ? 0x477ff000u : 0x7f7f8000u)) atomicOr(&p.flags[FLAG_NONFINITE], 1);
+        if (top >= FIRST_INFINITE<CACHE>) atomicOr(&p.flags[FLAG_NONFINITE], 1);
     }
 }
 

@@ -730,7 +730,7 @@ __global__ __launch_bounds__(THREADS, KP == 256 ? 2 : 4) void k_linear_out(Linea
                 const int t = 16 * i + 4 * g + r;
                 if (t < c.count && row_live) {
                     store1<TYPE>(p.out, ((int64_t)(c.first + t) * p.heads + head) * p.value_dim + row, acc[i][r]);
-                    finite &= __builtin_isfinite(acc[i][r]);
+                    finite &= fits<TYPE>(acc[i][r]);
                 }
             }
     }

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void k_linear_step(LinearParams p) {
         if (lane % LANES == 0) {
             const float out = fmaf(u, kq, decay * sq);
             store1<TYPE>(p.out, sh * p.value_dim + row, out);
-            finite &= __builtin_isfinite(out);
+            finite &= fits<TYPE>(out);
         }
     }
     if (!finite) atomicOr(&p.flags[FLAG_NONFINITE], 1);

@@ -175,6 +175,15 @@ __device__ __forceinline__ void store1(void* base, int64_t at, float x) {
     else ((__bf16*)base)[at] = (__bf16)x;
 }
 
+// whether x, rounded to a type, is finite there (NaN and infinity are not): the bits of
+// the least magnitude that rounds to infinity (half a step past the largest number)
+template <int TYPE>
+constexpr uint32_t FIRST_INFINITE = TYPE == MIX_F16 ? 0x477ff000u : TYPE == MIX_BF16 ? 0x7f7f8000u : 0x7f800000u;
+template <int TYPE>
+__device__ __forceinline__ bool fits(float x) {
+    return (__float_as_uint(x) & 0x7fffffffu) < FIRST_INFINITE<TYPE>;
+}
+
 // eight FP32 values to a row, each rounded once (to nearest, ties to even)
 template <int TYPE>
 __device__ __forceinline__ void store8(void* base, int64_t at, const float (&x)[8]) {

@@ -422,3 +422,19 @@ def test_values_of_zero_alone(new):
     with_zero_rows(p, [torch.randn(3000, 2, 64, generator=g) for _ in range(2)], 1.0, torch.arange(3000), 0.125, 32)
     c = cache_of(p)
     assert not call(c, p, single=new == 1).any() and c.status() == 0
+
+
+@pytest.mark.parametrize("new,length", [(1, 40), (1, 5000), (9, 40), (9, 5000)])
+@pytest.mark.parametrize("qt,value", [(torch.float16, 1e5), (torch.bfloat16, 3.399e38)], ids=str)
+def test_outputs_their_type_cannot_hold_are_reported(new, length, qt, value):
+    """FP32 sums that are finite and round to infinity, whole and joined from splits."""
+    p = problem([new], [length], 2, 1, 64, 32, torch.int8, qt, seed=2)
+    vc, vs = p["cache"][1], p["cache"][3]
+    vc.fill_(100)
+    vc[..., 3] = 127   # channel 3 alone is the value
+    vs.fill_(value / 127)
+    c = cache_of(p)
+    got = call(c, p, single=new == 1)
+    assert got[..., 3].isinf().all() and c.status() == -4
+    vs.fill_(6e4 / 127)
+    assert call(c, p, single=new == 1).isfinite().all() and c.status() == 0

@@ -324,3 +324,30 @@ def test_captured_replayed_and_other_streams(delta):
             assert all(torch.equal(x, y) for x, y in zip((a, b, st.state), w))
             assert all(torch.equal(x, y) for x, y in zip(again, w))
             assert st.status() == 0
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("dtype,value", [(torch.float16, 6e4), (torch.bfloat16, 3.3895e38)], ids=str)
+def test_outputs_their_type_cannot_hold_are_reported(dtype, value, delta):
+    """An FP32 output that is finite and rounds to infinity: writes of two tokens under one query."""
+    from flash_moe_hip.linear_attention import LinearState
+
+    v = torch.zeros(2, 1, 16, dtype=dtype)
+    v[0], v[1, 0, 5] = 1.0, value
+    q, k = torch.zeros(2, 1, 16, dtype=dtype), torch.zeros(2, 1, 16, dtype=dtype)
+    k[0, 0, 0] = k[1, 0, 1] = 1.0   # orthogonal keys: beta 1 writes each value as it is
+    q[:, 0, :2] = 1.0
+    v[0, 0, 5] = value * 0.003 if dtype == torch.bfloat16 else value
+    gate, beta = torch.zeros(2, 1), torch.ones(2, 1) if delta else None
+    rows = cuda([q, k, v, beta, gate])
+    for prompt in (False, True):
+        st = LinearState(1, 1, 16, 16)
+        if prompt:
+            got = st.prefill(*rows)[1]
+        else:
+            got = [st.step(*[None if t is None else t[i:i + 1] for t in rows]) for i in range(2)][1][0]
+        assert st.state.isfinite().all()
+        assert got[0, 5].isinf() and got[0, :5].isfinite().all() and st.status() == -4, prompt
+        st.reset()
+        st.step(*[None if t is None else t[:1] for t in rows])
+        assert st.status() == 0
