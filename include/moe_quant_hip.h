@@ -352,7 +352,8 @@ int mqh_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, 
 
 /* Rows at slots[tokens] as values of `type` (F32, F16 or BF16) into k, v
  * [tokens x kv_heads x dim], contiguous and 16-byte aligned; rows of negative
- * slots and of slots past the cache (-9) are zeros.  Returns 0, -1, -2 or -5. */
+ * slots and of slots past the cache (-9) are zeros; a number that `type` cannot
+ * hold becomes infinite (-4).  Returns 0, -1, -2 or -5. */
 int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc, const float* ks, const float* vs,
                 int cache_type, int64_t pages, int kv_heads, int page_size, int dim, void* k, void* v, int type,
                 int32_t* flags, void* stream);

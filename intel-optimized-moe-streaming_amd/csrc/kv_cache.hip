@@ -147,6 +147,13 @@ __global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
             for (int i = 0; i < 8; ++i) x[n][i] = 0.0f;
             if (slot[n] >= p.n_slots && lane == 0) atomicOr(&p.flags[FLAG_BAD_ID], 1);
         }
+        // a number that becomes infinite here (one that is stored so is no fault of this
+        // call; a code's product with its scale is never stored so)
+        bool fit = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            fit &= fits<TYPE>(x[n][i]) || x[n][i] != x[n][i] || (CACHE != MIX_Q8 && __builtin_isinf(x[n][i]));
+        if (!fit) atomicOr(&p.flags[FLAG_NONFINITE], 1);
         store8<TYPE>((void*)(is_v ? p.v : p.k), (token * p.kv_heads + head) * DIM + lane * 8, x[n]);
     }
 }

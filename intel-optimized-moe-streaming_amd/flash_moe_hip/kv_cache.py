@@ -194,7 +194,8 @@ class PagedCache:
     def read(self, slots, dtype=None, *, stream=None):
         """(k, v) [tokens, kv_heads, head_dim] at `slots` [tokens] int64 as `dtype`
         (the cache's own, FP32 for int8); rows of negative slots are zeros, so are
-        those past the cache, which latch -9."""
+        those past the cache, which latch -9.  A number that `dtype` cannot hold
+        becomes infinite and latches -4."""
         n = self._tokens(slots)
         if dtype is None:
             dtype = self._read_type

@@ -184,3 +184,27 @@ def test_another_stream_and_no_tokens():
     side.synchronize()
     torch.testing.assert_close(k, x, rtol=0, atol=0)
     torch.testing.assert_close(v, x, rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("cache", [torch.bfloat16, torch.int8], ids=str)
+def test_values_a_read_type_cannot_hold_are_reported(cache):
+    """Finite rows read as a narrower type become infinite and say so; rows stored as they are not finite do not."""
+    from flash_moe_hip.kv_cache import PagedCache
+
+    c = PagedCache.empty(2, 1, 128, 16, cache)
+    x = torch.ones(2, 1, 128)
+    x[1, 0, 77] = 1e5
+    slots = torch.tensor([3, 20]).cuda()
+    c.write(x.cuda(), x.cuda(), slots)
+    assert c.status() == 0
+    k, _ = c.read(slots[:1], torch.float16)
+    assert k.isfinite().all() and c.status() == 0
+    for dtype in (torch.float32, torch.bfloat16):
+        assert c.read(slots, dtype)[1].isfinite().all() and c.status() == 0
+    k, v = c.read(slots, torch.float16)
+    assert k[1, 0, 77].isinf() and v[1, 0, 77].isinf() and k[0].isfinite().all() and c.status() == -4
+    x[1, 0, 77] = math.inf
+    c.write(x.cuda(), x.cuda(), slots)
+    assert c.status() == -4
+    c.read(slots, torch.float16)
+    assert c.status() == 0
