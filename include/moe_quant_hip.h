@@ -420,7 +420,10 @@ int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const voi
                        int64_t workspace_bytes, int32_t* flags, void* stream);
 
 /* The calls of this group with their arguments, in order, as 64-bit words (20,
- * 16, 27, 23 and 27; pointers as integers, the scale as the bits of a double). */
+ * 16, 27, 23 and 27; pointers as integers, the scale as the bits of a double).
+ * The linear calls take strides past 2^22 in this form (up to 2^40): all of a step's,
+ * and all of a prompt's but the token strides of q, k and v where it has more than
+ * one token. */
 int mqh_kv_write_words(const int64_t* args);
 int mqh_kv_read_words(const int64_t* args);
 int mqh_attend_words(const int64_t* args);

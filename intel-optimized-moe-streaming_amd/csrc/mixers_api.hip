@@ -2,6 +2,7 @@
 // include/moe_quant_hip.h): the paged key/value cache, attention over it and
 // linear attention.  They validate and enqueue only; nothing is allocated, and
 // no state is kept between calls.
+#include <algorithm>
 #include <initializer_list>
 
 #include "../../include/moe_quant_hip.h"
@@ -75,10 +76,16 @@ bool attend_sizes(int tokens, int seqs, int single, int heads, int kv_heads, int
     return ((int64_t)tokens + seqs) * kv_heads < (int64_t)1 << 31 && (int64_t)tokens * heads * dim < (int64_t)1 << 40;
 }
 
+// The largest strides of the linear calls.  The token strides of q, k and v in a
+// prompt of more than one token: a chunk's offsets are 32-bit.  Every other stride is
+// used in 64 bits; the calls with named arguments keep to the first limit for all of
+// them, as they are documented.
+constexpr int64_t CHUNK_STRIDE_MAX = (int64_t)1 << 22, STRIDE_MAX = (int64_t)1 << 40;
+
 // what both linear calls have to hold
 int check_linear(const void* q, const void* k, const void* v, int type, const float* gate, const float* state,
                  const void* out, int tokens, int seqs, int heads, int key_heads, int key_dim, int value_dim,
-                 const int32_t* flags, std::initializer_list<int64_t> strides) {
+                 const int32_t* flags, int64_t stride_max, std::initializer_list<int64_t> strides) {
     if (!q || !k || !v || !gate || !state || !out || !flags) return ST_ARG;
     if (!row_type(type)) return ST_TYPE;
     if (tokens <= 0 || seqs <= 0 || heads <= 0 || key_heads <= 0 || heads % key_heads || heads > 4096) return ST_ARG;
@@ -88,7 +95,7 @@ int check_linear(const void* q, const void* k, const void* v, int type, const fl
     if (unaligned(q, size) || unaligned(k, size) || unaligned(v, size) || unaligned(out, size)) return ST_ARG;
     if (unaligned(state, 16) || unaligned(gate, 4)) return ST_ARG;
     for (int64_t stride : strides)
-        if (stride < 0 || stride > (int64_t)1 << 22) return ST_ARG;   // (a chunk's offsets are 32-bit)
+        if (stride < 0 || stride > stride_max) return ST_ARG;
     return tokens > 1 << 24 || seqs > 1 << 20 || (int64_t)seqs * heads >= (int64_t)1 << 24 ? ST_ARG : ST_OK;
 }
 
@@ -100,6 +107,65 @@ int64_t linear_pass_chunks(int tokens, int seqs, int heads, int key_dim, int val
     const int64_t all = linear_chunks(tokens, seqs);
     const int64_t one = heads * linear_chunk_floats(linear_kp(key_dim), linear_vp(value_dim), delta) * 4;
     return std::min(all, std::max<int64_t>(8, LINEAR_PASS_BYTES / one));
+}
+
+int linear_step(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                const void* v, int64_t v_token, int64_t v_head, int type, const float* beta, int64_t beta_token,
+                const float* gate, int64_t gate_token, float* state, void* out, int seqs, int heads, int key_heads,
+                int key_dim, int value_dim, int32_t* flags, void* stream, int64_t stride_max) {
+    const int st = check_linear(q, k, v, type, gate, state, out, seqs, seqs, heads, key_heads, key_dim, value_dim, flags,
+                                stride_max, {q_token, q_head, k_token, k_head, v_token, v_head, beta_token, gate_token});
+    if (st) return st;
+    LinearParams p{};
+    p.q = q; p.k = k; p.v = v;
+    p.q_token = q_token; p.q_head = q_head; p.k_token = k_token; p.k_head = k_head;
+    p.v_token = v_token; p.v_head = v_head;
+    p.beta = beta; p.beta_token = beta_token; p.gate = gate; p.gate_token = gate_token;
+    p.state = state; p.out = out; p.type = type;
+    p.tokens = seqs; p.seqs = seqs; p.heads = heads; p.key_heads = key_heads;
+    p.key_dim = key_dim; p.value_dim = value_dim; p.flags = flags;
+    return status(launch_linear_step(p, (hipStream_t)stream));
+}
+
+int linear_prefill(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                   const void* v, int64_t v_token, int64_t v_head, int type, const float* beta, int64_t beta_token,
+                   const float* gate, int64_t gate_token, float* state, void* out, const int32_t* starts,
+                   int tokens, int seqs, int heads, int key_heads, int key_dim, int value_dim, void* workspace,
+                   int64_t workspace_bytes, int32_t* flags, void* stream, int64_t stride_max) {
+    if (tokens == 1) q_token = k_token = v_token = 0;   // (the stride of one token means nothing)
+    const int st = check_linear(q, k, v, type, gate, state, out, tokens, seqs, heads, key_heads, key_dim, value_dim, flags,
+                                stride_max, {q_token, q_head, k_token, k_head, v_token, v_head, beta_token, gate_token});
+    if (st) return st;
+    if (std::max({q_token, k_token, v_token}) > CHUNK_STRIDE_MAX) return ST_ARG;
+    if (!starts && seqs != 1) return ST_ARG;
+    const bool delta = beta != nullptr;
+    const int64_t pass = linear_pass_chunks(tokens, seqs, heads, key_dim, value_dim, delta), units = pass * heads;
+    const int kp = linear_kp(key_dim), vp = linear_vp(value_dim);
+    if (workspace_bytes < units * linear_chunk_floats(kp, vp, delta) * 4) return ST_WORKSPACE;
+    if (!workspace || unaligned(workspace, 256)) return ST_ARG;
+    LinearParams p{};
+    p.q = q; p.k = k; p.v = v;
+    p.q_token = q_token; p.q_head = q_head; p.k_token = k_token; p.k_head = k_head;
+    p.v_token = v_token; p.v_head = v_head;
+    p.beta = beta; p.beta_token = beta_token; p.gate = gate; p.gate_token = gate_token;
+    p.state = state; p.out = out; p.starts = starts; p.type = type;
+    p.tokens = tokens; p.seqs = seqs; p.heads = heads; p.key_heads = key_heads;
+    p.key_dim = key_dim; p.value_dim = value_dim; p.flags = flags;
+    // (every part is a multiple of 16 bytes a unit)
+    p.g = (double*)workspace;
+    p.e = (float*)workspace + units * 128;
+    p.s0 = p.e + units * 4;
+    p.k_end = p.s0 + units * vp * kp;
+    p.u = p.k_end + units * 64 * kp;
+    p.w = p.u + units * 64 * vp;
+    const int64_t all = linear_chunks(tokens, seqs);
+    for (int64_t at = 0; at < all; at += pass) {
+        p.chunk0 = (int)at;
+        p.chunks = (int)std::min(pass, all - at);
+        const hipError_t e = launch_linear_prompt(p, (hipStream_t)stream);
+        if (e != hipSuccess) return ST_HIP;
+    }
+    return ST_OK;
 }
 
 }  // namespace
@@ -190,18 +256,9 @@ int mqh_linear_step(const void* q, int64_t q_token, int64_t q_head, const void* 
                     const void* v, int64_t v_token, int64_t v_head, int type, const float* beta, int64_t beta_token,
                     const float* gate, int64_t gate_token, float* state, void* out, int seqs, int heads, int key_heads,
                     int key_dim, int value_dim, int32_t* flags, void* stream) {
-    const int st = check_linear(q, k, v, type, gate, state, out, seqs, seqs, heads, key_heads, key_dim, value_dim, flags,
-                                {q_token, q_head, k_token, k_head, v_token, v_head, beta_token, gate_token});
-    if (st) return st;
-    LinearParams p{};
-    p.q = q; p.k = k; p.v = v;
-    p.q_token = q_token; p.q_head = q_head; p.k_token = k_token; p.k_head = k_head;
-    p.v_token = v_token; p.v_head = v_head;
-    p.beta = beta; p.beta_token = beta_token; p.gate = gate; p.gate_token = gate_token;
-    p.state = state; p.out = out; p.type = type;
-    p.tokens = seqs; p.seqs = seqs; p.heads = heads; p.key_heads = key_heads;
-    p.key_dim = key_dim; p.value_dim = value_dim; p.flags = flags;
-    return status(launch_linear_step(p, (hipStream_t)stream));
+    return linear_step(q, q_token, q_head, k, k_token, k_head, v, v_token, v_head, type, beta, beta_token, gate,
+                       gate_token, state, out, seqs, heads, key_heads, key_dim, value_dim, flags, stream,
+                       CHUNK_STRIDE_MAX);
 }
 
 int64_t mqh_linear_prefill_workspace_bytes(int tokens, int seqs, int heads, int key_dim, int value_dim, int delta) {
@@ -218,38 +275,9 @@ int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const voi
                        const float* gate, int64_t gate_token, float* state, void* out, const int32_t* starts,
                        int tokens, int seqs, int heads, int key_heads, int key_dim, int value_dim, void* workspace,
                        int64_t workspace_bytes, int32_t* flags, void* stream) {
-    const int st = check_linear(q, k, v, type, gate, state, out, tokens, seqs, heads, key_heads, key_dim, value_dim, flags,
-                                {q_token, q_head, k_token, k_head, v_token, v_head, beta_token, gate_token});
-    if (st) return st;
-    if (!starts && seqs != 1) return ST_ARG;
-    const bool delta = beta != nullptr;
-    const int64_t pass = linear_pass_chunks(tokens, seqs, heads, key_dim, value_dim, delta), units = pass * heads;
-    const int kp = linear_kp(key_dim), vp = linear_vp(value_dim);
-    if (workspace_bytes < units * linear_chunk_floats(kp, vp, delta) * 4) return ST_WORKSPACE;
-    if (!workspace || unaligned(workspace, 256)) return ST_ARG;
-    LinearParams p{};
-    p.q = q; p.k = k; p.v = v;
-    p.q_token = q_token; p.q_head = q_head; p.k_token = k_token; p.k_head = k_head;
-    p.v_token = v_token; p.v_head = v_head;
-    p.beta = beta; p.beta_token = beta_token; p.gate = gate; p.gate_token = gate_token;
-    p.state = state; p.out = out; p.starts = starts; p.type = type;
-    p.tokens = tokens; p.seqs = seqs; p.heads = heads; p.key_heads = key_heads;
-    p.key_dim = key_dim; p.value_dim = value_dim; p.flags = flags;
-    // (every part is a multiple of 16 bytes a unit)
-    p.g = (double*)workspace;
-    p.e = (float*)workspace + units * 128;
-    p.s0 = p.e + units * 4;
-    p.k_end = p.s0 + units * vp * kp;
-    p.u = p.k_end + units * 64 * kp;
-    p.w = p.u + units * 64 * vp;
-    const int64_t all = linear_chunks(tokens, seqs);
-    for (int64_t at = 0; at < all; at += pass) {
-        p.chunk0 = (int)at;
-        p.chunks = (int)std::min(pass, all - at);
-        const hipError_t e = launch_linear_prompt(p, (hipStream_t)stream);
-        if (e != hipSuccess) return ST_HIP;
-    }
-    return ST_OK;
+    return linear_prefill(q, q_token, q_head, k, k_token, k_head, v, v_token, v_head, type, beta, beta_token, gate,
+                          gate_token, state, out, starts, tokens, seqs, heads, key_heads, key_dim, value_dim, workspace,
+                          workspace_bytes, flags, stream, CHUNK_STRIDE_MAX);
 }
 
 // The calls with their arguments, in order, as 64-bit words (pointers as
@@ -258,18 +286,18 @@ int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const voi
 int mqh_linear_step_words(const int64_t* a) {
     if (!a || a[16] != (int)a[16]) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
-    return mqh_linear_step(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10), a[11],
-                           (const float*)P(12), a[13], (float*)P(14), P(15), (int)a[16], (int)a[17], (int)a[18],
-                           (int)a[19], (int)a[20], (int32_t*)P(21), P(22));
+    return linear_step(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10), a[11],
+                       (const float*)P(12), a[13], (float*)P(14), P(15), (int)a[16], (int)a[17], (int)a[18],
+                       (int)a[19], (int)a[20], (int32_t*)P(21), P(22), STRIDE_MAX);
 }
 
 int mqh_linear_prefill_words(const int64_t* a) {
     if (!a || a[17] != (int)a[17] || a[18] != (int)a[18]) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
-    return mqh_linear_prefill(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10),
-                              a[11], (const float*)P(12), a[13], (float*)P(14), P(15), (const int32_t*)P(16),
-                              (int)a[17], (int)a[18], (int)a[19], (int)a[20], (int)a[21], (int)a[22], P(23), a[24],
-                              (int32_t*)P(25), P(26));
+    return linear_prefill(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10),
+                          a[11], (const float*)P(12), a[13], (float*)P(14), P(15), (const int32_t*)P(16), (int)a[17],
+                          (int)a[18], (int)a[19], (int)a[20], (int)a[21], (int)a[22], P(23), a[24], (int32_t*)P(25),
+                          P(26), STRIDE_MAX);
 }
 
 int mqh_kv_write_words(const int64_t* a) {

@@ -26,6 +26,7 @@ from .kv_cache import OnStream, _types, check_index, check_rows
 _STEP_WORDS = struct.Struct("23q")
 _PREFILL_WORDS = struct.Struct("27q")
 KEY_DIM_MAX, VALUE_DIM_MAX = 256, 1024
+CHUNK_STRIDE_MAX = 1 << 22   # a prompt's offsets within a chunk of tokens are 32-bit
 
 
 @functools.lru_cache(maxsize=512)
@@ -39,7 +40,7 @@ def check_dims(key_dim: int, value_dim: int):
                          f"got {key_dim} and {value_dim}")
 
 
-def _inputs(state, n, q, k, v, beta, gate, out):
+def _inputs(state, n, q, k, v, beta, gate, out, prompt):
     """Check one call's rows against the states' shape; the shared argument words."""
     _, heads, dv, dk = state.shape
     index, types = state.get_device(), _types()
@@ -51,6 +52,9 @@ def _inputs(state, n, q, k, v, beta, gate, out):
     like = (v.dtype,)
     qt, qh, _ = check_rows(q, (n, key_heads, dk), like, index, "q")
     kt, kh, _ = check_rows(k, (n, key_heads, dk), like, index, "k")
+    if prompt and n > 1 and max(qt, kt, vt) > CHUNK_STRIDE_MAX:
+        name, stride = max(("q", qt), ("k", kt), ("v", vt), key=lambda t: t[1])
+        raise ValueError(f"{name} has a token stride of {stride} elements; a prompt takes up to {CHUNK_STRIDE_MAX}")
     gt, _ = check_rows(gate, (n, heads), _FP32(), index, "gate")
     bp = bt = 0
     if beta is not None:
@@ -77,7 +81,7 @@ def prefill_states(lib, run, flags, state, q, k, v, beta, gate, starts, out, str
 
     seqs, heads, dv, dk = state.shape
     n = v.shape[0]
-    words, key_heads = _inputs(state, n, q, k, v, beta, gate, out)
+    words, key_heads = _inputs(state, n, q, k, v, beta, gate, out, True)
     if starts is not None:
         check_index(starts, (seqs + 1,), torch.int32, state.get_device(), "starts")
     elif seqs != 1:
@@ -137,7 +141,7 @@ class LinearState:
         no delta rule) and gate [sequences, heads] FP32.  Returns out [sequences,
         heads, value_dim] of v's type."""
         seqs, heads, dv, dk = self.shape
-        words, key_heads = _inputs(self.state, seqs, q, k, v, beta, gate, out)
+        words, key_heads = _inputs(self.state, seqs, q, k, v, beta, gate, out, False)
         return self._run(stream, self._step, v, out, words, (seqs, heads, key_heads, dk, dv))
 
     def _step(self, handle, v, out, words, sizes):
@@ -149,8 +153,8 @@ class LinearState:
         return out
 
     def prefill(self, q, k, v, beta, gate, *, starts=None, out=None, stream=None):
-        """Prompts: the arguments of ``step`` with [tokens, ...] rows; sequence b's
-        are rows starts[b] .. starts[b + 1] - 1 (int32 [sequences + 1] on the device;
+        """Prompts: the arguments of ``step`` with [tokens, ...] rows (token strides of
+        q, k and v up to 2^22 elements); sequence b's are rows starts[b] .. starts[b + 1] - 1 (int32 [sequences + 1] on the device;
         may be omitted for one sequence).  The same states and outputs as ``step``
         token by token up to FP32 rounding; rows of no sequence are left as they
         were.  A value that is not finite also reaches earlier tokens of its

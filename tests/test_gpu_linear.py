@@ -351,3 +351,36 @@ def test_outputs_their_type_cannot_hold_are_reported(dtype, value, delta):
         st.reset()
         st.step(*[None if t is None else t[:1] for t in rows])
         assert st.status() == 0
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_strides_past_32_bits_of_a_chunk(delta):
+    """Steps over one token of a long buffer, prompts with the heads outside the tokens, one token of any stride."""
+    from flash_moe_hip.linear_attention import LinearState
+
+    heads, key_heads, dk, dv, far = 4, 2, 64, 32, 2 ** 22 + 8
+
+    def spread(t, strides):   # the same rows a stride apart
+        at = sum((n - 1) * s for n, s in zip(t.shape, strides)) + t.shape[-1]
+        base = torch.zeros(at, dtype=t.dtype, device="cuda")
+        return base.as_strided(t.shape, strides).copy_(t)
+
+    args = inputs(3, heads, key_heads, dk, dv, torch.bfloat16, delta, seed=5)
+    one, two = LinearState(3, heads, dv, dk), LinearState(3, heads, dv, dk)
+    apart = [None if t is None else spread(t, (far,) + ((far * 4, 1) if t.dim() == 3 else (1,))) for t in args]
+    assert torch.equal(one.step(*cuda(args)), two.step(*apart)) and torch.equal(one.state, two.state)
+
+    args = inputs(100, heads, key_heads, dk, dv, torch.float32, delta, seed=6)
+    q, k, v, beta, gate = args
+    apart = [spread(t, (dim, far, 1)) for t, dim in ((q, dk), (k, dk), (v, dv))]
+    apart += [None if t is None else spread(t, (2 ** 22 + 4, 1)) for t in (beta, gate)]
+    one, two = LinearState(1, heads, dv, dk), LinearState(1, heads, dv, dk)
+    assert torch.equal(one.prefill(*cuda(args)), two.prefill(*apart)) and torch.equal(one.state, two.state)
+
+    rows = cuda([None if t is None else t[:1] for t in args])
+    single = [None if t is None else t.as_strided(t.shape, (2 ** 30,) + t.stride()[1:]) for t in rows]
+    assert torch.equal(one.prefill(*rows), two.prefill(*single))
+    assert torch.equal(one.step(*rows), two.step(*single)) and torch.equal(one.state, two.state)
+    assert one.status() == 0 and two.status() == 0
+    with pytest.raises(ValueError, match="token stride"):
+        one.prefill(*[None if t is None else spread(t[:2], (far,) + t.stride()[1:]) for t in args])

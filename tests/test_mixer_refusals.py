@@ -199,3 +199,49 @@ def test_row_checks():
             check_index(bad, (6,), torch.int32, cpu, "i")
     with pytest.raises(ValueError, match="on cpu"):
         check_index(i, (6,), torch.int32, 0, "i")
+
+
+def rows_of_stride(tokens, heads, dim, token, head):
+    """[tokens, heads, dim] of any strides, without memory."""
+    return torch.empty(0, device="meta").as_strided((tokens, heads, dim), (token, head, 1))
+
+
+def test_strides_of_prompts_that_are_refused_by_name(monkeypatch):
+    """Only a chunk's own token offsets are 32-bit: q, k and v of more than one token."""
+    from flash_moe_hip import linear_attention as la
+
+    far, near = 2 ** 22 + 4, 64
+    state = torch.empty(2, 4, 16, 16, device="meta")
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: 4096)
+
+    def inputs(prompt, n=8, q=near, k=near, v=near, head=16, gate=4):
+        return la._inputs(state, n, rows_of_stride(n, 4, 16, q, head), rows_of_stride(n, 4, 16, k, head),
+                          rows_of_stride(n, 4, 16, v, head), None,
+                          torch.empty(0, device="meta").as_strided((n, 4), (gate, 1)), None, prompt)
+
+    for name in "qkv":
+        with pytest.raises(ValueError, match=f"{name} .*4194304"):
+            inputs(True, **{name: far})
+        inputs(False, n=2, **{name: far})   # a step
+        inputs(True, n=1, **{name: far})    # one token: its stride means nothing
+    inputs(True, head=far, gate=far)
+
+
+def test_strides_that_the_word_forms_refuse(lib):
+    import struct
+
+    p = 4096
+
+    def words(q=64, qh=16, bt=4, **_):
+        return [p, q, qh, p, 64, 16, p, 64, 16, 0, p, bt, p, 4, p, p]
+
+    def step(**kw):
+        return lib.mqh_linear_step_words(struct.pack("23q", *words(**kw), 2, 4, 4, 16, 16, p, 0))
+
+    def prompt(tokens=8, **kw):
+        return lib.mqh_linear_prefill_words(struct.pack("27q", *words(**kw), p, tokens, 2, 4, 4, 16, 16, p, 1 << 30, p, 0))
+
+    for call in (step, prompt):
+        for bad in (dict(q=-1), dict(qh=-1), dict(bt=-1), dict(q=2 ** 41), dict(qh=2 ** 41), dict(bt=2 ** 41)):
+            assert call(**bad) == -1, bad
+    assert prompt(q=2 ** 22 + 1) == -1
