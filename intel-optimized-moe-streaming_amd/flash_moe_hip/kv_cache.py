@@ -132,7 +132,8 @@ class PagedCache:
             raise ValueError("a cache's tensors must be contiguous and on one device")
         if k.device.type != "cuda":
             raise ValueError(f"expected a CUDA device, got {k.device}")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._held = held
+        self._like = [(t.shape, t.dtype, t.device) for t in held]
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, dim
         self.device = k.device
         self.lib = _lib.load()
@@ -144,8 +145,27 @@ class PagedCache:
         self._q_types = (torch.float16, torch.bfloat16) if int8 else (k.dtype,)
         self._read_type = torch.float32 if int8 else k.dtype
         self._flags = torch.zeros(64, dtype=torch.int32, device=k.device)
-        scales = (k_scale.data_ptr(), v_scale.data_ptr()) if len(held) == 4 else (0, 0)
-        self._words = (k.data_ptr(), v.data_ptr(), *scales, types[k.dtype], pages, kv_heads, page_size, dim)
+        self._at = [t.data_ptr() for t in held]
+        self._sizes = (types[k.dtype], pages, kv_heads, page_size, dim)
+
+    # (a call's addresses and sizes are those of the tensors checked here: no others can be put in their place)
+    k = property(lambda self: self._held[0], doc="The keys [pages, kv_heads, page_size, head_dim].")
+    v = property(lambda self: self._held[1], doc="The values, as the keys.")
+    k_scale = property(lambda self: self._held[2] if len(self._held) == 4 else None,
+                       doc="An int8 cache's scales [pages, kv_heads, page_size].")
+    v_scale = property(lambda self: self._held[3] if len(self._held) == 4 else None, doc="The values' scales.")
+
+    def _words(self):
+        """The cache's share of a call's words, at the addresses its tensors have now
+        (their storage may have moved)."""
+        at = [t.data_ptr() for t in self._held]
+        if at != self._at:
+            for t, (shape, dtype, device) in zip(self._held, self._like):
+                if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous() or (
+                        t.untyped_storage().nbytes() < (t.storage_offset() + t.numel()) * t.element_size()):
+                    raise ValueError(f"a tensor of the cache is no longer {dtype} {tuple(shape)}, contiguous, on {device}")
+            self._at = at
+        return (*at, *self._sizes) if len(at) == 4 else (*at, 0, 0, *self._sizes)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dtype=None, device="cuda"):
@@ -179,7 +199,7 @@ class PagedCache:
         vt, vh, _ = check_rows(v, shape, (k.dtype,), self._index, "v")
         if n:
             self._run(stream, self._write, (k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, self._types[k.dtype],
-                                            slots.data_ptr(), n, *self._words, self._flags.data_ptr()))
+                                            slots.data_ptr(), n, *self._words(), self._flags.data_ptr()))
 
     def _write(self, handle, words):
         rc = self.lib.mqh_kv_write_words(_WRITE_WORDS.pack(*words, handle))
@@ -208,7 +228,7 @@ class PagedCache:
         k, v = rows.unbind()
         if n:
             rc = self.lib.mqh_kv_read_words(_READ_WORDS.pack(
-                slots.data_ptr(), n, *self._words, k.data_ptr(), v.data_ptr(), self._types[dtype],
+                slots.data_ptr(), n, *self._words(), k.data_ptr(), v.data_ptr(), self._types[dtype],
                 self._flags.data_ptr(), handle))
             if rc:
                 _lib.check(rc, "mqh_kv_read")
@@ -265,7 +285,7 @@ class PagedCache:
                 _lib.check(need, "mqh_attend_workspace_bytes")
         return self._run(stream, self._attend, q, out, need, (
             q.data_ptr(), qt, qh, self._types[q.dtype], tokens, starts.data_ptr() if starts is not None else 0, seqs,
-            heads, *self._words, page_table.data_ptr(), row if seqs > 1 else cols, cols, lengths.data_ptr(), scale))
+            heads, *self._words(), page_table.data_ptr(), row if seqs > 1 else cols, cols, lengths.data_ptr(), scale))
 
     def _attend(self, handle, q, out, need, words):
         if out is None:

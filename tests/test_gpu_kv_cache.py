@@ -208,3 +208,37 @@ def test_values_a_read_type_cannot_hold_are_reported(cache):
     assert c.status() == -4
     c.read(slots, torch.float16)
     assert c.status() == 0
+
+
+@pytest.mark.parametrize("cache", [torch.float16, torch.int8], ids=str)
+def test_a_cache_follows_its_tensors(cache):
+    """The tensors cannot be exchanged for others; one whose storage moves is written and read where it lies."""
+    from flash_moe_hip.kv_cache import PagedCache
+
+    c = PagedCache.empty(2, 1, 64, 16, cache)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name))
+    x = rows(1, 1, 64, torch.float16, 1)
+    slots = torch.tensor([17]).cuda()
+    c.write(x, x, slots)
+    before = c.k.detach()          # keeps the old memory
+    kept = before.clone()
+    c.k.set_(torch.zeros_like(c.k))
+    c.write(2 * x, 2 * x, slots)
+    assert torch.equal(before, kept) and c.k.any()
+    k, v = c.read(slots)
+    assert torch.equal(k, v) and c.status() == 0
+    for moved in (torch.zeros(1, 1, 16, 64, dtype=cache), torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16),
+                  torch.zeros(2, 1, 64, 16, dtype=cache).transpose(2, 3), torch.zeros(0, dtype=cache)):
+        moved = moved.cuda() if moved.is_contiguous() else moved.transpose(2, 3).cuda().transpose(2, 3)
+        c = PagedCache.empty(2, 1, 64, 16, cache)
+        c.v.data = moved
+        for call in (lambda: c.write(x, x, slots), lambda: c.read(slots)):
+            with pytest.raises(ValueError, match="no longer"):
+                call()
+    c = PagedCache.empty(2, 1, 64, 16, cache)
+    c.k.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="no longer"):
+        c.attend(torch.zeros(1, 1, 64, dtype=torch.float16, device="cuda"), torch.zeros(1, 1, dtype=torch.int32,
+                 device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda"))
