@@ -21,7 +21,7 @@ import functools
 import struct
 
 from . import _lib
-from .kv_cache import OnStream, _types, check_index, check_rows
+from .kv_cache import OnStream, _device_name, _types, check_index, check_rows
 
 _STEP_WORDS = struct.Struct("23q")
 _PREFILL_WORDS = struct.Struct("27q")
@@ -38,6 +38,16 @@ def check_dims(key_dim: int, value_dim: int):
     if key_dim < 4 or key_dim > KEY_DIM_MAX or key_dim % 4 or value_dim < 4 or value_dim > VALUE_DIM_MAX or value_dim % 4:
         raise ValueError(f"key_dim must be a multiple of 4 up to {KEY_DIM_MAX}, value_dim one up to {VALUE_DIM_MAX}; "
                          f"got {key_dim} and {value_dim}")
+
+
+def check_state(state, shape, index):
+    """The state a call is about to update in place is still the one its object was made
+    for: FP32 of its shape, contiguous, on CUDA device `index` (-1: the CPU)."""
+    if state.shape == shape and state.dtype is _FP32()[0] and state.is_contiguous() and not state.requires_grad:
+        if state.get_device() != index:
+            raise ValueError(f"the state is on {state.device}, expected {_device_name(index)}")
+        return
+    raise ValueError(f"the state must be a contiguous FP32 tensor of shape {tuple(shape)} without grad")
 
 
 def _inputs(state, n, q, k, v, beta, gate, out, prompt):
@@ -128,7 +138,7 @@ class LinearState:
         if self.state.device.type != "cuda":
             raise ValueError(f"expected a CUDA device, got {self.state.device}")
         self.lib = _lib.load()
-        self._run, self._empty = OnStream(self.state.device), torch.empty
+        self._run, self._empty, self._index = OnStream(self.state.device), torch.empty, self.state.get_device()
         self._flags = torch.zeros(64, dtype=torch.int32, device=self.state.device)
 
     def reset(self):
@@ -141,6 +151,7 @@ class LinearState:
         no delta rule) and gate [sequences, heads] FP32.  Returns out [sequences,
         heads, value_dim] of v's type."""
         seqs, heads, dv, dk = self.shape
+        check_state(self.state, self.shape, self._index)
         words, key_heads = _inputs(self.state, seqs, q, k, v, beta, gate, out, False)
         return self._run(stream, self._step, v, out, words, (seqs, heads, key_heads, dk, dv))
 
@@ -159,6 +170,7 @@ class LinearState:
         token by token up to FP32 rounding; rows of no sequence are left as they
         were.  A value that is not finite also reaches earlier tokens of its
         64-token chunk."""
+        check_state(self.state, self.shape, self._index)
         return prefill_states(self.lib, self._run, self._flags, self.state, q, k, v, beta, gate, starts, out, stream)
 
     def status(self, stream=None) -> int:

@@ -146,10 +146,11 @@ class DeltaState:
         bit.  key_dim a multiple of 4 up to 256, value_dim one up to 1024.  A call
         takes a workspace from torch's allocator, about 1 GiB for the longest."""
         from .kv_cache import OnStream
-        from .linear_attention import check_dims, prefill_states
+        from .linear_attention import check_dims, check_state, prefill_states
 
         nv, dv, dk = self.shape
         check_dims(dk, dv)
+        check_state(self.state, self.shape, self._flags.get_device())
         if self.state.get_device() < 0:
             raise ValueError(f"expected a CUDA device, got {self.state.device}")
         return prefill_states(self.lib, OnStream(self.state.device), self._flags, self.state.view(1, nv, dv, dk), q, k,

@@ -245,3 +245,31 @@ def test_strides_that_the_word_forms_refuse(lib):
         for bad in (dict(q=-1), dict(qh=-1), dict(bt=-1), dict(q=2 ** 41), dict(qh=2 ** 41), dict(bt=2 ** 41)):
             assert call(**bad) == -1, bad
     assert prompt(q=2 ** 22 + 1) == -1
+
+
+def test_states_put_in_place_of_the_checked_one():
+    """A state of another shape, type, device or layout than the object was made for is refused at the call."""
+    from flash_moe_hip.linear_attention import LinearState
+    from flash_moe_hip.native_expert import DeltaState
+
+    good = torch.zeros(2, 4, 16, 16)
+    rows = [torch.zeros(2, 4, 16) for _ in range(3)] + [None, torch.zeros(2, 4)]
+    for bad in (good[:1], torch.zeros(2, 4, 16, 8), good.half(), good.transpose(2, 3).contiguous().transpose(2, 3),
+                good.clone().requires_grad_()):
+        st = LinearState.__new__(LinearState)   # (a CPU has none to make)
+        st.shape, st._index, st.state = (2, 4, 16, 16), 0, bad
+        for call in (st.step, st.prefill):
+            with pytest.raises(ValueError, match="the state must be"):
+                call(*rows)
+    st.state = good
+    with pytest.raises(ValueError, match="on cuda:0"):
+        st.step(*rows)
+    one = [t if t is None else t[:1] for t in rows]
+    for bad in (torch.zeros(4, 16, 8), good[:, 0], good[0].half(), good[0].transpose(1, 2), torch.zeros(4, 256)):
+        ds = DeltaState.__new__(DeltaState)
+        ds.shape, ds._flags, ds.state = (4, 16, 16), torch.zeros(64, dtype=torch.int32), bad
+        with pytest.raises(ValueError, match="the state must be"):
+            ds.prefill(*one)
+    ds.state = good[0]
+    with pytest.raises(ValueError, match="CUDA device"):
+        ds.prefill(*one)
