@@ -262,7 +262,7 @@ def test_states_put_in_place_of_the_checked_one():
             with pytest.raises(ValueError, match="the state must be"):
                 call(*rows)
     st.state = good
-    with pytest.raises(ValueError, match="on cuda:0"):
+    with pytest.raises(ValueError, match="expected cuda:0"):
         st.step(*rows)
     one = [t if t is None else t[:1] for t in rows]
     for bad in (torch.zeros(4, 16, 8), good[:, 0], good[0].half(), good[0].transpose(1, 2), torch.zeros(4, 256)):
