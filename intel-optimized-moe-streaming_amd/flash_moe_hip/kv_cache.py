@@ -74,7 +74,8 @@ def check_index(t, shape, dtype, index, what):
 
 class OnStream:
     """Runs a call on a device: with it current and the handle of its current
-    stream, or of the stream given, which the call's tensors are then allocated on."""
+    stream, or of the stream given (of the same device), which the call's tensors
+    are then allocated on."""
 
     def __init__(self, device):
         import torch
@@ -86,6 +87,8 @@ class OnStream:
 
     def __call__(self, stream, call, *args):
         if stream is not None:
+            if stream.device.index != self.index:
+                raise ValueError(f"the stream is on {stream.device}, expected {_device_name(self.index)}")
             with self._torch.cuda.stream(stream):
                 return call(stream.cuda_stream, *args)
         if self._current() != self.index:
@@ -301,8 +304,4 @@ class PagedCache:
     def status(self, stream=None) -> int:
         """Synchronizes; 0, -4 (a value that is not finite) or -9 (a slot, page,
         length or start out of range) since the last call."""
-        import torch
-
-        if stream is None:
-            stream = torch.cuda.current_stream(self.device)
-        return int(self.lib.mqh_status(self._flags.data_ptr(), stream.cuda_stream))
+        return int(self._run(stream, lambda handle: self.lib.mqh_status(self._flags.data_ptr(), handle)))

@@ -176,8 +176,4 @@ class LinearState:
     def status(self, stream=None) -> int:
         """Synchronizes; 0, -4 (an output was not finite) or -9 (starts out of
         range) since the last call."""
-        import torch
-
-        if stream is None:
-            stream = torch.cuda.current_stream(self.state.device)
-        return int(self.lib.mqh_status(self._flags.data_ptr(), stream.cuda_stream))
+        return int(self._run(stream, lambda handle: self.lib.mqh_status(self._flags.data_ptr(), handle)))

@@ -273,3 +273,55 @@ def test_states_put_in_place_of_the_checked_one():
     ds.state = good[0]
     with pytest.raises(ValueError, match="CUDA device"):
         ds.prefill(*one)
+
+
+def test_streams_of_another_device(monkeypatch):
+    """A launch goes to its stream's device: that has to be the tensors'."""
+    from types import SimpleNamespace
+
+    from flash_moe_hip.kv_cache import OnStream
+
+    run = OnStream(torch.device("cuda", 0))
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: pytest.fail("the call went on"))
+    with pytest.raises(ValueError, match="stream is on cuda:1, expected cuda:0"):
+        run(SimpleNamespace(device=torch.device("cuda", 1), cuda_stream=0), lambda handle: None)
+    from flash_moe_hip.linear_attention import LinearState
+    from flash_moe_hip.native_expert import DeltaState
+    from flash_moe_hip.kv_cache import PagedCache
+
+    for cls in (PagedCache, LinearState):
+        x = cls.__new__(cls)
+        x._run = run
+        x._flags, x.lib = torch.zeros(64, dtype=torch.int32), None
+        with pytest.raises(ValueError, match="expected cuda:0"):
+            x.status(SimpleNamespace(device=torch.device("cuda", 1), cuda_stream=0))
+
+
+def test_status_on_the_objects_device(monkeypatch):
+    """A default stream's handle is 0 on every device: the object's is made current for the wait and the copy."""
+    from contextlib import contextmanager
+    from types import SimpleNamespace
+
+    from flash_moe_hip.kv_cache import OnStream, PagedCache
+    from flash_moe_hip.linear_attention import LinearState
+
+    seen, now = [], [1]
+
+    @contextmanager
+    def device(index):
+        was, now[0] = now[0], index
+        yield
+        now[0] = was
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(cuda_stream=0))
+    run = OnStream(torch.device("cuda", 0))
+    run._stream_of = lambda index: 0
+    for cls in (PagedCache, LinearState):
+        x = cls.__new__(cls)
+        x._run, x._flags, x.device = run, torch.zeros(64, dtype=torch.int32), torch.device("cuda", 0)
+        x.state = SimpleNamespace(device=x.device)
+        x.lib = SimpleNamespace(mqh_status=lambda flags, handle: seen.append(now[0]) or 0)
+        assert x.status() == 0
+    assert seen == [0, 0] and now == [1]
