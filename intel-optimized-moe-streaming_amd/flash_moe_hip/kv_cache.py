@@ -133,6 +133,8 @@ class PagedCache:
             raise ValueError("only int8 caches have scales")
         if any(t.device != k.device or not t.is_contiguous() for t in held):
             raise ValueError("a cache's tensors must be contiguous and on one device")
+        if any(t.requires_grad for t in held):
+            raise ValueError("a tensor of the cache requires grad; these calls have no backward")
         if k.device.type != "cuda":
             raise ValueError(f"expected a CUDA device, got {k.device}")
         self._held = held

@@ -325,3 +325,21 @@ def test_status_on_the_objects_device(monkeypatch):
         x.lib = SimpleNamespace(mqh_status=lambda flags, handle: seen.append(now[0]) or 0)
         assert x.status() == 0
     assert seen == [0, 0] and now == [1]
+
+
+def test_caches_that_require_grad():
+    from flash_moe_hip.kv_cache import PagedCache
+
+    def make(*grads, dtype=torch.float16):
+        k, v = (torch.zeros(2, 2, 16, 64, dtype=dtype) for _ in range(2))
+        scales = [torch.zeros(2, 2, 16) for _ in range(2)] if dtype == torch.int8 else [None, None]
+        held = [k, v, *scales]
+        for i in grads:
+            held[i].requires_grad_()
+        return PagedCache(*held)
+
+    for grads, dtype in (((0,), torch.float16), ((1,), torch.bfloat16), ((2,), torch.int8), ((3,), torch.int8)):
+        with pytest.raises(ValueError, match="no backward"):
+            make(*grads, dtype=dtype)
+    with pytest.raises(ValueError, match="CUDA device"):
+        make()
