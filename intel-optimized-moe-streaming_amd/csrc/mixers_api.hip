@@ -26,6 +26,11 @@ int page_shift_of(int size) {
     return __builtin_ctz((unsigned)size);
 }
 
+// tokens of one write or read: token indexes are 32-bit, the last workgroup's past the end among them
+bool kv_tokens_ok(int tokens, int kv_heads) {
+    return tokens > 0 && tokens <= 1 << 30 && (int64_t)tokens * kv_heads < (int64_t)1 << 31;
+}
+
 // what every call on a cache has to hold
 int check_cache(const void* kc, const void* vc, const float* ks, const float* vs, int cache_type, int64_t pages,
                 int kv_heads, int page_size, int dim) {
@@ -180,7 +185,7 @@ int mqh_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, 
     const int st = check_cache(kc, vc, ks, vs, cache_type, pages, kv_heads, page_size, dim);
     if (st) return st;
     const int size = mix_bytes(type);
-    if (unaligned(k, size) || unaligned(v, size) || (int64_t)tokens * kv_heads >= (int64_t)1 << 31) return ST_ARG;
+    if (unaligned(k, size) || unaligned(v, size) || !kv_tokens_ok(tokens, kv_heads)) return ST_ARG;
     KvParams p{};
     p.k = k; p.v = v;
     p.k_token = k_token; p.k_head = k_head; p.v_token = v_token; p.v_head = v_head;
@@ -199,7 +204,7 @@ int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc
     if (!row_type(type)) return ST_TYPE;
     const int st = check_cache(kc, vc, ks, vs, cache_type, pages, kv_heads, page_size, dim);
     if (st) return st;
-    if (unaligned(k, 16) || unaligned(v, 16) || (int64_t)tokens * kv_heads >= (int64_t)1 << 31) return ST_ARG;
+    if (unaligned(k, 16) || unaligned(v, 16) || !kv_tokens_ok(tokens, kv_heads)) return ST_ARG;
     KvParams p{};
     p.k = k; p.v = v; p.slots = slots;
     p.kc = const_cast<void*>(kc); p.vc = const_cast<void*>(vc);

@@ -343,3 +343,10 @@ def test_caches_that_require_grad():
             make(*grads, dtype=dtype)
     with pytest.raises(ValueError, match="CUDA device"):
         make()
+
+
+def test_token_counts_whose_workgroups_pass_31_bits(lib):
+    """The last workgroup's tokens are counted past the end: room for it."""
+    for tokens in (2 ** 31 - 1, 2 ** 30 + 1):
+        assert kv_write(lib, tokens=tokens, heads=1) == -1
+        assert lib.mqh_kv_read(P, tokens, P, P, None, None, 1, 4, 1, 16, 64, P, P, 1, P, None) == -1
