@@ -41,6 +41,13 @@ int check_cache(const void* kc, const void* vc, const float* ks, const float* vs
     return unaligned(kc, 16) || unaligned(vc, 16) ? ST_ARG : ST_OK;
 }
 
+// whether the words of a call's int arguments are ints (one that is not is refused, not cut)
+bool ints_ok(const int64_t* a, std::initializer_list<int> at) {
+    for (int i : at)
+        if (a[i] != (int)a[i]) return false;
+    return true;
+}
+
 // Workgroups of an attention call, their query tokens, and the splits of their
 // keys.  Many rows: the splits that make one round of what the chip holds (two
 // workgroups a CU, one at dim 256); more cost their sums' traffic and a second
@@ -286,10 +293,9 @@ int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const voi
 }
 
 // The calls with their arguments, in order, as 64-bit words (pointers as
-// integers, floats as the bits of a double).  A count that an int does not hold is
-// refused, not cut.
+// integers, floats as the bits of a double).
 int mqh_linear_step_words(const int64_t* a) {
-    if (!a || a[16] != (int)a[16]) return ST_ARG;
+    if (!a || !ints_ok(a, {9, 16, 17, 18, 19, 20})) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     return linear_step(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10), a[11],
                        (const float*)P(12), a[13], (float*)P(14), P(15), (int)a[16], (int)a[17], (int)a[18],
@@ -297,7 +303,7 @@ int mqh_linear_step_words(const int64_t* a) {
 }
 
 int mqh_linear_prefill_words(const int64_t* a) {
-    if (!a || a[17] != (int)a[17] || a[18] != (int)a[18]) return ST_ARG;
+    if (!a || !ints_ok(a, {9, 17, 18, 19, 20, 21, 22})) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     return linear_prefill(P(0), a[1], a[2], P(3), a[4], a[5], P(6), a[7], a[8], (int)a[9], (const float*)P(10),
                           a[11], (const float*)P(12), a[13], (float*)P(14), P(15), (const int32_t*)P(16), (int)a[17],
@@ -306,7 +312,7 @@ int mqh_linear_prefill_words(const int64_t* a) {
 }
 
 int mqh_kv_write_words(const int64_t* a) {
-    if (!a || a[8] != (int)a[8]) return ST_ARG;
+    if (!a || !ints_ok(a, {6, 8, 13, 15, 16, 17})) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     return mqh_kv_write(P(0), a[1], a[2], P(3), a[4], a[5], (int)a[6], (const int64_t*)P(7), (int)a[8], P(9), P(10),
                         (float*)P(11), (float*)P(12), (int)a[13], a[14], (int)a[15], (int)a[16], (int)a[17],
@@ -314,14 +320,14 @@ int mqh_kv_write_words(const int64_t* a) {
 }
 
 int mqh_kv_read_words(const int64_t* a) {
-    if (!a || a[1] != (int)a[1]) return ST_ARG;
+    if (!a || !ints_ok(a, {1, 6, 8, 9, 10, 13})) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     return mqh_kv_read((const int64_t*)P(0), (int)a[1], P(2), P(3), (const float*)P(4), (const float*)P(5), (int)a[6],
                        a[7], (int)a[8], (int)a[9], (int)a[10], P(11), P(12), (int)a[13], (int32_t*)P(14), P(15));
 }
 
 int mqh_attend_words(const int64_t* a) {
-    if (!a || a[4] != (int)a[4] || a[6] != (int)a[6] || a[19] != (int)a[19]) return ST_ARG;
+    if (!a || !ints_ok(a, {3, 4, 6, 7, 12, 14, 15, 16, 19})) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     double scale;
     __builtin_memcpy(&scale, &a[21], 8);

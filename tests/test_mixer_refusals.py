@@ -350,3 +350,25 @@ def test_token_counts_whose_workgroups_pass_31_bits(lib):
     for tokens in (2 ** 31 - 1, 2 ** 30 + 1):
         assert kv_write(lib, tokens=tokens, heads=1) == -1
         assert lib.mqh_kv_read(P, tokens, P, P, None, None, 1, 4, 1, 16, 64, P, P, 1, P, None) == -1
+
+
+def test_words_of_every_int_argument_past_32_bits(lib):
+    import struct
+
+    p = 4096
+    cache = [p, p, 0, 0, 1, 4, 2, 16, 64]
+    rows = [p, 64, 16, p, 64, 16, p, 64, 16, 0, p, 4, p, 4, p, p]
+    calls = (
+        (lib.mqh_kv_write_words, "20q", [p, 128, 64, p, 128, 64, 1, p, 4, *cache, p, 0], (6, 8, 13, 15, 16, 17)),
+        (lib.mqh_kv_read_words, "16q", [p, 4, *cache, p, p, 1, p, 0], (1, 6, 8, 9, 10, 13)),
+        (lib.mqh_attend_words, "21qd5q", [p, 512, 64, 1, 4, p, 2, 8, *cache, p, 4, 4, p, 0.125, p, p, 1 << 30, p, 0],
+         (3, 4, 6, 7, 12, 14, 15, 16, 19)),
+        (lib.mqh_linear_step_words, "23q", [*rows, 2, 4, 4, 16, 16, p, 0], (9, 16, 17, 18, 19, 20)),
+        (lib.mqh_linear_prefill_words, "27q", [*rows, p, 8, 2, 4, 4, 16, 16, p, 1 << 30, p, 0], (9, 17, 18, 19, 20, 21, 22)),
+    )
+    for call, layout, words, ints in calls:
+        for i in ints:
+            for far in (2 ** 32, -2 ** 32):
+                bad = list(words)
+                bad[i] += far
+                assert call(struct.pack(layout, *bad)) == -1, (call.__name__, i)
