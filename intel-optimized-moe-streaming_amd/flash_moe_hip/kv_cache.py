@@ -186,9 +186,14 @@ class PagedCache:
 
     def slots(self, page_table, seq, position):
         """Slots of positions of sequences: page_table [sequences, columns], seq
-        and position index tensors of one shape."""
-        page = page_table[seq, position // self.page_size].long()
-        return page * self.page_size + position % self.page_size
+        and position index tensors of one shape.  A negative position gives -1,
+        which write and read skip; one past the table gives a slot past the cache,
+        which they report."""
+        column, last = position // self.page_size, page_table.shape[1] - 1
+        page = page_table[seq, column.clamp(0, max(last, 0))].long()
+        slot = page * self.page_size + position % self.page_size
+        slot = slot.masked_fill(column > last, self.pages * self.page_size)
+        return slot.masked_fill(position < 0, -1)
 
     def write(self, k, v, slots, *, stream=None):
         """Store rows k, v [tokens, kv_heads, head_dim] (FP32, FP16 or BF16, any

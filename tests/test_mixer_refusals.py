@@ -372,3 +372,20 @@ def test_words_of_every_int_argument_past_32_bits(lib):
                 bad = list(words)
                 bad[i] += far
                 assert call(struct.pack(layout, *bad)) == -1, (call.__name__, i)
+
+
+def test_slots_of_positions_that_are_none():
+    """A padded batch: a negative position has no slot, one past the table's columns a slot past the cache (which
+    write and read report), and neither reads the table out of its bounds."""
+    from flash_moe_hip.kv_cache import PagedCache
+
+    c = PagedCache.__new__(PagedCache)
+    c.page_size, c.pages = 16, 9
+    table = torch.tensor([[3, 5, 8], [7, 1, -1]], dtype=torch.int32)
+    seq = torch.tensor([0, 0, 0, 1, 1, 0, 0, 1, 1])
+    position = torch.tensor([0, 17, 47, 15, 16, -1, 48, -1000, 2 ** 40])
+    want = [48, 81, 143, 127, 16, -1, 144, -1, 144]
+    assert c.slots(table, seq, position).tolist() == want
+    assert c.slots(table, seq[:7], position[:7].int()).tolist() == want[:7]
+    assert (c.slots(table, torch.tensor([1]), torch.tensor([40])) < 0).all()   # a page that is none
+    assert c.slots(table[:, :0], seq[:0], position[:0]).tolist() == []
