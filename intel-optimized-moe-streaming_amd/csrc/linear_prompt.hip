@@ -516,9 +516,11 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
 // FP32 instructions would bound this kernel (13,300 cycles a SIMD for a workgroup
 // at 128 x 128), so the long products run on BF16 ones, 16 times as fast, with
 // every operand as the exact sum of BF16 planes of 8 bits each: three of an FP32
-// value, two of an FP16, one of a BF16.  The products of planes a and b with
-// a + b <= 2 are summed; what is left out is below 2^-23 of a term, as FP32's own
-// rounding is.
+// value, two of an FP16, one of a BF16, each the rest of those before it to nearest
+// (numbers of 3.396e38 and more, a 500th below FP32's end, become infinite by it).  The
+// products of planes a and b with a + b <= 2 are summed; what is left out is at most
+// 2^-23 of a term, of either sign, as FP32's own rounding of a product and a sum is.
+// (Truncated planes would leave out up to 2^-21 of a term, always of its own sign.)
 //
 // The 16x16x32 instruction contracts slots (g, e): with columns
 // 32 m + 16 (e / 4) + 4 g + e % 4 in them, the right operand is two tiles in
@@ -528,6 +530,8 @@ __global__ __launch_bounds__(256, 1) void k_linear_scan(LinearParams p) {
 template <int TYPE>
 constexpr int PLANES = TYPE == MIX_F32 ? 3 : TYPE == MIX_F16 ? 2 : 1;
 
+typedef __bf16 bfloat2 __attribute__((ext_vector_type(2)));
+
 // v as the sum of N BF16 values, packed in pairs: p[plane][i] holds v[2 i], v[2 i + 1]
 template <int N, int COUNT>
 __device__ __forceinline__ void split(const float (&v)[COUNT], uint32_t (&p)[N][COUNT / 2]) {
@@ -536,10 +540,10 @@ __device__ __forceinline__ void split(const float (&v)[COUNT], uint32_t (&p)[N][
         float a = v[2 * i], b = v[2 * i + 1];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            p[n][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+            p[n][i] = __builtin_bit_cast(uint32_t, bfloat2{(__bf16)a, (__bf16)b});
             if (n + 1 < N) {
-                a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-                b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+                a -= __uint_as_float(p[n][i] << 16);
+                b -= __uint_as_float(p[n][i] & 0xffff0000u);
             }
         }
     }

@@ -384,3 +384,39 @@ def test_strides_past_32_bits_of_a_chunk(delta):
     assert one.status() == 0 and two.status() == 0
     with pytest.raises(ValueError, match="token stride"):
         one.prefill(*[None if t is None else spread(t[:2], (far,) + t.stride()[1:]) for t in args])
+
+
+def test_products_of_a_prompts_outputs_to_fp32():
+    """Outputs that are one product each, of the state and q or of a write and q k: what the kernel leaves out of a
+    product and its roundings are counted.  The two factors are sums of three BF16 numbers to nearest (off by at most
+    2^-8 of what they stand for, each the rest of the one before), and the products of the second with the third or
+    less are left out: two of at most 2^-24 of the term, and 2^-32.  The six others are added in FP32 (five roundings,
+    the partial sums at most 1.02 of the term)."""
+    from flash_moe_hip.linear_attention import LinearState
+
+    g = torch.Generator().manual_seed(0)
+    i = torch.arange(64)
+    # all bits of the second and third part set, for every first part; and any numbers
+    x = torch.stack([1 + (i % 64) / 64 - 2.0 ** -23 * (1 + i % 5), 1 + (2 * i + 1) / 128 - 2.0 ** -23,
+                     torch.randn(64, generator=g), torch.rand(64, generator=g) + 1])
+    y = torch.stack([x[0].flip(0), 1 + (2 * i + 1) / 128 - 2.0 ** -22, torch.randn(64, generator=g), x[3].roll(9)])
+    x, y = torch.cat([x, x]), torch.cat([y, x])
+    heads = x.shape[0]
+    tol = (2.0 ** -23 + 2.0 ** -32 + 5 * 1.02 * 2.0 ** -24) * (x.double() * y.double()).abs() * 1.001
+    none, gate = torch.zeros(1, heads, 64), torch.zeros(1, heads)
+    # the state: row r has one entry, in column r
+    st = LinearState(1, heads, 64, 64, state=torch.diag_embed(y).unsqueeze(0).cuda())
+    got = st.prefill(x.unsqueeze(0).cuda(), none.cuda(), none.cuda(), None, gate.cuda())[0].cpu().double()
+    err = (got - x.double() * y.double()).abs()
+    assert (err <= tol).all(), f"{float((err / tol).max()):.3g} of the bound"
+    # a write: (q k) v of one token, a head for every x
+    n = heads * 64
+    one = torch.zeros(1, n, 64)
+    one[:, :, 3] = 1.0
+    k = torch.zeros(1, n, 64)
+    k[0, :, 3] = x.flatten()
+    st = LinearState(1, n, 4, 64)
+    got = st.prefill(one.cuda(), k.cuda(), y.flatten().view(1, n, 1).expand(1, n, 4).contiguous().cuda(), None,
+                     torch.zeros(1, n).cuda())[0, :, 1].cpu().double().view(heads, 64)
+    err = (got - x.double() * y.double()).abs()
+    assert (err <= tol).all(), f"{float((err / tol).max()):.3g} of the bound"
