@@ -420,3 +420,41 @@ def test_products_of_a_prompts_outputs_to_fp32():
                      torch.zeros(1, n).cuda())[0, :, 1].cpu().double().view(heads, 64)
     err = (got - x.double() * y.double()).abs()
     assert (err <= tol).all(), f"{float((err / tol).max()):.3g} of the bound"
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_several_passes_over_ragged_sequences(delta):
+    """Sequences that end before a pass, begin in it, lie inside it, go over its ends, and hold nothing: the same bits
+    as each alone in calls of one pass (cut at its chunks' ends), and as the recurrence in 64 bits."""
+    from flash_moe_hip import _lib
+    from flash_moe_hip.linear_attention import LinearState
+
+    heads, dk, dv, parts = 64, 256, 512, [0, 700, 1500, 0, 30, 64, 900, 1, 0]
+    n, seqs = sum(parts), len(parts)
+    need = _lib.load().mqh_linear_prefill_workspace_bytes
+    assert need(n, seqs, heads, dk, dv, int(delta)) == need(8 * n, seqs, heads, dk, dv, int(delta))   # as large as it gets
+    assert need(1216, 1, heads, dk, dv, int(delta)) < need(n, seqs, heads, dk, dv, int(delta))        # one pass
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k = (torch.nn.functional.normalize(torch.randn(n, 1, dk, generator=g, device="cuda"), dim=2) * (1 - 2.0 ** -7)
+            for _ in range(2))
+    v = torch.randn(n, heads, dv, generator=g, device="cuda")
+    gate = -torch.rand(n, heads, generator=g, device="cuda") * 0.1
+    beta = torch.rand(n, heads, generator=g, device="cuda") if delta else None
+    first = torch.randn(seqs, heads, dv, dk, generator=g, device="cuda") * 0.1
+    st = LinearState(seqs, heads, dv, dk, state=first.clone())
+    starts = torch.tensor([0] + parts).cumsum(0)
+    got = st.prefill(q, k, v, beta, gate, starts=starts.to(torch.int32).cuda())
+    assert st.status() == 0
+    for b, m in enumerate(parts):
+        alone = LinearState(1, heads, dv, dk, state=first[b:b + 1].clone())
+        for at in range(int(starts[b]), int(starts[b + 1]), 1216):
+            to = min(at + 1216, int(starts[b + 1]))
+            out = alone.prefill(*[None if t is None else t[at:to] for t in (q, k, v, beta, gate)])
+            assert torch.equal(out, got[at:to]), b
+        assert torch.equal(alone.state[0], st.state[b]), b
+    b, h = 2, 5
+    rows = [None if t is None else t[starts[b]:starts[b + 1]].cpu() for t in (q, k, v, beta, gate)]
+    rows = rows[:2] + [None if t is None else t[:, h:h + 1] for t in rows[2:]]
+    want, state, size = ref.linear(first[b, h:h + 1].cpu(), *rows)
+    close(got[starts[b]:starts[b + 1], h:h + 1], want, size, parts[b], dk, torch.float32)
+    close(st.state[b, h:h + 1], state, size, parts[b], dk)
