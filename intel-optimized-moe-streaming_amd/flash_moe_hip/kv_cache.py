@@ -137,8 +137,8 @@ class PagedCache:
             raise ValueError("a tensor of the cache requires grad; these calls have no backward")
         if k.device.type != "cuda":
             raise ValueError(f"expected a CUDA device, got {k.device}")
-        self._held = held
-        self._like = [(t.shape, t.dtype, t.device) for t in held]
+        self._held = (k, v, k_scale, v_scale)
+        self._like = [None if t is None else (t.shape, t.dtype, t.device) for t in self._held]
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, dim
         self.device = k.device
         self.lib = _lib.load()
@@ -150,27 +150,31 @@ class PagedCache:
         self._q_types = (torch.float16, torch.bfloat16) if int8 else (k.dtype,)
         self._read_type = torch.float32 if int8 else k.dtype
         self._flags = torch.zeros(64, dtype=torch.int32, device=k.device)
-        self._at = [t.data_ptr() for t in held]
-        self._sizes = (types[k.dtype], pages, kv_heads, page_size, dim)
+        self._fixed = (*self._addresses(), types[k.dtype], pages, kv_heads, page_size, dim)
 
     # (a call's addresses and sizes are those of the tensors checked here: no others can be put in their place)
     k = property(lambda self: self._held[0], doc="The keys [pages, kv_heads, page_size, head_dim].")
     v = property(lambda self: self._held[1], doc="The values, as the keys.")
-    k_scale = property(lambda self: self._held[2] if len(self._held) == 4 else None,
-                       doc="An int8 cache's scales [pages, kv_heads, page_size].")
-    v_scale = property(lambda self: self._held[3] if len(self._held) == 4 else None, doc="The values' scales.")
+    k_scale = property(lambda self: self._held[2], doc="An int8 cache's scales [pages, kv_heads, page_size], or None.")
+    v_scale = property(lambda self: self._held[3], doc="The values' scales.")
+
+    def _addresses(self):
+        return tuple(0 if t is None else t.data_ptr() for t in self._held)
 
     def _words(self):
         """The cache's share of a call's words, at the addresses its tensors have now
         (their storage may have moved)."""
-        at = [t.data_ptr() for t in self._held]
-        if at != self._at:
-            for t, (shape, dtype, device) in zip(self._held, self._like):
-                if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous() or (
-                        t.untyped_storage().nbytes() < (t.storage_offset() + t.numel()) * t.element_size()):
+        k, v, ks, vs = self._held
+        w = self._fixed
+        if k.data_ptr() != w[0] or v.data_ptr() != w[1] or (
+                ks is not None and (ks.data_ptr() != w[2] or vs.data_ptr() != w[3])):
+            for t, like in zip(self._held, self._like):
+                if t is not None and ((t.shape, t.dtype, t.device) != like or not t.is_contiguous() or (
+                        t.untyped_storage().nbytes() < (t.storage_offset() + t.numel()) * t.element_size())):
+                    shape, dtype, device = like
                     raise ValueError(f"a tensor of the cache is no longer {dtype} {tuple(shape)}, contiguous, on {device}")
-            self._at = at
-        return (*at, *self._sizes) if len(at) == 4 else (*at, 0, 0, *self._sizes)
+            self._fixed = w = (*self._addresses(), *w[4:])
+        return w
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dtype=None, device="cuda"):
