@@ -458,7 +458,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendParams p) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
     const float ref = top == -INFINITY ? 0.0f : top;
-    // (a split without keys for this row weighs nothing, whatever lies in its place)
+    // (a split without keys for this row weighs nothing)
     const float wa = a.x == -INFINITY && a.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(a.x - ref);
     const float wb = b.x == -INFINITY && b.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(b.x - ref);
     float l = fmaf(wa, a.y, wb * b.y);
@@ -476,7 +476,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendParams p) {
         for (int i = 0; i < 8; ++i) {
             const int s = s0 + i;
             const float w = __shfl(s < 64 ? wa : wb, s & 63);
-            if (s < p.splits && w != 0.0f)
+            if (s < p.splits)   // (also where w is 0: infinity and NaN stay so; a split without keys left zeros)
 #pragma unroll
                 for (int e = 0; e < N; ++e) sum[e] = fmaf(w, v[i][e], sum[e]);
         }

@@ -438,3 +438,22 @@ def test_outputs_their_type_cannot_hold_are_reported(new, length, qt, value):
     assert got[..., 3].isinf().all() and c.status() == -4
     vs.fill_(6e4 / 127)
     assert call(c, p, single=new == 1).isfinite().all() and c.status() == 0
+
+
+@pytest.mark.parametrize("what", [math.inf, math.nan])
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("length", [330, 9000])
+def test_a_seen_value_that_is_not_finite_is_not_lost_where_its_weight_underflows(length, new, what):
+    """Keys far below the others in score, in one workgroup's share with them or in shares of their own."""
+    p = problem([new], [length], 2, 1, 64, 64, torch.bfloat16, torch.bfloat16, seed=4)
+    p["q"][:, :, 0] = 64
+    kc, vc = p["cache"][:2]
+    kc[..., 0] = 0
+    for page_ in p["table"][0, :length // 320].tolist():   # the first fifth of the keys: scores of -4096 or so
+        kc[page_, 0, :, 0] = -64
+    vc[int(p["table"][0, 0]), 0, 3, 5] = what
+    c = cache_of(p)
+    got = call(c, p, single=new == 1, scale=1.0)
+    assert not got[..., 5].isfinite().any() and c.status() == -4
+    others = [d for d in range(64) if d != 5]
+    assert got[..., others].isfinite().all()
