@@ -67,6 +67,8 @@ struct MixMath<MIX_BF16> {
     static __device__ __forceinline__ floatx4 mfma16(vec8 a, vec8 b, floatx4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
+    // (probabilities are BF16 as the values are: one type to an instruction, and a BF16
+    // cache's values may lie past FP16's range)
     static constexpr float P_SHIFT = 0.0f;
     static constexpr uint32_t EXPONENT = 0x7f80u;
 };

@@ -16,8 +16,8 @@
 // row's maximum goes over them by lane exchanges, no LDS.  A workgroup takes one
 // head of consecutive tokens, whose scales usually share a line: with the heads of
 // a token together, every line of scales was written piecemeal from several XCDs.
-// 16,384 BF16 tokens of 8 heads of 128: 26.5 us written as codes (3.8 TB/s), 16.5 read
-// back (6.1 TB/s).
+// 16,384 BF16 tokens of 8 heads of 128: 27.1 us written as codes (3.8 TB/s), 16.8 read
+// back (6.0 TB/s, in part from the last-level cache).
 
 #include "mixers.h"
 

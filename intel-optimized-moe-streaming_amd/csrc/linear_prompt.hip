@@ -30,8 +30,8 @@
 // bytes a lane, a 16 x 16 tile's 1 KiB in one run (rows 256 bytes and more apart
 // cost the address unit 64 cycles a load: the scan took 4 us a chunk so).
 //
-// 4096 FP32 tokens, 32 heads over 16 key heads, 128 x 128: 80 + 153 + 82 us.  The
-// first and last are bound by memory (160 and 192 KB a chunk and head, 4.2 and 4.9
+// 4096 FP32 tokens, 32 heads over 16 key heads, 128 x 128: 80 + 156 + 89 us.  The
+// first and last are bound by memory (160 and 192 KB a chunk and head, 4.2 and 4.5
 // TB/s), the scan by its chain (2.4 us a chunk: products 0.7, the waves' exchange of
 // W S0^T 0.9, loads and stores the rest).
 

@@ -101,7 +101,8 @@ class PagedCache:
     """One layer's paged cache over tensors the caller keeps: k and v [pages,
     kv_heads, page_size, head_dim], FP16, BF16 or int8 (then k_scale and v_scale
     [pages, kv_heads, page_size] FP32), contiguous.  head_dim 64, 128 or 256,
-    page_size a power of two from 16 to 1024.
+    page_size a power of two from 16 to 1024.  Scales are those that ``write``
+    stores: 0, NaN, or 2^-100 and more.
 
     A *slot* is page * page_size + offset; a sequence's page table lists its
     pages in order."""
@@ -203,7 +204,7 @@ class PagedCache:
         """Store rows k, v [tokens, kv_heads, head_dim] (FP32, FP16 or BF16, any
         token and head strides) at `slots` [tokens] int64; a negative slot is
         skipped, one past the cache is skipped and latched (-9).  Each slot may
-        occur once in a call.  16-bit caches round once; an int8 cache stores
+        occur once in a call, of at most 2^30 tokens.  16-bit caches round once; an int8 cache stores
         round(x / s), s = max|x| / 127 of the row.  A value that is not finite (or
         that an FP16 cache cannot hold) latches -4; in an int8 cache its row then
         reads back as NaN."""
@@ -262,7 +263,8 @@ class PagedCache:
         of `out` that belong to no sequence are left as they were (without `out`
         they hold anything).  scale > 0
         (default head_dim ** -0.5).  Returns out [tokens, heads, head_dim] of q's
-        type.  Page numbers, lengths and starts out of range latch -9 (the
+        type; probabilities are rounded once to the cache's 16-bit type (FP16 for
+        int8), sums are FP32.  Page numbers, lengths and starts out of range latch -9 (the
         rows concerned are then undefined), outputs that are not finite -4."""
         if q.dim() != 3 or page_table.dim() != 2:
             raise ValueError("q must be [tokens, heads, head_dim] and page_table [sequences, columns]")

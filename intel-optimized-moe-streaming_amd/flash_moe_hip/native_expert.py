@@ -144,7 +144,8 @@ class DeltaState:
         FP32; the state is updated and [tokens, heads, value_dim] returned.  FP32
         sums in an order of their own, where ``step`` has the reference's bit for
         bit.  key_dim a multiple of 4 up to 256, value_dim one up to 1024.  A call
-        takes a workspace from torch's allocator, about 1 GiB for the longest."""
+        takes a workspace from torch's allocator: that of its chunks of 64 tokens,
+        up to 1 GiB or eight chunks, whichever is more."""
         from .kv_cache import OnStream
         from .linear_attention import check_dims, check_state, prefill_states
 
