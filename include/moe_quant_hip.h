@@ -343,8 +343,8 @@ int mqh_status(void* workspace, void* stream);
 /* Store rows k, v [tokens x kv_heads x dim] (F32, F16 or BF16; element
  * strides *_token and *_head, dim contiguous) at slots[tokens].  Negative
  * slots are skipped, so are those past the cache (-9); a slot may occur once
- * in a call, of at most 2^30 tokens.  16-bit caches round once.  Q8: s = max|x| / 127 in FP32, codes
- * x / s to nearest, ties to even; a row with s < 2^-100 is zeros, a row that is
+ * in a call, of at most 2^30 tokens.  16-bit caches round once.  Q8: s =
+ * max|x| / 127 in FP32, codes x / s to nearest, ties to even; a row with s < 2^-100 is zeros, a row that is
  * not finite has s = NaN (-4).  Returns 0, -1, -2 or -5. */
 int mqh_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
                  int type, const int64_t* slots, int tokens, void* kc, void* vc, float* ks, float* vs, int cache_type,
@@ -371,12 +371,13 @@ int64_t mqh_attend_workspace_bytes(int tokens, int seqs, int single, int heads, 
  * lengths[seqs] tokens it holds, the new ones included.  starts[seqs + 1]:
  * sequence b's queries are rows starts[b] .. starts[b + 1] - 1, the last of its
  * tokens; NULL: one query a sequence (tokens == seqs).  A query sees the keys
- * up to its own position; a row that sees none, or scores of -inf alone, is zeros; rows of no sequence
- * are left as they were.  out [tokens x heads x dim] contiguous, 16-byte
+ * up to its own position; a row that sees none, or scores of -inf alone, is
+ * zeros; rows of no sequence are left as they were.  out [tokens x heads x dim] contiguous, 16-byte
  * aligned, of q's type.  Products on the matrix cores with FP32 sums, maximum
  * and probability sums in FP32, probabilities rounded to the cache's 16-bit
- * type (FP16 for Q8).  Q8 scales are 0, NaN or at least 2^-100, as mqh_kv_write
- * leaves them.  The workspace (256-byte aligned) is the call's own until
+ * type (FP16 for Q8); BF16 queries of a Q8 cache as FP16 times a power of two of
+ * their row, exact down to 2^-17 of its largest.  Q8 scales are 0,
+ * NaN or at least 2^-100, as mqh_kv_write leaves them.  The workspace (256-byte aligned) is the call's own until
  * its kernels have run.  Returns 0, -1, -2, -5 or -6. */
 int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int tokens, const int32_t* starts,
                int seqs, int heads, const void* kc, const void* vc, const float* ks, const float* vs, int cache_type,

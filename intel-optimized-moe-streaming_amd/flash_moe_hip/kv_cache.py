@@ -204,10 +204,10 @@ class PagedCache:
         """Store rows k, v [tokens, kv_heads, head_dim] (FP32, FP16 or BF16, any
         token and head strides) at `slots` [tokens] int64; a negative slot is
         skipped, one past the cache is skipped and latched (-9).  Each slot may
-        occur once in a call, of at most 2^30 tokens.  16-bit caches round once; an int8 cache stores
-        round(x / s), s = max|x| / 127 of the row.  A value that is not finite (or
-        that an FP16 cache cannot hold) latches -4; in an int8 cache its row then
-        reads back as NaN."""
+        occur once in a call, of at most 2^30 tokens.  16-bit caches round once; an
+        int8 cache stores round(x / s), s = max|x| / 127 of the row.  A value that is
+        not finite (or that an FP16 cache cannot hold) latches -4; in an int8 cache
+        its row then reads back as NaN."""
         n = self._tokens(slots)
         shape = (n, self.kv_heads, self.head_dim)
         kt, kh, _ = check_rows(k, shape, self._types, self._index, "k")
@@ -263,9 +263,11 @@ class PagedCache:
         of `out` that belong to no sequence are left as they were (without `out`
         they hold anything).  scale > 0
         (default head_dim ** -0.5).  Returns out [tokens, heads, head_dim] of q's
-        type; probabilities are rounded once to the cache's 16-bit type (FP16 for
-        int8), sums are FP32.  Page numbers, lengths and starts out of range latch -9 (the
-        rows concerned are then undefined), outputs that are not finite -4."""
+        type.  Probabilities are rounded once to the cache's 16-bit type (FP16 for
+        int8), sums are FP32; BF16 queries of an int8 cache are multiplied as FP16
+        times a power of two of their row (exact down to 2^-17 of its largest).  Page
+        numbers, lengths and starts out of range latch -9 (the rows concerned are
+        then undefined), outputs that are not finite -4."""
         if q.dim() != 3 or page_table.dim() != 2:
             raise ValueError("q must be [tokens, heads, head_dim] and page_table [sequences, columns]")
         tokens, heads, _ = shape = q.shape

@@ -165,11 +165,11 @@ class LinearState:
 
     def prefill(self, q, k, v, beta, gate, *, starts=None, out=None, stream=None):
         """Prompts: the arguments of ``step`` with [tokens, ...] rows (token strides of
-        q, k and v up to 2^22 elements); sequence b's are rows starts[b] .. starts[b + 1] - 1 (int32 [sequences + 1] on the device;
-        may be omitted for one sequence).  The same states and outputs as ``step``
-        token by token up to FP32 rounding; rows of no sequence are left as they
-        were.  A value that is not finite also reaches earlier tokens of its
-        64-token chunk."""
+        q, k and v up to 2^22 elements); sequence b's are rows starts[b] ..
+        starts[b + 1] - 1 (int32 [sequences + 1] on the device; may be omitted for one
+        sequence).  The same states and outputs as ``step`` token by token up to FP32
+        rounding; rows of no sequence are left as they were.  A value that is not
+        finite also reaches earlier tokens of its 64-token chunk."""
         check_state(self.state, self.shape, self._index)
         return prefill_states(self.lib, self._run, self._flags, self.state, q, k, v, beta, gate, starts, out, stream)
 
