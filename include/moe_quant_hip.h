@@ -333,10 +333,14 @@ int mqh_status(void* workspace, void* stream);
 #define MQH_MIX_F16 1
 #define MQH_MIX_BF16 2
 #define MQH_MIX_Q8 3   /* int8 codes with one FP32 scale per token and head */
+#define MQH_MIX_F4 5   /* 4-bit codes (E2M1, the even channel in a byte's low half) with a power of two 2^e per 32
+                        * channels, held as the byte e + 127 */
 
 /* A cache: kc, vc [pages x kv_heads x page_size x dim] of F16, BF16 or Q8
  * (16-byte aligned), for Q8 ks, vs [pages x kv_heads x page_size] FP32
- * (16-byte aligned; else NULL).  page_size is a power of two from 16 to 1024,
+ * (16-byte aligned; else NULL).  F4: kc, vc [pages x kv_heads x page_size x
+ * dim / 2] bytes, ks, vs [pages x kv_heads x page_size x dim / 32] bytes, all
+ * 16-byte aligned.  page_size is a power of two from 16 to 1024,
  * dim 64, 128 or 256, kv_heads at most 1024.  A token's slot is
  * page * page_size + offset. */
 
@@ -345,16 +349,18 @@ int mqh_status(void* workspace, void* stream);
  * slots are skipped, so are those past the cache (-9); a slot may occur once
  * in a call, of at most 2^30 tokens.  16-bit caches round once.  Q8: s =
  * max|x| / 127 in FP32, codes x / s to nearest, ties to even; a row with s < 2^-100 is zeros, a row that is
- * not finite has s = NaN (-4).  Returns 0, -1, -2 or -5. */
+ * not finite has s = NaN (-4).  F4: e the least with max|x| < 7 * 2^e, at least
+ * -23, codes x / 2^e to nearest, ties to even; 32 channels with a value that is not
+ * finite, or of 57344 and more, have the byte 255 (-4) and read as NaN.  Returns 0, -1, -2 or -5. */
 int mqh_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
-                 int type, const int64_t* slots, int tokens, void* kc, void* vc, float* ks, float* vs, int cache_type,
+                 int type, const int64_t* slots, int tokens, void* kc, void* vc, void* ks, void* vs, int cache_type,
                  int64_t pages, int kv_heads, int page_size, int dim, int32_t* flags, void* stream);
 
 /* Rows at slots[tokens] as values of `type` (F32, F16 or BF16) into k, v
  * [tokens x kv_heads x dim], contiguous and 16-byte aligned; rows of negative
  * slots and of slots past the cache (-9) are zeros; a number that `type` cannot
  * hold becomes infinite (-4).  Returns 0, -1, -2 or -5. */
-int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc, const float* ks, const float* vs,
+int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc, const void* ks, const void* vs,
                 int cache_type, int64_t pages, int kv_heads, int page_size, int dim, void* k, void* v, int type,
                 int32_t* flags, void* stream);
 
@@ -375,12 +381,13 @@ int64_t mqh_attend_workspace_bytes(int tokens, int seqs, int single, int heads, 
  * zeros; rows of no sequence are left as they were.  out [tokens x heads x dim] contiguous, 16-byte
  * aligned, of q's type.  Products on the matrix cores with FP32 sums, maximum
  * and probability sums in FP32, probabilities rounded to the cache's 16-bit
- * type (FP16 for Q8); BF16 queries of a Q8 cache as FP16 times a power of two of
+ * type (FP16 for Q8 and F4); BF16 queries of such a cache as FP16 times a power of two of
  * their row, exact down to 2^-17 of its largest.  Q8 scales are 0,
- * NaN or at least 2^-100, as mqh_kv_write leaves them.  The workspace (256-byte aligned) is the call's own until
+ * NaN or at least 2^-100, F4 scales 104 to 140 or 255 (or 0 with codes of 0), as
+ * mqh_kv_write leaves them.  The workspace (256-byte aligned) is the call's own until
  * its kernels have run.  Returns 0, -1, -2, -5 or -6. */
 int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int tokens, const int32_t* starts,
-               int seqs, int heads, const void* kc, const void* vc, const float* ks, const float* vs, int cache_type,
+               int seqs, int heads, const void* kc, const void* vc, const void* ks, const void* vs, int cache_type,
                int64_t pages, int kv_heads, int page_size, int dim, const int32_t* table, int64_t table_stride,
                int table_cols, const int32_t* lengths, float scale, void* out, void* workspace,
                int64_t workspace_bytes, int32_t* flags, void* stream);

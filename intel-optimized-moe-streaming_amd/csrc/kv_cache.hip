@@ -10,6 +10,7 @@
 // A row whose scale is below 2^-100 is stored as zeros (the attention kernels
 // take the scale's logarithm and reciprocal); a row with a value that is not
 // finite gets the scale NaN, so it reads back as NaN, and latches the fault.
+// 4-bit caches (fp4.h) hold E2M1 codes and one power of two a 32 channels.
 //
 // Bound by memory: a row is read and written once.  dim / 8 lanes own a row of
 // eight values each (16-byte loads of 16-bit rows, 8-byte stores of codes); the
@@ -19,6 +20,7 @@
 // 16,384 BF16 tokens of 8 heads of 128: 27.1 us written as codes (3.8 TB/s), 16.8 read
 // back (6.0 TB/s, in part from the last-level cache).
 
+#include "fp4.h"
 #include "mixers.h"
 
 namespace mqh {
@@ -67,8 +69,16 @@ __device__ __forceinline__ void write_row(const KvParams& p, const float (&x)[8]
         const uintx2 codes = {w[0], w[1]};
         *(uintx2*)((int8_t*)cache + dst * DIM + lane * 8) = codes;
         if (lane == 0) {
-            (is_v ? p.vs : p.ks)[dst] = scale;
+            ((float*)(is_v ? p.vs : p.ks))[dst] = scale;
             if (!finite) atomicOr(&p.flags[FLAG_NONFINITE], 1);
+        }
+    } else if constexpr (CACHE == MIX_F4) {
+        // (`top` is that of the 32 channels this lane has eight of)
+        const uint32_t scale = f4_scale(top);
+        ((uint32_t*)cache)[dst * (DIM / 8) + lane] = scale == F4_NONE ? 0u : f4_codes(x, f4_factor(scale));
+        if (lane % 4 == 0) {
+            ((uint8_t*)(is_v ? p.vs : p.ks))[dst * (DIM / F4_BLOCK) + lane / 4] = (uint8_t)scale;
+            if (scale == F4_NONE) atomicOr(&p.flags[FLAG_NONFINITE], 1);
         }
     } else {
         // (an FP32 value past the cache's range becomes infinite: a fault as well)
@@ -101,6 +111,7 @@ __global__ __launch_bounds__(256) void k_kv_write(KvParams p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[n][i]) & 0x7fffffffu);
         if constexpr (CACHE == MIX_Q8) top = row_max<LANES>(top);
+        if constexpr (CACHE == MIX_F4) top = row_max<F4_BLOCK / 8>(top);
         if (first + n * ROWS >= p.tokens || slot[n] < 0) continue;
         if (slot[n] >= p.n_slots) {
             if (lane == 0) atomicOr(&p.flags[FLAG_BAD_ID], 1);
@@ -120,7 +131,8 @@ __global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
     const bool is_v = blockIdx.y;
     const void* cache = is_v ? p.vc : p.kc;
     int64_t slot[N];
-    float x[N][8], scale[N];   // (scale: 8-bit caches)
+    float x[N][8], scale[N];   // (scale: of codes)
+    constexpr float LARGEST = CACHE == MIX_Q8 ? 127.0f : CACHE == MIX_F4 ? 6.0f : 0.0f;   // code
 #pragma unroll
     for (int n = 0; n < N; ++n) slot[n] = p.slots[min(first + n * ROWS, p.tokens - 1)];
 #pragma unroll
@@ -131,9 +143,14 @@ __global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
         const int64_t src = ((page * p.kv_heads + head) << p.page_shift) + off;
         if constexpr (CACHE == MIX_Q8) {
             const uintx2 codes = *(const uintx2*)((const int8_t*)cache + src * DIM + lane * 8);
-            scale[n] = (is_v ? p.vs : p.ks)[src];
+            scale[n] = ((const float*)(is_v ? p.vs : p.ks))[src];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[n][i] = (float)(int8_t)(codes[i >> 2] >> (8 * (i & 3))) * scale[n];
+        } else if constexpr (CACHE == MIX_F4) {
+            const uint32_t codes = ((const uint32_t*)cache)[src * (DIM / 8) + lane];
+            const float factor = f4_factor(((const uint8_t*)(is_v ? p.vs : p.ks))[src * (DIM / F4_BLOCK) + lane / 4]);
+            scale[n] = factor;
+            f4_to_float(codes, factor, x[n]);
         } else {
             load8<CACHE>(cache, src * DIM + lane * 8, x[n]);
         }
@@ -150,11 +167,11 @@ __global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
         // a number that becomes infinite here (one that is stored so is no fault of this
         // call; codes are looked at where their scale can make one: 44.5 us a pass of
         // 16,384 tokens, 45.8 with every value looked at, 44.2 with none)
-        if (CACHE == MIX_Q8 ? !fits<TYPE>(127.0f * scale[n]) : TYPE == MIX_F16 && CACHE == MIX_BF16) {
+        if (CACHE == MIX_Q8 || CACHE == MIX_F4 ? !fits<TYPE>(LARGEST * scale[n]) : TYPE == MIX_F16 && CACHE == MIX_BF16) {
             bool fit = true;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                fit &= fits<TYPE>(x[n][i]) || x[n][i] != x[n][i] || (CACHE != MIX_Q8 && __builtin_isinf(x[n][i]));
+                fit &= fits<TYPE>(x[n][i]) || x[n][i] != x[n][i] || (LARGEST == 0.0f && __builtin_isinf(x[n][i]));
             if (!fit) atomicOr(&p.flags[FLAG_NONFINITE], 1);
         }
         store8<TYPE>((void*)(is_v ? p.v : p.k), (token * p.kv_heads + head) * DIM + lane * 8, x[n]);
@@ -184,6 +201,7 @@ static hipError_t launch_kv_types(const KvParams& p, bool write, hipStream_t s) 
     MQH_KV(MIX_F32, MIX_F16); MQH_KV(MIX_F32, MIX_BF16); MQH_KV(MIX_F32, MIX_Q8);
     MQH_KV(MIX_F16, MIX_F16); MQH_KV(MIX_F16, MIX_BF16); MQH_KV(MIX_F16, MIX_Q8);
     MQH_KV(MIX_BF16, MIX_F16); MQH_KV(MIX_BF16, MIX_BF16); MQH_KV(MIX_BF16, MIX_Q8);
+    MQH_KV(MIX_F32, MIX_F4); MQH_KV(MIX_F16, MIX_F4); MQH_KV(MIX_BF16, MIX_F4);
 #undef MQH_KV
     return hipErrorInvalidValue;
 }

@@ -10,8 +10,8 @@
 namespace mqh {
 
 // element types of the mixers' tensors, as the C ABI numbers them
-// (MQH_MIX_F32, _F16, _BF16, _Q8)
-enum : int { MIX_F32 = 0, MIX_F16 = 1, MIX_BF16 = 2, MIX_Q8 = 3 };
+// (MQH_MIX_F32, _F16, _BF16, _Q8, _F4)
+enum : int { MIX_F32 = 0, MIX_F16 = 1, MIX_BF16 = 2, MIX_Q8 = 3, MIX_F4 = 5 };
 
 // the least scale of an 8-bit cache's row; a row below it is stored as zeros, its scale 0
 constexpr float KV_MIN_SCALE = 0x1p-100f;
@@ -26,8 +26,8 @@ struct KvParams {
     const int64_t* slots;       // [tokens], negative: skipped
     void* kc;                   // [pages x kv_heads x page_size x dim]
     void* vc;
-    float* ks;                  // [pages x kv_heads x page_size], 8-bit caches
-    float* vs;
+    void* ks;                   // 8-bit caches: FP32 [pages x kv_heads x page_size]
+    void* vs;                   // 4-bit caches: exponent bytes [pages x kv_heads x page_size x dim / 32]
     int64_t n_slots;            // pages * page_size
     int type, cache_type;       // of the rows, of the cache
     int tokens, kv_heads, dim, page_shift;
@@ -39,8 +39,8 @@ struct AttendParams {
     int64_t q_token, q_head;    // strides in elements
     const void* kc;
     const void* vc;
-    const float* ks;
-    const float* vs;
+    const void* ks;             // as KvParams
+    const void* vs;
     const int32_t* table;       // [seqs x table_cols] page ids, row stride table_stride
     int64_t table_stride;
     const int32_t* lengths;     // [seqs] cached tokens, the new ones included

@@ -17,7 +17,7 @@ constexpr int ST_OK = 0, ST_ARG = -1, ST_TYPE = -2, ST_HIP = -5, ST_WORKSPACE = 
 
 bool unaligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) != 0; }
 bool row_type(int t) { return t == MIX_F32 || t == MIX_F16 || t == MIX_BF16; }
-bool cache_type_ok(int t) { return t == MIX_F16 || t == MIX_BF16 || t == MIX_Q8; }
+bool cache_type_ok(int t) { return t == MIX_F16 || t == MIX_BF16 || t == MIX_Q8 || t == MIX_F4; }
 int status(hipError_t e) { return e == hipSuccess ? ST_OK : ST_HIP; }
 
 // log2 of a page size the kernels take (16 keys never straddle pages), or -1
@@ -32,12 +32,12 @@ bool kv_tokens_ok(int tokens, int kv_heads) {
 }
 
 // what every call on a cache has to hold
-int check_cache(const void* kc, const void* vc, const float* ks, const float* vs, int cache_type, int64_t pages,
+int check_cache(const void* kc, const void* vc, const void* ks, const void* vs, int cache_type, int64_t pages,
                 int kv_heads, int page_size, int dim) {
     if (!kc || !vc || pages <= 0 || kv_heads <= 0 || kv_heads > 1024) return ST_ARG;
     if (!cache_type_ok(cache_type) || (dim != 64 && dim != 128 && dim != 256)) return ST_TYPE;
     if (page_shift_of(page_size) < 0 || pages >= (int64_t)1 << 31) return ST_ARG;
-    if (cache_type == MIX_Q8 && (!ks || !vs || unaligned(ks, 16) || unaligned(vs, 16))) return ST_ARG;
+    if ((cache_type == MIX_Q8 || cache_type == MIX_F4) && (!ks || !vs || unaligned(ks, 16) || unaligned(vs, 16))) return ST_ARG;
     return unaligned(kc, 16) || unaligned(vc, 16) ? ST_ARG : ST_OK;
 }
 
@@ -185,7 +185,7 @@ int linear_prefill(const void* q, int64_t q_token, int64_t q_head, const void* k
 extern "C" {
 
 int mqh_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
-                 int type, const int64_t* slots, int tokens, void* kc, void* vc, float* ks, float* vs, int cache_type,
+                 int type, const int64_t* slots, int tokens, void* kc, void* vc, void* ks, void* vs, int cache_type,
                  int64_t pages, int kv_heads, int page_size, int dim, int32_t* flags, void* stream) {
     if (!k || !v || !slots || !flags || tokens <= 0) return ST_ARG;
     if (!row_type(type)) return ST_TYPE;
@@ -204,7 +204,7 @@ int mqh_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, 
     return status(launch_kv_write(p, (hipStream_t)stream));
 }
 
-int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc, const float* ks, const float* vs,
+int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc, const void* ks, const void* vs,
                 int cache_type, int64_t pages, int kv_heads, int page_size, int dim, void* k, void* v, int type,
                 int32_t* flags, void* stream) {
     if (!k || !v || !slots || !flags || tokens <= 0) return ST_ARG;
@@ -215,7 +215,7 @@ int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc
     KvParams p{};
     p.k = k; p.v = v; p.slots = slots;
     p.kc = const_cast<void*>(kc); p.vc = const_cast<void*>(vc);
-    p.ks = const_cast<float*>(ks); p.vs = const_cast<float*>(vs);
+    p.ks = const_cast<void*>(ks); p.vs = const_cast<void*>(vs);
     p.n_slots = pages * page_size;
     p.type = type; p.cache_type = cache_type;
     p.tokens = tokens; p.kv_heads = kv_heads; p.dim = dim; p.page_shift = page_shift_of(page_size);
@@ -230,16 +230,16 @@ int64_t mqh_attend_workspace_bytes(int tokens, int seqs, int single, int heads, 
 }
 
 int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int tokens, const int32_t* starts,
-               int seqs, int heads, const void* kc, const void* vc, const float* ks, const float* vs, int cache_type,
+               int seqs, int heads, const void* kc, const void* vc, const void* ks, const void* vs, int cache_type,
                int64_t pages, int kv_heads, int page_size, int dim, const int32_t* table, int64_t table_stride,
                int table_cols, const int32_t* lengths, float scale, void* out, void* workspace,
                int64_t workspace_bytes, int32_t* flags, void* stream) {
     if (!q || !table || !lengths || !out || !flags || table_cols <= 0 || table_stride < table_cols) return ST_ARG;
     const int st = check_cache(kc, vc, ks, vs, cache_type, pages, kv_heads, page_size, dim);
     if (st) return st;
-    // 16-bit caches are multiplied with queries of their own type; 8-bit ones take either
+    // 16-bit caches are multiplied with queries of their own type; those of codes take either
     if (q_type != MIX_F16 && q_type != MIX_BF16) return ST_TYPE;
-    if (cache_type != MIX_Q8 && q_type != cache_type) return ST_TYPE;
+    if (cache_type != MIX_Q8 && cache_type != MIX_F4 && q_type != cache_type) return ST_TYPE;
     const bool single = starts == nullptr;
     const int64_t most = (int64_t)table_cols * page_size;
     if (!attend_sizes(tokens, seqs, single, heads, kv_heads, dim, most)) return ST_ARG;
@@ -315,14 +315,14 @@ int mqh_kv_write_words(const int64_t* a) {
     if (!a || !ints_ok(a, {6, 8, 13, 15, 16, 17})) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
     return mqh_kv_write(P(0), a[1], a[2], P(3), a[4], a[5], (int)a[6], (const int64_t*)P(7), (int)a[8], P(9), P(10),
-                        (float*)P(11), (float*)P(12), (int)a[13], a[14], (int)a[15], (int)a[16], (int)a[17],
+                        P(11), P(12), (int)a[13], a[14], (int)a[15], (int)a[16], (int)a[17],
                         (int32_t*)P(18), P(19));
 }
 
 int mqh_kv_read_words(const int64_t* a) {
     if (!a || !ints_ok(a, {1, 6, 8, 9, 10, 13})) return ST_ARG;
     const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
-    return mqh_kv_read((const int64_t*)P(0), (int)a[1], P(2), P(3), (const float*)P(4), (const float*)P(5), (int)a[6],
+    return mqh_kv_read((const int64_t*)P(0), (int)a[1], P(2), P(3), P(4), P(5), (int)a[6],
                        a[7], (int)a[8], (int)a[9], (int)a[10], P(11), P(12), (int)a[13], (int32_t*)P(14), P(15));
 }
 
@@ -332,7 +332,7 @@ int mqh_attend_words(const int64_t* a) {
     double scale;
     __builtin_memcpy(&scale, &a[21], 8);
     return mqh_attend(P(0), a[1], a[2], (int)a[3], (int)a[4], (const int32_t*)P(5), (int)a[6], (int)a[7], P(8), P(9),
-                      (const float*)P(10), (const float*)P(11), (int)a[12], a[13], (int)a[14], (int)a[15], (int)a[16],
+                      P(10), P(11), (int)a[12], a[13], (int)a[14], (int)a[15], (int)a[16],
                       (const int32_t*)P(17), a[18], (int)a[19], (const int32_t*)P(20), (float)scale, P(22), P(23),
                       a[24], (int32_t*)P(25), P(26));
 }

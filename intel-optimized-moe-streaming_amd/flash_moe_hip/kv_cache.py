@@ -1,9 +1,10 @@
 """Paged key/value cache of an attention layer in HBM, and attention over it.
 
 ``PagedCache`` holds one layer's keys and values as pages [pages, kv_heads,
-page_size, head_dim] in FP16, BF16 or as 8-bit codes with one FP32 scale per
-token and head.  ``write`` stores new tokens' rows (quantizing them for an 8-bit
-cache), ``read`` gives rows back as values, ``attend`` is attention of new
+page_size, head_dim] in FP16, BF16, as 8-bit codes with one FP32 scale per
+token and head, or as 4-bit codes (E2M1) with a power of two per 32 channels.
+``write`` stores new tokens' rows (quantizing them for a cache of codes), ``read``
+gives rows back as values, ``attend`` is attention of new
 tokens over what the sequences hold: chunks of prompts, drafts, or one token a
 sequence.  (The reference keeps a preallocated FP16 cache per sequence and
 attends on the host, attention.py:144-306.)
@@ -21,7 +22,8 @@ import struct
 from . import _lib
 
 HEAD_DIMS = (64, 128, 256)
-F32, F16, BF16, Q8 = 0, 1, 2, 3   # the library's element types (MQH_MIX_*)
+F32, F16, BF16, Q8, F4 = 0, 1, 2, 3, 5   # the library's element types (MQH_MIX_*)
+F4_BLOCK = 32   # channels of a 4-bit cache's scale
 
 _WRITE_WORDS = struct.Struct("20q")
 _READ_WORDS = struct.Struct("16q")
@@ -104,6 +106,11 @@ class PagedCache:
     page_size a power of two from 16 to 1024.  Scales are those that ``write``
     stores: 0, NaN, or 2^-100 and more.
 
+    Or 4-bit: k and v float4_e2m1fn_x2 [pages, kv_heads, page_size, head_dim / 2] (the
+    even channel in a byte's low half), k_scale and v_scale float8_e8m0fnu [pages,
+    kv_heads, page_size, head_dim / 32], one a 32 channels: those that ``write``
+    stores, 2^-23 to 2^13 or NaN (or 2^-127 with codes of 0, as ``empty`` has them).
+
     A *slot* is page * page_size + offset; a sequence's page table lists its
     pages in order."""
 
@@ -113,15 +120,17 @@ class PagedCache:
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v must be [pages, kv_heads, page_size, head_dim] of one type")
         pages, kv_heads, page_size, dim = k.shape
+        if k.dtype == torch.float4_e2m1fn_x2:
+            dim *= 2
         if dim not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {dim}")
         if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
         if pages < 1 or kv_heads < 1 or kv_heads > 1024:
             raise ValueError("a cache has at least one page and 1 to 1024 kv heads")
-        types = {torch.float16: F16, torch.bfloat16: BF16, torch.int8: Q8}
+        types = {torch.float16: F16, torch.bfloat16: BF16, torch.int8: Q8, torch.float4_e2m1fn_x2: F4}
         if k.dtype not in types:
-            raise ValueError(f"a cache is FP16, BF16 or int8, got {k.dtype}")
+            raise ValueError(f"a cache is FP16, BF16, int8 or float4_e2m1fn_x2, got {k.dtype}")
         held = [k, v]
         if k.dtype == torch.int8:
             if k_scale is None or v_scale is None:
@@ -130,8 +139,15 @@ class PagedCache:
                 if s.dtype != torch.float32 or tuple(s.shape) != (pages, kv_heads, page_size):
                     raise ValueError("scales must be FP32 [pages, kv_heads, page_size]")
             held += [k_scale, v_scale]
+        elif k.dtype == torch.float4_e2m1fn_x2:
+            if k_scale is None or v_scale is None:
+                raise ValueError("a 4-bit cache needs k_scale and v_scale")
+            for s in (k_scale, v_scale):
+                if s.dtype != torch.float8_e8m0fnu or tuple(s.shape) != (pages, kv_heads, page_size, dim // F4_BLOCK):
+                    raise ValueError("scales must be float8_e8m0fnu [pages, kv_heads, page_size, head_dim / 32]")
+            held += [k_scale, v_scale]
         elif k_scale is not None or v_scale is not None:
-            raise ValueError("only int8 caches have scales")
+            raise ValueError("only int8 and 4-bit caches have scales")
         if any(t.device != k.device or not t.is_contiguous() for t in held):
             raise ValueError("a cache's tensors must be contiguous and on one device")
         if any(t.requires_grad for t in held):
@@ -147,16 +163,16 @@ class PagedCache:
         self._index = k.device.index
         self._types = _types()
         self._empty, self._int32, self._int64, self._uint8 = torch.empty, torch.int32, torch.int64, torch.uint8
-        int8 = k.dtype == torch.int8
-        self._q_types = (torch.float16, torch.bfloat16) if int8 else (k.dtype,)
-        self._read_type = torch.float32 if int8 else k.dtype
+        codes = k.dtype in (torch.int8, torch.float4_e2m1fn_x2)
+        self._q_types = (torch.float16, torch.bfloat16) if codes else (k.dtype,)
+        self._read_type = torch.float32 if codes else k.dtype
         self._flags = torch.zeros(64, dtype=torch.int32, device=k.device)
         self._fixed = (*self._addresses(), types[k.dtype], pages, kv_heads, page_size, dim)
 
     # (a call's addresses and sizes are those of the tensors checked here: no others can be put in their place)
-    k = property(lambda self: self._held[0], doc="The keys [pages, kv_heads, page_size, head_dim].")
-    v = property(lambda self: self._held[1], doc="The values, as the keys.")
-    k_scale = property(lambda self: self._held[2], doc="An int8 cache's scales [pages, kv_heads, page_size], or None.")
+    k = property(lambda self: self._held[0], doc="The keys, as given.")
+    v = property(lambda self: self._held[1], doc="The values, as given.")
+    k_scale = property(lambda self: self._held[2], doc="The scales of a cache of codes, or None.")
     v_scale = property(lambda self: self._held[3], doc="The values' scales.")
 
     def _addresses(self):
@@ -179,11 +195,18 @@ class PagedCache:
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dtype=None, device="cuda"):
-        """A cache of zeros; dtype torch.float16 (default), torch.bfloat16 or torch.int8."""
+        """A cache of zeros; dtype torch.float16 (default), torch.bfloat16, torch.int8 or
+        torch.float4_e2m1fn_x2."""
         import torch
 
         dtype = torch.float16 if dtype is None else dtype
         shape = (pages, kv_heads, page_size, head_dim)
+        if dtype == torch.float4_e2m1fn_x2:
+            if head_dim not in HEAD_DIMS:
+                raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
+            k, v = (torch.zeros((*shape[:3], head_dim // 2), dtype=torch.uint8, device=device) for _ in range(2))
+            ks, vs = (torch.zeros((*shape[:3], head_dim // F4_BLOCK), dtype=torch.uint8, device=device) for _ in range(2))
+            return cls(k.view(dtype), v.view(dtype), ks.view(torch.float8_e8m0fnu), vs.view(torch.float8_e8m0fnu))
         k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
         if dtype != torch.int8:
             return cls(k, v)
@@ -207,7 +230,10 @@ class PagedCache:
         occur once in a call, of at most 2^30 tokens.  16-bit caches round once; an
         int8 cache stores round(x / s), s = max|x| / 127 of the row.  A value that is
         not finite (or that an FP16 cache cannot hold) latches -4; in an int8 cache
-        its row then reads back as NaN."""
+        its row then reads back as NaN.  A 4-bit cache stores each 32 channels as E2M1
+        codes (0, 0.5, 1, 1.5, 2, 3, 4, 6, to nearest, ties to even) of x / 2^e, e the least
+        with max|x| < 7 * 2^e, -23 at least; 32 channels with a value that is not finite, or
+        of 57344 and more, latch -4 and read back as NaN."""
         n = self._tokens(slots)
         shape = (n, self.kv_heads, self.head_dim)
         kt, kh, _ = check_rows(k, shape, self._types, self._index, "k")
@@ -228,7 +254,7 @@ class PagedCache:
 
     def read(self, slots, dtype=None, *, stream=None):
         """(k, v) [tokens, kv_heads, head_dim] at `slots` [tokens] int64 as `dtype`
-        (the cache's own, FP32 for int8); rows of negative slots are zeros, so are
+        (the cache's own, FP32 for codes); rows of negative slots are zeros, so are
         those past the cache, which latch -9.  A number that `dtype` cannot hold
         becomes infinite and latches -4."""
         n = self._tokens(slots)
@@ -253,7 +279,7 @@ class PagedCache:
         """Attention of new tokens, whose rows are already written, over the cache.
 
         q [tokens, heads, head_dim] (heads a multiple of kv_heads, at most 128
-        times; the cache's type, FP16 or BF16 for int8 caches; any token and head
+        times; the cache's type, FP16 or BF16 for caches of codes; any token and head
         strides); page_table [sequences, columns] int32; lengths [sequences] int32:
         tokens a sequence holds, the new ones included.  starts [sequences + 1]
         int32: sequence b's queries are rows starts[b] .. starts[b + 1] - 1, the
@@ -264,7 +290,7 @@ class PagedCache:
         they hold anything).  scale > 0
         (default head_dim ** -0.5).  Returns out [tokens, heads, head_dim] of q's
         type.  Probabilities are rounded once to the cache's 16-bit type (FP16 for
-        int8), sums are FP32; BF16 queries of an int8 cache are multiplied as FP16
+        codes), sums are FP32; BF16 queries of a cache of codes are multiplied as FP16
         times a power of two of their row (exact down to 2^-17 of its largest).  Page
         numbers, lengths and starts out of range latch -9 (the rows concerned are
         then undefined), outputs that are not finite -4."""
