@@ -313,11 +313,13 @@ int mqh_profile_next_decode(void* a_start, void* a_stop, void* b_start, void* b_
 int mqh_workspace_init(void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Synchronize `stream`, then read and clear the fault flags latched in
- * `workspace`: 0, -4 (non-finite output), -9 (bad expert id) or -5. */
+ * `workspace`: 0, -4 (non-finite output), -9 (bad expert id), -10 (no free
+ * pages left) or -5. */
 int mqh_status(void* workspace, void* stream);
 
 /* ------------------------------------------------------------------------ */
-/* 3. Token mixers: paged key/value cache, attention, linear attention        */
+/* 3. Token mixers: page tables, rotary positions, paged key/value cache,     */
+/*    attention, linear attention                                             */
 /* ------------------------------------------------------------------------ */
 
 /* What a full-attention layer keeps between calls, and the attention that
@@ -392,6 +394,48 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
                int table_cols, const int32_t* lengths, float scale, void* out, void* workspace,
                int64_t workspace_bytes, int32_t* flags, void* stream);
 
+/* Page tables on the device.  table [seqs x cols] int32: the pages of each
+ * sequence in order; lengths [seqs] int32: the tokens it holds; free_pages
+ * [pages] int32: the first *count of them are free pages (int32 count), the last
+ * of those goes first.  page_size as the caches', cols * page_size at most 2^30,
+ * at most 8192 sequences; `flags` of their own (256 bytes, zeroed once), calls on
+ * one table in order.
+ *
+ * extend: sequence b grows by grow[b] >= 0 tokens: its new pages enter the table
+ * and leave the free ones, lengths grow, starts [seqs + 1] int32 become the first
+ * row of each sequence, and rows 0 .. rows - 1 get their slots (int64) and
+ * positions (int32; both 16-byte aligned), -1 past the last sequence.  A call that
+ * cannot be served changes nothing and gives no rows (starts of 0, slots and
+ * positions of -1): -10 latches if pages are lacking, -9 if grow is negative, a
+ * sequence outgrows its columns, the new tokens are more than `rows`, or lengths,
+ * count or pages are out of range.
+ *
+ * trim: sequence b keeps its first min(lengths[b], keep[b]) tokens, pages behind
+ * them go back to the free ones (what the last extend took, to where it was).
+ * keep[b] < 0, and lengths or count out of range, change nothing: -9.
+ * Both return 0, -1 or -5. */
+int mqh_pages_extend(const int32_t* grow, int32_t* table, int cols, int32_t* lengths, int32_t* free_pages, int32_t* count,
+                     int seqs, int pages, int page_size, int rows, int32_t* starts, int64_t* slots, int32_t* positions,
+                     int32_t* flags, void* stream);
+int mqh_pages_trim(const int32_t* keep, int32_t* table, int cols, int32_t* lengths, int32_t* free_pages, int32_t* count,
+                   int seqs, int pages, int page_size, int32_t* flags, void* stream);
+
+/* Rotary positions of q [tokens x heads x dim] and k [tokens x kv_heads x dim]
+ * (F32, F16 or BF16; element strides, dim contiguous; dim 64, 128 or 256): the
+ * first `rotary` channels of a head (a multiple of 16) are turned in pairs, (a, b)
+ * to amplitude * (a cos - b sin, a sin + b cos), pairs (i, i + rotary / 2), or
+ * (2 i, 2 i + 1) with `interleaved`; the others stay.  turns [rotary / 2] uint64:
+ * turns a position of each pair, in units of 2^-64; positions [tokens] int32 (they
+ * may be negative).  q_weight, k_weight [dim] FP32 or NULL: the row first goes
+ * through x / sqrt(mean x^2 + eps) * weight.  FP32 throughout, rounded once; the
+ * outputs may be the inputs themselves.  An output that its type cannot hold
+ * latches -4.  Returns 0, -1, -2 or -5. */
+int mqh_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, int type,
+               const int32_t* positions, int tokens, int heads, int kv_heads, int dim, const uint64_t* turns, int rotary,
+               int interleaved, float amplitude, const float* q_weight, const float* k_weight, float eps, void* q_out,
+               int64_t q_out_token, int64_t q_out_head, void* k_out, int64_t k_out_token, int64_t k_out_head,
+               int32_t* flags, void* stream);
+
 /* One token of each of `seqs` sequences through linear attention with a decay
  * per head (the gated recurrence of mqh_delta_heads for many sequences, other
  * types and shared key heads, and the same without the delta rule):
@@ -429,7 +473,7 @@ int mqh_linear_prefill(const void* q, int64_t q_token, int64_t q_head, const voi
                        int64_t workspace_bytes, int32_t* flags, void* stream);
 
 /* The calls of this group with their arguments, in order, as 64-bit words (20,
- * 16, 27, 23 and 27; pointers as integers, the scale as the bits of a double).
+ * 16, 27, 23, 27, 15, 11 and 27; pointers as integers, floats as the bits of a double).
  * The linear calls take strides past 2^22 in this form (up to 2^40): all of a step's,
  * and all of a prompt's but the token strides of q, k and v where it has more than
  * one token. */
@@ -438,6 +482,9 @@ int mqh_kv_read_words(const int64_t* args);
 int mqh_attend_words(const int64_t* args);
 int mqh_linear_step_words(const int64_t* args);
 int mqh_linear_prefill_words(const int64_t* args);
+int mqh_pages_extend_words(const int64_t* args);
+int mqh_pages_trim_words(const int64_t* args);
+int mqh_rotary_words(const int64_t* args);
 
 #ifdef __cplusplus
 }

@@ -17,7 +17,7 @@ using namespace mqh;
 namespace {
 
 constexpr int ST_OK = 0, ST_ARG = -1, ST_TYPE = -2, ST_BYTES = -3, ST_NONFINITE = -4, ST_HIP = -5,
-              ST_WORKSPACE = -6, ST_BAD_ID = -9;
+              ST_WORKSPACE = -6, ST_BAD_ID = -9, ST_NO_PAGES = -10;
 
 // dequant_k and moe_quant_expert accept the reference's five types; the
 // device entry points also IQ4_NL
@@ -131,15 +131,16 @@ void release_ctx(Ctx* c) {
 }
 
 int read_and_clear_flags(int* flags_dev, hipStream_t s) {
-    int h[2] = {0, 0};   // FLAG_NONFINITE, FLAG_BAD_ID
+    int h[3] = {0, 0, 0};   // FLAG_NONFINITE, FLAG_BAD_ID, FLAG_NO_PAGES
     if (hipStreamSynchronize(s) != hipSuccess) return ST_HIP;
     if (hipMemcpyAsync(h, flags_dev, sizeof(h), hipMemcpyDeviceToHost, s) != hipSuccess) return ST_HIP;
     if (hipStreamSynchronize(s) != hipSuccess) return ST_HIP;
-    if (h[0] | h[1]) {
-        if (zero_words(flags_dev, 2, s) != hipSuccess) return ST_HIP;
+    if (h[0] | h[1] | h[2]) {
+        if (zero_words(flags_dev, 3, s) != hipSuccess) return ST_HIP;
         if (hipStreamSynchronize(s) != hipSuccess) return ST_HIP;
     }
     if (h[FLAG_BAD_ID]) return ST_BAD_ID;
+    if (h[FLAG_NO_PAGES]) return ST_NO_PAGES;
     if (h[FLAG_NONFINITE]) return ST_NONFINITE;
     return ST_OK;
 }

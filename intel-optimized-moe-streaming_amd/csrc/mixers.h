@@ -1,5 +1,6 @@
-// mixers.h -- parameter blocks of the token mixers' kernels (paged key/value
-// cache, attention over it, linear attention) and the lane helpers they share.
+// mixers.h -- parameter blocks of the token mixers' kernels (page tables, rotary
+// positions, paged key/value cache, attention over it, linear attention) and the
+// lane helpers they share.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -81,6 +82,42 @@ struct LinearParams {
     float* e;                   // e^(G_end), 16 bytes a unit
     int chunk0, chunks;
 };
+
+struct PageParams {
+    const int32_t* change;      // [seqs] extend: new tokens; trim: tokens kept
+    int32_t* table;             // [seqs x cols]
+    int32_t* lengths;           // [seqs]
+    int32_t* free_pages;        // [pages]: the first *count are free, the last of them goes first
+    int32_t* count;
+    int32_t* starts;            // extend: [seqs + 1], [rows], [rows]
+    int64_t* slots;
+    int32_t* positions;
+    int seqs, cols, pages, page_shift, rows;
+    int* flags;
+};
+
+struct RotaryParams {
+    const void* q;              // [tokens x heads x dim], dim contiguous
+    const void* k;              // [tokens x kv_heads x dim]
+    int64_t q_token, q_head, k_token, k_head;   // strides in elements
+    void* q_out;                // may be q itself, as k_out k
+    void* k_out;
+    int64_t qo_token, qo_head, ko_token, ko_head;
+    const int32_t* positions;   // [tokens]
+    const uint64_t* turns;      // [rotary / 2] turns a position, in units of 2^-64
+    const float* q_weight;      // [dim] weights of the norm before, or null
+    const float* k_weight;
+    float eps, amplitude;
+    int type, tokens, heads, kv_heads, dim, rotary, interleaved;
+    int per;                    // heads of a workgroup
+    int* flags;
+};
+
+constexpr int PAGE_SEQS_MAX = 8192;   // sequences of a page table: three words each in LDS
+
+hipError_t launch_pages_extend(const PageParams& p, hipStream_t s);
+hipError_t launch_pages_trim(const PageParams& p, hipStream_t s);
+hipError_t launch_rotary(RotaryParams p, hipStream_t s);
 
 constexpr int LINEAR_CHUNK = 64;
 // key dims are padded to 64, 128 or 256, value dims to a multiple of 16

@@ -1,6 +1,6 @@
 // mixers_api.hip -- C entry points of the token mixers (declared in
-// include/moe_quant_hip.h): the paged key/value cache, attention over it and
-// linear attention.  They validate and enqueue only; nothing is allocated, and
+// include/moe_quant_hip.h): page tables, rotary positions, the paged key/value
+// cache, attention over it and linear attention.  They validate and enqueue only; nothing is allocated, and
 // no state is kept between calls.
 #include <algorithm>
 #include <initializer_list>
@@ -180,9 +180,63 @@ int linear_prefill(const void* q, int64_t q_token, int64_t q_head, const void* k
     return ST_OK;
 }
 
+// what both page calls have to hold
+int page_params(PageParams& p, const int32_t* change, int32_t* table, int cols, int32_t* lengths, int32_t* free_pages,
+                int32_t* count, int seqs, int pages, int page_size, int32_t* flags) {
+    if (!change || !table || !lengths || !free_pages || !count || !flags) return ST_ARG;
+    if (seqs <= 0 || seqs > PAGE_SEQS_MAX || cols <= 0 || pages <= 0 || page_shift_of(page_size) < 0) return ST_ARG;
+    if ((int64_t)cols * page_size > (int64_t)1 << 30) return ST_ARG;
+    p.change = change; p.table = table; p.cols = cols; p.lengths = lengths; p.free_pages = free_pages; p.count = count;
+    p.seqs = seqs; p.pages = pages; p.page_shift = page_shift_of(page_size); p.flags = flags;
+    return ST_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int mqh_pages_extend(const int32_t* grow, int32_t* table, int cols, int32_t* lengths, int32_t* free_pages, int32_t* count,
+                     int seqs, int pages, int page_size, int rows, int32_t* starts, int64_t* slots, int32_t* positions,
+                     int32_t* flags, void* stream) {
+    PageParams p{};
+    const int st = page_params(p, grow, table, cols, lengths, free_pages, count, seqs, pages, page_size, flags);
+    if (st) return st;
+    if (!starts || rows < 0 || rows > 1 << 30 || (rows && (!slots || !positions)) || unaligned(slots, 16) ||
+        unaligned(positions, 16))
+        return ST_ARG;
+    p.rows = rows; p.starts = starts; p.slots = slots; p.positions = positions;
+    return status(launch_pages_extend(p, (hipStream_t)stream));
+}
+
+int mqh_pages_trim(const int32_t* keep, int32_t* table, int cols, int32_t* lengths, int32_t* free_pages, int32_t* count,
+                   int seqs, int pages, int page_size, int32_t* flags, void* stream) {
+    PageParams p{};
+    const int st = page_params(p, keep, table, cols, lengths, free_pages, count, seqs, pages, page_size, flags);
+    return st ? st : status(launch_pages_trim(p, (hipStream_t)stream));
+}
+
+int mqh_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, int type,
+               const int32_t* positions, int tokens, int heads, int kv_heads, int dim, const uint64_t* turns, int rotary,
+               int interleaved, float amplitude, const float* q_weight, const float* k_weight, float eps, void* q_out,
+               int64_t q_out_token, int64_t q_out_head, void* k_out, int64_t k_out_token, int64_t k_out_head,
+               int32_t* flags, void* stream) {
+    if (!q || !k || !positions || !turns || !q_out || !k_out || !flags) return ST_ARG;
+    if (!row_type(type) || (dim != 64 && dim != 128 && dim != 256)) return ST_TYPE;
+    if (tokens <= 0 || tokens > 1 << 24 || heads <= 0 || heads > 4096 || kv_heads <= 0 || kv_heads > 4096) return ST_ARG;
+    if (rotary <= 0 || rotary > dim || rotary % 16 || (interleaved != 0 && interleaved != 1)) return ST_ARG;
+    if (!(amplitude > 0.0f) || !(amplitude < INFINITY) || !(eps > 0.0f) || !(eps < INFINITY)) return ST_ARG;
+    const int size = mix_bytes(type);
+    if (unaligned(q, size) || unaligned(k, size) || unaligned(q_out, size) || unaligned(k_out, size)) return ST_ARG;
+    if (unaligned(turns, 8) || unaligned(positions, 4) || unaligned(q_weight, 4) || unaligned(k_weight, 4)) return ST_ARG;
+    RotaryParams p{};
+    p.q = q; p.k = k; p.q_token = q_token; p.q_head = q_head; p.k_token = k_token; p.k_head = k_head;
+    p.q_out = q_out; p.k_out = k_out; p.qo_token = q_out_token; p.qo_head = q_out_head;
+    p.ko_token = k_out_token; p.ko_head = k_out_head;
+    p.positions = positions; p.turns = turns; p.q_weight = q_weight; p.k_weight = k_weight;
+    p.eps = eps; p.amplitude = amplitude; p.type = type; p.tokens = tokens; p.heads = heads; p.kv_heads = kv_heads;
+    p.dim = dim; p.rotary = rotary; p.interleaved = interleaved; p.flags = flags;
+    return status(launch_rotary(p, (hipStream_t)stream));
+}
 
 int mqh_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
                  int type, const int64_t* slots, int tokens, void* kc, void* vc, void* ks, void* vs, int cache_type,
@@ -309,6 +363,31 @@ int mqh_linear_prefill_words(const int64_t* a) {
                           a[11], (const float*)P(12), a[13], (float*)P(14), P(15), (const int32_t*)P(16), (int)a[17],
                           (int)a[18], (int)a[19], (int)a[20], (int)a[21], (int)a[22], P(23), a[24], (int32_t*)P(25),
                           P(26), STRIDE_MAX);
+}
+
+int mqh_pages_extend_words(const int64_t* a) {
+    if (!a || !ints_ok(a, {2, 6, 7, 8, 9})) return ST_ARG;
+    const auto P = [a](int i) { return (int32_t*)(uintptr_t)a[i]; };
+    return mqh_pages_extend(P(0), P(1), (int)a[2], P(3), P(4), P(5), (int)a[6], (int)a[7], (int)a[8], (int)a[9], P(10),
+                            (int64_t*)P(11), P(12), P(13), P(14));
+}
+
+int mqh_pages_trim_words(const int64_t* a) {
+    if (!a || !ints_ok(a, {2, 6, 7, 8})) return ST_ARG;
+    const auto P = [a](int i) { return (int32_t*)(uintptr_t)a[i]; };
+    return mqh_pages_trim(P(0), P(1), (int)a[2], P(3), P(4), P(5), (int)a[6], (int)a[7], (int)a[8], P(9), P(10));
+}
+
+int mqh_rotary_words(const int64_t* a) {
+    if (!a || !ints_ok(a, {6, 8, 9, 10, 11, 13, 14})) return ST_ARG;
+    const auto P = [a](int i) { return (void*)(uintptr_t)a[i]; };
+    double amplitude, eps;
+    __builtin_memcpy(&amplitude, &a[15], 8);
+    __builtin_memcpy(&eps, &a[18], 8);
+    return mqh_rotary(P(0), a[1], a[2], P(3), a[4], a[5], (int)a[6], (const int32_t*)P(7), (int)a[8], (int)a[9],
+                      (int)a[10], (int)a[11], (const uint64_t*)P(12), (int)a[13], (int)a[14], (float)amplitude,
+                      (const float*)P(16), (const float*)P(17), (float)eps, P(19), a[20], a[21], P(22), a[23], a[24],
+                      (int32_t*)P(25), P(26));
 }
 
 int mqh_kv_write_words(const int64_t* a) {

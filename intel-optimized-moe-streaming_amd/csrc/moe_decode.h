@@ -9,8 +9,9 @@
 namespace mqh {
 
 // workspace flag words (int32) at the start of every workspace, sticky until
-// read by mqh_status
-enum : int { FLAG_NONFINITE = 0, FLAG_BAD_ID = 1, N_FLAGS = 64 };
+// read by mqh_status (but FLAG_TICKET: the page kernels' count of workgroups, 0
+// between calls)
+enum : int { FLAG_NONFINITE = 0, FLAG_BAD_ID = 1, FLAG_NO_PAGES = 2, FLAG_TICKET = 32, N_FLAGS = 64 };
 constexpr int64_t WS_HEAD_BYTES = (int64_t)N_FLAGS * 4;
 
 constexpr int ROUTE_PROLOGUE_MAX_EXPERTS = 256;   // 4 router scores per lane

@@ -55,6 +55,12 @@ EXPORTS = (
     "mqh_linear_prefill",
     "mqh_linear_step_words",
     "mqh_linear_prefill_words",
+    "mqh_pages_extend",
+    "mqh_pages_trim",
+    "mqh_rotary",
+    "mqh_pages_extend_words",
+    "mqh_pages_trim_words",
+    "mqh_rotary_words",
 )
 
 STATUS_TEXT = {
@@ -66,6 +72,7 @@ STATUS_TEXT = {
     -5: "HIP runtime failure",
     -6: "workspace too small",
     -9: "an id, slot, page or length out of range",
+    -10: "no free pages left",
 }
 
 _P = C.c_void_p
@@ -174,8 +181,19 @@ def _declare(lib: C.CDLL) -> C.CDLL:
     lib.mqh_linear_prefill_workspace_bytes.restype = _I64
     lib.mqh_linear_prefill.argtypes = [*rows, _P, _I, _I, _I, _I, _I, _I, _P, _I64, _P, _P]
     lib.mqh_linear_prefill.restype = _I
+    pages = [_P, _P, _I, _P, _P, _P, _I, _I, _I]   # change, table, columns, lengths, free, count, seqs, pages, page_size
+    lib.mqh_pages_extend.argtypes = [*pages, _I, _P, _P, _P, _P, _P]
+    lib.mqh_pages_extend.restype = _I
+    lib.mqh_pages_trim.argtypes = [*pages, _P, _P]
+    lib.mqh_pages_trim.restype = _I
+    lib.mqh_rotary.argtypes = [
+        *[_P, _I64, _I64] * 2, _I, _P, _I, _I, _I, _I,   # q, k with strides, type, positions, tokens, heads, dim
+        _P, _I, _I, C.c_float, _P, _P, C.c_float,        # turns, rotary, interleaved, amplitude, weights, eps
+        *[_P, _I64, _I64] * 2, _P, _P,                   # the rows out, flags, stream
+    ]
+    lib.mqh_rotary.restype = _I
     for f in (lib.mqh_kv_write_words, lib.mqh_kv_read_words, lib.mqh_attend_words, lib.mqh_linear_step_words,
-              lib.mqh_linear_prefill_words):
+              lib.mqh_linear_prefill_words, lib.mqh_pages_extend_words, lib.mqh_pages_trim_words, lib.mqh_rotary_words):
         f.argtypes = [C.c_char_p]
         f.restype = _I
     return lib
