@@ -371,6 +371,10 @@ int mqh_kv_read(const int64_t* slots, int tokens, const void* kc, const void* vc
 int64_t mqh_attend_workspace_bytes(int tokens, int seqs, int single, int heads, int kv_heads, int dim,
                                    int64_t most_keys);
 
+/* The same for an F4 cache. */
+int64_t mqh_attend_f4_workspace_bytes(int tokens, int seqs, int single, int heads, int kv_heads, int dim,
+                                      int64_t most_keys);
+
 /* Attention of new tokens, whose rows are already in the cache: q [tokens x
  * heads x dim] (strides q_token, q_head; F16 or BF16, for 16-bit caches the
  * cache's own type), heads a multiple of kv_heads (at most 128 times), query

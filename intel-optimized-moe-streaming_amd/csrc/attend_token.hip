@@ -20,10 +20,7 @@
 // TB/s.  One sequence of 4,099 keys, 16 heads of 256 over 2, 8-bit: 12.1 us, round trips
 // (length, pages, keys, the next keys) of 32 workgroups, and 3.9 to join.
 
-#include <type_traits>
-
 #include "attend.h"
-#include "fp4.h"
 
 namespace mqh {
 
@@ -32,13 +29,11 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
     using M = MixMath<CACHE>;
     typedef typename M::vec8 vec8;
     typedef typename M::vec4 vec4;
-    constexpr bool Q8 = CACHE == MIX_Q8, F4 = CACHE == MIX_F4;
+    constexpr bool Q8 = CACHE == MIX_Q8;
     constexpr int ROW = DIM * 2;
-    constexpr int PIECES = F4 ? DIM / 32 : Q8 ? DIM / 16 : DIM / 8;   // 16-byte pieces of a cache row
+    constexpr int PIECES = Q8 ? DIM / 16 : DIM / 8;   // 16-byte pieces of a cache row
     constexpr int KK = DIM / 32, DB = DIM / 16;
-    constexpr int KL = F4 ? (KK + 3) / 4 : Q8 ? KK / 2 : KK;   // loads of a key's row by its four lanes
-    constexpr int KW = F4 && DIM == 64 ? 2 : 4;       // dwords of such a load
-    typedef typename std::conditional<KW == 2, uintx2, uintx4>::type kload_t;
+    constexpr int KL = Q8 ? KK / 2 : KK;              // loads of a key's row by its four lanes
     constexpr int PASS = 64 / PIECES;                 // keys of one load of V by the wave
     constexpr int VL = 32 / PASS;
     constexpr int PAD = DIM + 4;
@@ -65,11 +60,10 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
         uintx4 raw[KK];
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-            const int d = F4 ? 32 * KW * (kk / KW) + 8 * KW * g + 8 * (kk % KW)
-                             : Q8 ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
+            const int d = Q8 ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
             raw[kk] = load_any<uintx4>(qp + d);
         }
-        if constexpr ((Q8 || F4) && QT == MIX_BF16) {
+        if constexpr (Q8 && QT == MIX_BF16) {
             // to FP16 by a power of two per head that brings its largest value to [1, 2)
             uint32_t top = 0;
 #pragma unroll
@@ -95,7 +89,6 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
         }
     }
     q_scale *= p.scale_log2;
-    if constexpr (F4) q_scale = fmaxf(q_scale, 0x1p-126f);   // (a score of infinity stays so)
 
     // ---- pages of this wave's blocks: lane i has those of its blocks i (mod 64)
     int page_a = 0, page_b = 0;   // of a block's first and last 16 keys
@@ -111,9 +104,7 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
         }
     };
 
-    kload_t kr[2][KL];
-    uintx4 vr[VL];
-    uint8_t kf[2][KL], vf[VL];   // 4-bit caches: the scales of these blocks
+    uintx4 kr[2][KL], vr[VL];
     floatx4 ks4[2], vs4[2];
     // the first row of each half of a block in the cache
     auto rows_of = [&](int block, int it, int64_t& ra, int64_t& rb) {
@@ -124,14 +115,9 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
     auto load_k = [&](int64_t ra, int64_t rb) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const kload_t* kp = (const kload_t*)p.kc + ((j ? rb : ra) + col) * (PIECES * 4 / KW) + g;
+            const uintx4* kp = (const uintx4*)p.kc + ((j ? rb : ra) + col) * PIECES + g;
 #pragma unroll
             for (int i = 0; i < KL; ++i) kr[j][i] = kp[4 * i];
-            if constexpr (F4) {
-                const uint8_t* sp = (const uint8_t*)p.ks + ((j ? rb : ra) + col) * PIECES + (KW == 2 ? g >> 1 : g);
-#pragma unroll
-                for (int i = 0; i < KL; ++i) kf[j][i] = sp[4 * i];
-            }
             if constexpr (Q8) ks4[j] = *(const floatx4*)((const float*)p.ks + (j ? rb : ra) + 4 * g);
         }
     };
@@ -139,10 +125,9 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
         const int piece = lane % PIECES, key = lane / PIECES;
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
-            const int k = key + PASS * i;   // (PASS divides 16, or is 32)
-            const int64_t r = (PASS > 16 ? k < 16 : PASS * i < 16) ? ra + k : rb + (k - 16);
+            const int k = key + PASS * i;   // (PASS divides 16)
+            const int64_t r = PASS * i < 16 ? ra + k : rb + (k - 16);
             vr[i] = ((const uintx4*)p.vc)[r * PIECES + piece];
-            if constexpr (F4) vf[i] = ((const uint8_t*)p.vs)[r * PIECES + piece];
         }
         if constexpr (Q8) {
             vs4[0] = *(const floatx4*)((const float*)p.vs + ra + 4 * g);
@@ -183,11 +168,6 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
                         const uintx2 d = codes_to_half(kr[j][i][2]), e = codes_to_half(kr[j][i][3]);
                         s[j] = M::mfma16(bits_as<vec8>(uintx4{a[0], a[1], c[0], c[1]}), qf[2 * i], s[j]);
                         s[j] = M::mfma16(bits_as<vec8>(uintx4{d[0], d[1], e[0], e[1]}), qf[2 * i + 1], s[j]);
-                    } else if constexpr (F4) {
-                        const float f = f4_factor(kf[j][i]);
-#pragma unroll
-                        for (int w = 0; w < KW; ++w)
-                            s[j] = M::mfma16(bits_as<vec8>(f4_to_half(kr[j][i][w], f)), qf[KW * i + w], s[j]);
                     } else {
                         s[j] = M::mfma16(bits_as<vec8>(kr[j][i]), qf[i], s[j]);
                     }
@@ -226,13 +206,6 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
                         const uintx2 d = codes_to_half(vr[i][2]), e = codes_to_half(vr[i][3]);
                         *(uintx4*)(vt + k * ROW + ((2 * piece) ^ sw) * 16) = uintx4{a[0], a[1], c[0], c[1]};
                         *(uintx4*)(vt + k * ROW + ((2 * piece + 1) ^ sw) * 16) = uintx4{d[0], d[1], e[0], e[1]};
-                    } else if constexpr (F4) {
-                        // (past the end there may be a block that is not finite: zeros for it)
-                        const bool there = !edge || block * 32 + k < keys;
-                        const float f = there ? f4_factor(vf[i]) : 0.0f;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w)
-                            *(uintx4*)(vt + k * ROW + ((4 * piece + w) ^ sw) * 16) = f4_to_half(vr[i][w], f);
                     } else {
                         const bool there = !edge || block * 32 + k < keys;
                         *(uintx4*)(vt + k * ROW + (piece ^ sw) * 16) = there ? vr[i] : uintx4{0, 0, 0, 0};
@@ -349,8 +322,6 @@ template <int DIM>
 static hipError_t launch_token_dim(const AttendParams& p, hipStream_t s) {
     if (p.cache_type == MIX_F16) return launch_token_of<DIM, MIX_F16, MIX_F16>(p, s);
     if (p.cache_type == MIX_BF16) return launch_token_of<DIM, MIX_BF16, MIX_BF16>(p, s);
-    if (p.cache_type == MIX_F4)
-        return p.q_type == MIX_F16 ? launch_token_of<DIM, MIX_F4, MIX_F16>(p, s) : launch_token_of<DIM, MIX_F4, MIX_BF16>(p, s);
     if (p.q_type == MIX_F16) return launch_token_of<DIM, MIX_Q8, MIX_F16>(p, s);
     return launch_token_of<DIM, MIX_Q8, MIX_BF16>(p, s);
 }

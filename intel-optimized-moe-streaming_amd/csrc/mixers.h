@@ -55,6 +55,11 @@ struct AttendParams {
     int tile_tokens;            // query tokens of a workgroup
     int tiles;                  // workgroups a kv head and split
     int splits;
+    // few rows (launch_attend_few): workgroups to share the keys out to (0: one piece a
+    // sequence) and the pieces there is room for; the sums are [pieces x kv_heads x tile
+    // rows] then
+    int even, pieces;
+    int4* part_rows;            // [tokens x kv_heads]: a token's first piece, its pieces, its place in the tile; or null
     int* flags;
 };
 

@@ -13,6 +13,12 @@ using namespace mqh;
 
 namespace {
 
+// Rows of a sequence, on average, up to which a 4-bit cache's call is one of few rows: 32
+// sequences of 4,000 keys, 32 heads of 128 over 8, take 42 us there with 16 rows (63 in
+// launch_attend's tiles), 78 with 64 (114), 135 with 128 (138); 4 sequences of 8,000 keys
+// 47 with 128 rows (49), 75 with 256 (62).
+constexpr int FEW_ROWS = 128;
+
 constexpr int ST_OK = 0, ST_ARG = -1, ST_TYPE = -2, ST_HIP = -5, ST_WORKSPACE = -6;
 
 bool unaligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) != 0; }
@@ -77,6 +83,38 @@ int64_t attend_workspace(const AttendPlan& a, int tokens, int heads, int dim) {
     return a.splits > 1 ? align256((int64_t)a.splits * tokens * heads * dim * 4) +
                               align256((int64_t)a.splits * tokens * heads * 8)
                         : 0;
+}
+
+// A 4-bit cache's call of few rows (attend_few.hip): tokens of a tile, workgroups to
+// share the keys out to, the pieces there is room for.
+struct FewPlan {
+    bool few, join;
+    int tile_tokens, even, pieces;
+};
+
+FewPlan few_plan(int tokens, int seqs, bool single, int heads, int kv_heads, int dim, int64_t most_keys) {
+    FewPlan a{};
+    const int group = heads / kv_heads;
+    a.few = group <= TOKEN_ROWS && (single || (seqs <= FEW_SEQS_MAX && (int64_t)tokens * group <= (int64_t)FEW_ROWS * seqs));
+    if (!a.few) return a;
+    a.tile_tokens = single ? 1 : TOKEN_ROWS / group;
+    // (a round of what the chip holds, and room for uneven ones: 64 ragged sequences 68 us with
+    // 768, 69 with 1024, 74 with 640; 32 at dim 256 21.6 us with 512, 26.5 with 768)
+    a.even = dim == 256 ? 512 : 768;
+    const int64_t tiles = single ? seqs : (int64_t)tokens / a.tile_tokens + seqs, most = (most_keys + 31) / 32;
+    if (single && (seqs > FEW_SEQS_MAX || (int64_t)seqs * kv_heads >= 4 * a.even)) {
+        a.even = 0;
+        a.pieces = seqs;
+        return a;
+    }
+    a.pieces = (int)(tiles + std::min<int64_t>(a.even / kv_heads, tiles * most / FEW_LEAST) + 1);
+    a.join = most > FEW_WHOLE;
+    return a;
+}
+
+int64_t few_workspace(const FewPlan& a, int tokens, int heads, int kv_heads, int dim) {
+    const int64_t rows = (int64_t)a.pieces * kv_heads * a.tile_tokens * (heads / kv_heads);
+    return a.join ? align256(rows * dim * 4) + align256(rows * 8) + align256((int64_t)tokens * kv_heads * 16) : 0;
 }
 
 // sizes both the query call and the attention call have to hold
@@ -283,6 +321,14 @@ int64_t mqh_attend_workspace_bytes(int tokens, int seqs, int single, int heads, 
     return attend_workspace(attend_plan(tokens, seqs, single, heads, kv_heads, dim, most_keys), tokens, heads, dim);
 }
 
+int64_t mqh_attend_f4_workspace_bytes(int tokens, int seqs, int single, int heads, int kv_heads, int dim,
+                                      int64_t most_keys) {
+    if (!attend_sizes(tokens, seqs, single, heads, kv_heads, dim, most_keys)) return ST_ARG;
+    const FewPlan f = few_plan(tokens, seqs, single, heads, kv_heads, dim, most_keys);
+    if (f.few) return few_workspace(f, tokens, heads, kv_heads, dim);
+    return attend_workspace(attend_plan(tokens, seqs, single, heads, kv_heads, dim, most_keys), tokens, heads, dim);
+}
+
 int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int tokens, const int32_t* starts,
                int seqs, int heads, const void* kc, const void* vc, const void* ks, const void* vs, int cache_type,
                int64_t pages, int kv_heads, int page_size, int dim, const int32_t* table, int64_t table_stride,
@@ -298,9 +344,11 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
     const int64_t most = (int64_t)table_cols * page_size;
     if (!attend_sizes(tokens, seqs, single, heads, kv_heads, dim, most)) return ST_ARG;
     if (!(scale > 0.0f) || !(scale < INFINITY) || unaligned(q, 2) || unaligned(out, 16)) return ST_ARG;
+    const FewPlan f = cache_type == MIX_F4 ? few_plan(tokens, seqs, single, heads, kv_heads, dim, most) : FewPlan{};
     const AttendPlan a = attend_plan(tokens, seqs, single, heads, kv_heads, dim, most);
-    if (workspace_bytes < attend_workspace(a, tokens, heads, dim)) return ST_WORKSPACE;
-    if (a.splits > 1 && (!workspace || unaligned(workspace, 256))) return ST_ARG;
+    const int64_t need = f.few ? few_workspace(f, tokens, heads, kv_heads, dim) : attend_workspace(a, tokens, heads, dim);
+    if (workspace_bytes < need) return ST_WORKSPACE;
+    if (need && (!workspace || unaligned(workspace, 256))) return ST_ARG;
     AttendParams p{};
     p.q = q; p.q_token = q_token; p.q_head = q_head; p.q_type = q_type;
     p.kc = kc; p.vc = vc; p.ks = ks; p.vs = vs; p.cache_type = cache_type;
@@ -313,6 +361,13 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
     p.dim = dim; p.page_shift = page_shift_of(page_size); p.pages = (int)pages;
     p.tile_tokens = a.tile_tokens; p.tiles = a.tiles; p.splits = a.splits; p.flags = flags;
     const hipStream_t s = (hipStream_t)stream;
+    if (f.few) {
+        const int64_t rows = (int64_t)f.pieces * kv_heads * f.tile_tokens * p.group;
+        p.tile_tokens = f.tile_tokens; p.even = f.even; p.pieces = f.pieces;
+        p.part_ml = (float*)((uint8_t*)workspace + align256(rows * dim * 4));
+        p.part_rows = f.join ? (int4*)((uint8_t*)p.part_ml + align256(rows * 8)) : nullptr;
+        return status(launch_attend_few(p, s));
+    }
     hipError_t e = a.token ? launch_attend_token(p, s) : launch_attend(p, s);
     if (e == hipSuccess && a.splits > 1) e = launch_attend_join(p, s);
     return status(e);

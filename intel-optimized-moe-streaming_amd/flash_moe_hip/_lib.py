@@ -61,6 +61,7 @@ EXPORTS = (
     "mqh_pages_extend_words",
     "mqh_pages_trim_words",
     "mqh_rotary_words",
+    "mqh_attend_f4_workspace_bytes",
 )
 
 STATUS_TEXT = {
@@ -166,8 +167,9 @@ def _declare(lib: C.CDLL) -> C.CDLL:
     lib.mqh_kv_write.restype = _I
     lib.mqh_kv_read.argtypes = [_P, _I, *cache, _P, _P, _I, _P, _P]
     lib.mqh_kv_read.restype = _I
-    lib.mqh_attend_workspace_bytes.argtypes = [_I, _I, _I, _I, _I, _I, _I64]
-    lib.mqh_attend_workspace_bytes.restype = _I64
+    for f in (lib.mqh_attend_workspace_bytes, lib.mqh_attend_f4_workspace_bytes):
+        f.argtypes = [_I, _I, _I, _I, _I, _I, _I64]
+        f.restype = _I64
     lib.mqh_attend.argtypes = [
         _P, _I64, _I64, _I, _I, _P, _I, _I, *cache,   # q, strides, type, tokens, starts, seqs, heads
         _P, _I64, _I, _P, C.c_float,                  # table, its stride and columns, lengths, scale

@@ -38,8 +38,9 @@ def _types():
 
 
 @functools.lru_cache(maxsize=512)
-def _attend_bytes(lib, tokens, seqs, single, heads, kv_heads, dim, most):
-    return int(lib.mqh_attend_workspace_bytes(tokens, seqs, single, heads, kv_heads, dim, most))
+def _attend_bytes(lib, f4, tokens, seqs, single, heads, kv_heads, dim, most):
+    query = lib.mqh_attend_f4_workspace_bytes if f4 else lib.mqh_attend_workspace_bytes
+    return int(query(tokens, seqs, single, heads, kv_heads, dim, most))
 
 
 def check_rows(t, shape, types, index, what):
@@ -323,8 +324,8 @@ class PagedCache:
         if tokens and seqs:
             if cols == 0:
                 raise ValueError("page_table has no columns")
-            need = _attend_bytes(self.lib, tokens, seqs, int(starts is None), heads, self.kv_heads, self.head_dim,
-                                 cols * self.page_size)
+            need = _attend_bytes(self.lib, self._fixed[4] == F4, tokens, seqs, int(starts is None), heads, self.kv_heads,
+                                 self.head_dim, cols * self.page_size)
             if need < 0:
                 _lib.check(need, "mqh_attend_workspace_bytes")
         return self._run(stream, self._attend, q, out, need, (

@@ -174,6 +174,8 @@ SHAPES = [   # new, lengths, heads, kv_heads, dim, page
     ([9, 9], [777, 64], 128, 1, 64, 64),
     ([300], [2300], 4, 1, 128, 128),
     ([7, 3], [9000, 4000], 4, 2, 128, 16),   # keys split over workgroups
+    ([200, 90], [5000, 700], 4, 2, 64, 64),
+    ([130, 131, 7], [2000, 3100, 900], 8, 1, 256, 16),
 ]
 
 
@@ -310,6 +312,32 @@ def test_bad_pages_and_lengths_are_reported(single):
     c = f4.cache(*p["held"])
     got = call(c, p, single=single)
     assert c.status() == -9 and not got[1].any()
+
+
+@pytest.mark.parametrize("new,lengths", [([2, 1], [300, 40]), ([2, 1], [3000, 4000]), ([150, 200], [300, 400])])
+def test_bad_starts_are_reported(new, lengths):
+    """Starts out of range or out of order, in calls of few rows and of many."""
+    total = sum(new)
+    for starts in ([0, total + 5, 2], [-3, 1, total], [0, 1, total + 9], [total, 0, 1], [1, total, 0]):
+        print(new, lengths, starts, flush=True)
+        p = problem(new, lengths, 4, 2, 64, 16, torch.float16)
+        p["starts"] = torch.tensor(starts, dtype=torch.int32)
+        c = f4.cache(*p["held"])
+        assert call(c, p).shape == (total, 4, 64) and c.status() in (-9, -4), starts   # (rows concerned: undefined)
+
+
+def test_rows_a_tile_and_one_more():
+    """Tiles of 16 rows, full and with one token more, of groups that do not divide 16; keys split and not."""
+    for heads, kv_heads in ((3, 1), (10, 2), (32, 2), (7, 7)):
+        group = heads // kv_heads
+        a = 16 // group
+        for lengths in ([5 + a, 77, 200], [1500, 5000, 2 * a + 1]):
+            new = [a, a + 1, 2 * a + 1]
+            print(heads, kv_heads, lengths, flush=True)
+            p = problem(new, lengths, heads, kv_heads, 128, 16, torch.bfloat16, seed=heads)
+            c = f4.cache(*p["held"])
+            check(call(c, p), p, 128 ** -0.5)
+            assert c.status() == 0
 
 
 def test_many_sequences():
