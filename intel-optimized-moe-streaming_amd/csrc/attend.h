@@ -22,7 +22,8 @@ constexpr float ATTEND_ZERO_SCALE = 0x1p-80f;
 hipError_t launch_attend(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_token(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_join(const AttendParams& p, hipStream_t s);
-hipError_t launch_attend_few(const AttendParams& p, hipStream_t s);   // 4-bit caches
+hipError_t launch_attend_few(const AttendParams& p, hipStream_t s);   // 4-bit caches: few rows, many
+hipError_t launch_attend_f4(const AttendParams& p, hipStream_t s);
 // threads and query rows (32 a wave) of a workgroup of launch_attend, keys of one
 // of its steps, and the workgroups a CU holds
 constexpr int attend_threads(int dim) { return dim == 256 ? 512 : 256; }
@@ -38,10 +39,11 @@ constexpr int attend_krow(int dim) { return 2 * dim + 16; }
 constexpr int attend_vrow(int dim) { return 2 * dim + 64; }
 // query heads a kv head may have in launch_attend_token
 constexpr int TOKEN_ROWS = 16;
-// launch_attend_few: pieces of one tile of rows, sequences whose keys are shared out
-// at most; blocks (32 keys) that one piece takes whole (700 keys: 10.1 us, 13.2 in pieces
-// of 8 and joined), and the fewest of a piece where sequences have more
-constexpr int FEW_SPLITS_MAX = 256, FEW_SEQS_MAX = 1024, FEW_WHOLE = 32, FEW_LEAST = 8;
+// 4-bit caches: pieces of one tile of rows, at most, and the sequences up to which keys
+// are shared out in pieces
+constexpr int PIECE_SPLITS_MAX = 256, PIECE_SEQS_MAX = 1024;
+// threads and query rows of a workgroup of launch_attend_f4
+constexpr int F4_THREADS = 512, F4_ROWS = F4_THREADS / 2;
 
 // the 16-bit type the matrix instructions take: BF16 for BF16 caches, else FP16
 // (8-bit codes are exact in it, and so are FP16 values)

@@ -43,7 +43,6 @@
 #include <type_traits>
 
 #include "attend.h"
-#include "fp4.h"
 
 namespace mqh {
 
@@ -52,12 +51,11 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
     using M = MixMath<CACHE>;
     typedef typename M::vec8 vec8;
     typedef typename M::vec4 vec4;
-    constexpr bool Q8 = CACHE == MIX_Q8, F4 = CACHE == MIX_F4;
-    typedef typename std::conditional<F4, uintx2, uintx4>::type piece_t;
+    constexpr bool Q8 = CACHE == MIX_Q8;
     constexpr int STEP = attend_step(DIM);
     constexpr int KROW = attend_krow(DIM), VROW = attend_vrow(DIM);
     constexpr int KTILE = STEP * KROW, BUFFER = KTILE + STEP * VROW;
-    constexpr int PIECES = Q8 || F4 ? DIM / 16 : DIM / 8;   // 16-byte pieces of a cache row (4-bit: 8 bytes)
+    constexpr int PIECES = Q8 ? DIM / 16 : DIM / 8;    // 16-byte pieces of a cache row
     constexpr int THREADS = attend_threads(DIM);
     constexpr int PASS = THREADS / PIECES;             // keys of one load of every thread
     constexpr int LOADS = STEP / PASS;
@@ -128,11 +126,11 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
     // ---- the query rows as operands: column `col`, d = 16 kk + 8 half + e
     vec8 qf[KR];
     uintx4* q_rest = (uintx4*)(lds + 2 * BUFFER) + wave * (KK - KR) * 64 + lane;
-    float q_scale = 1.0f;   // caches of codes with BF16 queries: what the FP16 operands were multiplied by, inverted
+    float q_scale = 1.0f;   // 8-bit caches with BF16 queries: what the FP16 operands were multiplied by, inverted
     {
         const int64_t at = (int64_t)(seq.first + i0 + (row_live ? r_tok : 0)) * p.q_token +
                            (int64_t)(row_live ? r_head : kvh * p.group) * p.q_head;
-        if constexpr ((Q8 || F4) && QT == MIX_BF16) {
+        if constexpr (Q8 && QT == MIX_BF16) {
             // BF16 to FP16 by a power of two per row that brings its largest value to
             // [1, 2): exact down to 2^-17 of it
             uint32_t top = 0;
@@ -185,8 +183,7 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
         }
         return page;
     };
-    piece_t kr[LOADS], vr[LOADS];
-    uint8_t kf[LOADS], vf[LOADS];   // 4-bit caches: the scales of the pieces' blocks
+    uintx4 kr[LOADS], vr[LOADS];
     float sk = 0, sv = 0;
     auto load_step = [&](int step) {
         const int base = step * STEP, group = (step - step0) * (STEP / 16);
@@ -199,12 +196,8 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
             const int page = __builtin_amdgcn_readlane(pages_now, (group + ((wave_key + PASS * i) >> 4)) & 63);
             const int key = min(base + key_in + PASS * i, keys - 1);
             const int64_t at = ((((int64_t)page * p.kv_heads + kvh) << p.page_shift) + (key & page_mask)) * PIECES + piece;
-            kr[i] = ((const piece_t*)p.kc)[at];
-            vr[i] = ((const piece_t*)p.vc)[at];
-            if constexpr (F4) {
-                kf[i] = ((const uint8_t*)p.ks)[at >> 1];
-                vf[i] = ((const uint8_t*)p.vs)[at >> 1];
-            }
+            kr[i] = ((const uintx4*)p.kc)[at];
+            vr[i] = ((const uintx4*)p.vc)[at];
         }
         if constexpr (Q8) {
             const int page = __shfl(pages_now, (group + (lane >> 4)) & 63);   // (with every lane: it reads all of them)
@@ -236,22 +229,6 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
                 *(uintx4*)(ko + 16) = uintx4{c[0], c[1], d[0], d[1]};
                 *(uintx4*)vo = uintx4{e[0], e[1], f[0], f[1]};
                 *(uintx4*)(vo + 16) = uintx4{g[0], g[1], h[0], h[1]};
-            } else if constexpr (F4) {
-                const float fk = f4_factor(kf[i]), fv = f4_factor(vf[i]);
-                uint8_t* ko = kt + key * KROW + piece * 32;
-                uint8_t* vo = vt + key * VROW + piece * 32;
-                *(uintx4*)ko = f4_to_half(kr[i][0], fk);
-                *(uintx4*)(ko + 16) = f4_to_half(kr[i][1], fk);
-                uintx4 a = f4_to_half(vr[i][0], fv), b2 = f4_to_half(vr[i][1], fv);
-                if (edge && vf[i] == F4_NONE) {
-                    if (base + key < keys) {
-                        for (int c = 0; c < 16; ++c) atomicMin(&s_bad[2][16 * piece + c], base + key);
-                        s_any_bad = 1;
-                    }
-                    a = b2 = uintx4{0, 0, 0, 0};
-                }
-                *(uintx4*)vo = a;
-                *(uintx4*)(vo + 16) = b2;
             } else {
                 *(uintx4*)(kt + key * KROW + piece * 16) = kr[i];
                 if (edge) {
@@ -284,9 +261,6 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
             }
         }
     };
-
-    // (never 0: a hidden key's score stays -infinity)
-    const float f4_scale_log2 = fmaxf(p.scale_log2 * q_scale, 0x1p-126f);
 
     floatx16 o[DB];
 #pragma unroll
@@ -332,7 +306,7 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
             // 8-bit caches: scores in log2 with the keys' scales and log2(vs) (else the
             // softmax scale goes into the exponential's argument)
             const int base = step * STEP;
-            const float c = Q8 ? 1.0f : F4 ? f4_scale_log2 : p.scale_log2;
+            const float c = Q8 ? 1.0f : p.scale_log2;
             if constexpr (Q8) {
 #pragma unroll
                 for (int j = 0; j < KB; ++j)
@@ -537,8 +511,6 @@ template <int DIM>
 static hipError_t launch_attend_dim(const AttendParams& p, hipStream_t s) {
     if (p.cache_type == MIX_F16) return launch_attend_of<DIM, MIX_F16, MIX_F16>(p, s);
     if (p.cache_type == MIX_BF16) return launch_attend_of<DIM, MIX_BF16, MIX_BF16>(p, s);
-    if (p.cache_type == MIX_F4)
-        return p.q_type == MIX_F16 ? launch_attend_of<DIM, MIX_F4, MIX_F16>(p, s) : launch_attend_of<DIM, MIX_F4, MIX_BF16>(p, s);
     if (p.q_type == MIX_F16) return launch_attend_of<DIM, MIX_Q8, MIX_F16>(p, s);
     return launch_attend_of<DIM, MIX_Q8, MIX_BF16>(p, s);
 }

@@ -20,123 +20,11 @@
 // transposed; 16-byte pieces are exchanged so that neither the writes (8 lanes: two
 // keys' pieces) nor the transposing reads (4 keys) meet in a bank.
 
-#include "attend.h"
-#include "fp4.h"
+#include "attend_pieces.h"
 
 namespace mqh {
 
 constexpr int FEW_BLOCK = 32;   // keys
-
-// sums, or the largest, over the lanes up to this one
-template <class T, class F>
-__device__ __forceinline__ T scan_lanes(T x, T none, F op) {
-    const int n = __builtin_bit_cast(int, none);
-    const auto step = [&](auto moved) { x = op(x, __builtin_bit_cast(T, moved)); };
-    step(__builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, x), 0x111, 0xf, 0xf, false));   // from 1, 2, 4, 8 lanes
-    step(__builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, x), 0x112, 0xf, 0xf, false));   // below, of 16
-    step(__builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, x), 0x114, 0xf, 0xf, false));
-    step(__builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, x), 0x118, 0xf, 0xf, false));
-    step(__builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, x), 0x142, 0xa, 0xf, false));   // the 16's last to the next
-    step(__builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, x), 0x143, 0xc, 0xf, false));   // the 32's to the others
-    return x;
-}
-template <class T>
-__device__ __forceinline__ T last_lane(T x) {
-    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
-}
-
-struct FewPiece {
-    int b, tile, split, splits, first;   // first: the tile's first piece
-    int per;                             // blocks of a piece
-    SeqRange seq;
-    bool live;
-};
-
-// Sequence i's tokens and length with every bound forced into what the tensors hold.
-__device__ __forceinline__ bool few_sequence(const AttendParams& p, int i, SeqRange& r) {
-    int s0 = i, s1 = i + 1;
-    bool bad = false;
-    if (p.starts) {
-        s0 = p.starts[i];
-        s1 = p.starts[i + 1];
-        bad = s0 < 0 || s1 < s0 || s1 > p.tokens;
-        s0 = min(max(s0, 0), p.tokens);
-        s1 = min(max(s1, s0), p.tokens);
-    }
-    const int len = p.lengths[i], most = p.table_cols << p.page_shift;
-    bad |= len < 0 || len > most;
-    r.first = s0;
-    r.count = s1 - s0;
-    r.length = min(max(len, 0), most);
-    return bad;
-}
-
-__device__ __forceinline__ FewPiece few_piece(const AttendParams& p, int piece, bool report) {
-    FewPiece r{};
-    const int lane = threadIdx.x & 63;
-    if (!p.even) {   // one piece a sequence, and nothing to sum
-        r.b = piece;
-        r.splits = 1;
-        r.first = piece;
-        r.per = 1 << 30;
-        r.live = true;
-        if (few_sequence(p, piece, r.seq) && lane == 0) atomicOr(&p.flags[FLAG_BAD_ID], 1);
-        return r;
-    }
-    // ---- blocks of all sequences, and of the longest
-    SeqRange seq{};
-    int longest = 0, all_tiles = 0;
-    float total = 0.0f;
-    bool bad = false;
-    for (int i0 = 0; i0 < p.seqs; i0 += 64) {
-        seq = SeqRange{};
-        if (i0 + lane < p.seqs) bad |= few_sequence(p, i0 + lane, seq);
-        const int tiles = (seq.count + p.tile_tokens - 1) / p.tile_tokens, blocks = (seq.length + FEW_BLOCK - 1) / FEW_BLOCK;
-        total += (float)tiles * (float)blocks;
-        all_tiles += tiles;
-        longest = max(longest, blocks);
-    }
-    if (report && bad) atomicOr(&p.flags[FLAG_BAD_ID], 1);
-    const auto add = [](auto a, auto b) { return a + b; };
-    total = last_lane(scan_lanes(total, 0.0f, add));
-    all_tiles = last_lane(scan_lanes(all_tiles, 0, add));
-    longest = last_lane(scan_lanes(longest, 0, [](int a, int b) { return max(a, b); }));
-    // (a tile's last piece is half full on average; the total is off by less than 80 * 2^-24)
-    const int want = max(max(p.even / p.kv_heads - all_tiles / 2, p.even / p.kv_heads / 2), 1);
-    int per = (int)fminf(total * 1.00001f / (float)want, 1e9f) + 1;
-    per = max(per, (longest + FEW_SPLITS_MAX - 1) / FEW_SPLITS_MAX);
-    r.per = longest <= FEW_WHOLE ? FEW_WHOLE : max((per + 3) & ~3, FEW_LEAST);
-    // ---- this piece's sequence
-    int before = 0;
-    for (int i0 = 0; i0 < p.seqs; i0 += 64) {
-        if (p.seqs > 64) {   // (else the first loop's values are still here)
-            seq = SeqRange{};
-            if (i0 + lane < p.seqs) few_sequence(p, i0 + lane, seq);
-        }
-        const int tiles = (seq.count + p.tile_tokens - 1) / p.tile_tokens, blocks = (seq.length + FEW_BLOCK - 1) / FEW_BLOCK;
-        const int splits = max((blocks + r.per - 1) / r.per, 1);
-        const int mine = tiles * splits;
-        const int sum = scan_lanes(mine, 0, add);
-        const int at = piece - before - (sum - mine);
-        const uint64_t hit = __ballot(at >= 0 && at < mine);
-        if (hit) {
-            const int who = __builtin_ctzll(hit);
-            r.b = i0 + who;
-            r.splits = __builtin_amdgcn_readlane(splits, who);
-            const int local = __builtin_amdgcn_readlane(at, who);
-            r.tile = local / r.splits;
-            r.split = local - r.tile * r.splits;
-            r.first = piece - r.split;
-            r.seq.first = __builtin_amdgcn_readlane(seq.first, who);
-            r.seq.count = __builtin_amdgcn_readlane(seq.count, who);
-            r.seq.length = __builtin_amdgcn_readlane(seq.length, who);
-            r.live = true;
-            return r;
-        }
-        before += __builtin_amdgcn_readlane(sum, 63);
-    }
-    return r;
-}
 
 template <int DIM, int QT>
 __global__ __launch_bounds__(256, DIM == 256 ? 2 : 4) void k_attend_few(AttendParams p) {
@@ -158,14 +46,9 @@ __global__ __launch_bounds__(256, DIM == 256 ? 2 : 4) void k_attend_few(AttendPa
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % p.kv_heads, piece = blockIdx.x / p.kv_heads;
-    FewPiece w = few_piece(p, piece, blockIdx.x == 0 && wave == 0);
+    const Piece w = piece_of(p, piece, FEW_BLOCK, blockIdx.x == 0 && wave == 0);
     if (!w.live) return;
-    w.b = __builtin_amdgcn_readfirstlane(w.b);
-    w.tile = __builtin_amdgcn_readfirstlane(w.tile);
-    w.split = __builtin_amdgcn_readfirstlane(w.split);
-    w.per = __builtin_amdgcn_readfirstlane(w.per);
-    const SeqRange seq = {__builtin_amdgcn_readfirstlane(w.seq.first), __builtin_amdgcn_readfirstlane(w.seq.count),
-                          __builtin_amdgcn_readfirstlane(w.seq.length)};
+    const SeqRange seq = w.seq;
     const int i0 = w.tile * p.tile_tokens, n_tok = min(p.tile_tokens, seq.count - i0);
     const int first_pos = seq.length - seq.count + i0;   // position of the tile's first token (negative: it sees nothing)
     const int r_tok = col / p.group, r_head = kvh * p.group + col - r_tok * p.group;
@@ -461,99 +344,13 @@ __global__ __launch_bounds__(256, DIM == 256 ? 2 : 4) void k_attend_few(AttendPa
         p.part_rows[(int64_t)(seq.first + i0 + tid) * p.kv_heads + kvh] = int4{w.first, w.splits, tid, 0};
 }
 
-// The pieces of a row joined, a workgroup CH channels of a row: thread i first takes
-// piece i's exponent and sum, then CH / 4 threads four channels each of every
-// 1024 / CH-th piece (always in the same order).
-template <int DIM, int QT, int CH>
-__global__ __launch_bounds__(256) void k_few_join(AttendParams p) {
-    constexpr int LANES = CH / 4, SUBS = 256 / LANES, N = 4;
-    __shared__ float s_w[FEW_SPLITS_MAX], s_top[4], s_sum[4];
-    __shared__ floatx4 s_part[SUBS][LANES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int out_row = blockIdx.x / (DIM / CH), t = out_row / p.heads, h = out_row - t * p.heads, kvh = h / p.group;
-    if (p.starts && (t < p.starts[0] || t >= p.starts[p.seqs])) return;   // rows of no sequence stay as they were
-    const int4 from = p.part_rows[(int64_t)t * p.kv_heads + kvh];
-    // (where starts are out of order a row may have no entry: what is read is kept within the workspace)
-    const int first = min(max(from.x, 0), p.pieces - 1), splits = min(min(from.y, FEW_SPLITS_MAX), p.pieces - first);
-    if (splits <= 1) return;
-    const int R = p.tile_tokens * p.group, r = min(max(from.z, 0), p.tile_tokens - 1) * p.group + h - kvh * p.group;
-    const int64_t row = ((int64_t)first * p.kv_heads + kvh) * R + r, step = (int64_t)p.kv_heads * R;   // of a piece, in rows
-    const float2 ml = tid < splits ? ((const float2*)p.part_ml)[row + tid * step] : float2{-INFINITY, 0.0f};
-    const int sub = tid / LANES, ch = blockIdx.x % (DIM / CH) * CH + (tid % LANES) * 4;
-    floatx4 v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        v[i] = *(const floatx4*)(p.part_o + (row + min(sub + i * SUBS, splits - 1) * step) * DIM + ch);
-    float top = ml.x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (lane == 0) s_top[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-    // (a piece without keys for this row weighs nothing)
-    const float ref = top == -INFINITY ? 0.0f : top;
-    const float weight = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - ref);
-    float l = weight * ml.y;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-    if (lane == 0) s_sum[wave] = l;
-    s_w[tid] = weight;
-    __syncthreads();
-    l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-    floatx4 sum = {0, 0, 0, 0};
-    for (int s0 = sub; s0 < splits; s0 += N * SUBS) {
-        floatx4 now[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) now[i] = v[i];
-        if (s0 + N * SUBS < splits) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                v[i] = *(const floatx4*)(p.part_o + (row + min(s0 + (N + i) * SUBS, splits - 1) * step) * DIM + ch);
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int s = s0 + i * SUBS;
-            if (s < splits) {   // (also where the weight is 0: infinity and NaN stay so)
-                const float x = s_w[s];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] = fmaf(x, now[i][e], sum[e]);
-            }
-        }
-    }
-    s_part[sub][tid % LANES] = sum;
-    __syncthreads();
-    if (tid >= LANES) return;
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    bool finite = true;
-    uint16_t y[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        float x = s_part[0][tid][e];
-#pragma unroll
-        for (int i = 1; i < SUBS; ++i) x += s_part[i][tid][e];
-        x *= inv;
-        finite &= fits<QT>(x);
-        if constexpr (QT == MIX_F16) y[e] = __builtin_bit_cast(uint16_t, (_Float16)x);
-        else y[e] = __builtin_bit_cast(uint16_t, (__bf16)x);
-    }
-    __builtin_memcpy(__builtin_assume_aligned((uint16_t*)p.out + (int64_t)out_row * DIM + ch, 8), y, 8);
-    if (!finite) atomicOr(&p.flags[FLAG_NONFINITE], 1);
-}
-
 template <int DIM, int QT>
 static hipError_t launch_few_of(const AttendParams& p, hipStream_t s) {
     constexpr int SEC = DIM == 256 ? 128 : DIM;
     const int bytes = std::max(4 * FEW_BLOCK * SEC * 2, 4 * p.tile_tokens * p.group * (DIM + 4) * 4);
     hipLaunchKernelGGL((k_attend_few<DIM, QT>), dim3((unsigned)(p.pieces * p.kv_heads)), dim3(256), bytes, s, p);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess && p.part_rows) {
-        // (few rows: 64 channels a workgroup, for more of them and more pieces in flight)
-        const unsigned rows = (unsigned)(p.tokens * p.heads);
-        if (rows <= 256) hipLaunchKernelGGL((k_few_join<DIM, QT, 64>), dim3(rows * (DIM / 64)), dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((k_few_join<DIM, QT, DIM>), dim3(rows), dim3(256), 0, s, p);
-        e = hipGetLastError();
-    }
-    return e;
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? launch_pieces_join(p, s) : e;
 }
 
 template <int DIM>

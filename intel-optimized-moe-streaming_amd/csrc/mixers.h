@@ -55,10 +55,10 @@ struct AttendParams {
     int tile_tokens;            // query tokens of a workgroup
     int tiles;                  // workgroups a kv head and split
     int splits;
-    // few rows (launch_attend_few): workgroups to share the keys out to (0: one piece a
-    // sequence) and the pieces there is room for; the sums are [pieces x kv_heads x tile
-    // rows] then
-    int even, pieces;
+    // 4-bit caches: workgroups to share the keys out to (0: a piece a tile), blocks of keys
+    // that one piece takes whole and the fewest of a piece where there are more, pieces
+    // there is room for; the sums are [pieces x kv_heads x tile rows] then
+    int even, whole, least, pieces;
     int4* part_rows;            // [tokens x kv_heads]: a token's first piece, its pieces, its place in the tile; or null
     int* flags;
 };

@@ -13,12 +13,6 @@ using namespace mqh;
 
 namespace {
 
-// Rows of a sequence, on average, up to which a 4-bit cache's call is one of few rows: 32
-// sequences of 4,000 keys, 32 heads of 128 over 8, take 42 us there with 16 rows (63 in
-// launch_attend's tiles), 78 with 64 (114), 135 with 128 (138); 4 sequences of 8,000 keys
-// 47 with 128 rows (49), 75 with 256 (62).
-constexpr int FEW_ROWS = 128;
-
 constexpr int ST_OK = 0, ST_ARG = -1, ST_TYPE = -2, ST_HIP = -5, ST_WORKSPACE = -6;
 
 bool unaligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) != 0; }
@@ -85,34 +79,43 @@ int64_t attend_workspace(const AttendPlan& a, int tokens, int heads, int dim) {
                         : 0;
 }
 
-// A 4-bit cache's call of few rows (attend_few.hip): tokens of a tile, workgroups to
-// share the keys out to, the pieces there is room for.
-struct FewPlan {
+// Rows of a sequence, on average, up to which a 4-bit cache's call is one of few rows: 32
+// sequences of 4,000 keys, 32 heads of 128 over 8, take 42 us there with 16 rows (63 in
+// launch_attend's tiles), 78 with 64 (114), 135 with 128 (138); 4 sequences of 8,000 keys
+// 47 with 128 rows (49), 75 with 256 (62).
+constexpr int FEW_ROWS = 128;
+
+// A call on a 4-bit cache.  Few rows (attend_few.hip): tiles of 16 rows, pieces for one
+// round of what the chip holds and room for uneven ones (64 ragged sequences 68 us with
+// 768 workgroups, 69 with 1024, 74 with 640; 32 at dim 256 21.6 us with 512, 26.5 with
+// 768); 1,024 keys are no more than one piece (700 keys: 10.1 us, 13.2 in pieces and
+// joined).  Many rows (attend_f4.hip): one round, a workgroup a CU, unless the tiles alone
+// are as many (2,048 rows after 30,000, 32 heads of 128 over 8: 922 us unsplit, 1,110 in
+// two rounds; four chunks of 2,048 in all at dim 256: 465 us, 472 in two, 793 unsplit).
+struct F4Plan {
     bool few, join;
-    int tile_tokens, even, pieces;
+    int tile_tokens, even, whole, least, pieces;
 };
 
-FewPlan few_plan(int tokens, int seqs, bool single, int heads, int kv_heads, int dim, int64_t most_keys) {
-    FewPlan a{};
+F4Plan f4_plan(int tokens, int seqs, bool single, int heads, int kv_heads, int dim, int64_t most_keys) {
+    F4Plan a{};
     const int group = heads / kv_heads;
-    a.few = group <= TOKEN_ROWS && (single || (seqs <= FEW_SEQS_MAX && (int64_t)tokens * group <= (int64_t)FEW_ROWS * seqs));
-    if (!a.few) return a;
-    a.tile_tokens = single ? 1 : TOKEN_ROWS / group;
-    // (a round of what the chip holds, and room for uneven ones: 64 ragged sequences 68 us with
-    // 768, 69 with 1024, 74 with 640; 32 at dim 256 21.6 us with 512, 26.5 with 768)
-    a.even = dim == 256 ? 512 : 768;
-    const int64_t tiles = single ? seqs : (int64_t)tokens / a.tile_tokens + seqs, most = (most_keys + 31) / 32;
-    if (single && (seqs > FEW_SEQS_MAX || (int64_t)seqs * kv_heads >= 4 * a.even)) {
-        a.even = 0;
-        a.pieces = seqs;
-        return a;
-    }
-    a.pieces = (int)(tiles + std::min<int64_t>(a.even / kv_heads, tiles * most / FEW_LEAST) + 1);
-    a.join = most > FEW_WHOLE;
+    a.few = group <= TOKEN_ROWS && (single || (int64_t)tokens * group <= (int64_t)FEW_ROWS * seqs);
+    const int rows = a.few ? TOKEN_ROWS : F4_ROWS, block = a.few ? 32 : attend_step(dim);
+    a.tile_tokens = single ? 1 : rows / group;
+    a.whole = a.few ? 32 : 1024 / block;
+    a.least = a.few ? 8 : 512 / block;
+    a.even = !a.few ? 256 : dim == 256 ? 512 : 768;
+    // (tiles enough by themselves: nothing is split)
+    const int64_t tiles_least = single ? seqs : tokens / a.tile_tokens, tiles = single ? seqs : (int64_t)tiles_least + seqs;
+    if (seqs > PIECE_SEQS_MAX || tiles_least * kv_heads >= (a.few ? 4 : 1) * a.even) a.even = 0;
+    const int64_t most = (most_keys + block - 1) / block;
+    a.pieces = (int)(tiles + (a.even ? std::min<int64_t>(a.even / kv_heads, tiles * most / a.least) + 1 : 0));
+    a.join = a.even && most > a.whole;
     return a;
 }
 
-int64_t few_workspace(const FewPlan& a, int tokens, int heads, int kv_heads, int dim) {
+int64_t f4_workspace(const F4Plan& a, int tokens, int heads, int kv_heads, int dim) {
     const int64_t rows = (int64_t)a.pieces * kv_heads * a.tile_tokens * (heads / kv_heads);
     return a.join ? align256(rows * dim * 4) + align256(rows * 8) + align256((int64_t)tokens * kv_heads * 16) : 0;
 }
@@ -324,9 +327,7 @@ int64_t mqh_attend_workspace_bytes(int tokens, int seqs, int single, int heads, 
 int64_t mqh_attend_f4_workspace_bytes(int tokens, int seqs, int single, int heads, int kv_heads, int dim,
                                       int64_t most_keys) {
     if (!attend_sizes(tokens, seqs, single, heads, kv_heads, dim, most_keys)) return ST_ARG;
-    const FewPlan f = few_plan(tokens, seqs, single, heads, kv_heads, dim, most_keys);
-    if (f.few) return few_workspace(f, tokens, heads, kv_heads, dim);
-    return attend_workspace(attend_plan(tokens, seqs, single, heads, kv_heads, dim, most_keys), tokens, heads, dim);
+    return f4_workspace(f4_plan(tokens, seqs, single != 0, heads, kv_heads, dim, most_keys), tokens, heads, kv_heads, dim);
 }
 
 int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int tokens, const int32_t* starts,
@@ -344,9 +345,10 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
     const int64_t most = (int64_t)table_cols * page_size;
     if (!attend_sizes(tokens, seqs, single, heads, kv_heads, dim, most)) return ST_ARG;
     if (!(scale > 0.0f) || !(scale < INFINITY) || unaligned(q, 2) || unaligned(out, 16)) return ST_ARG;
-    const FewPlan f = cache_type == MIX_F4 ? few_plan(tokens, seqs, single, heads, kv_heads, dim, most) : FewPlan{};
+    const bool f4 = cache_type == MIX_F4;
+    const F4Plan f = f4 ? f4_plan(tokens, seqs, single, heads, kv_heads, dim, most) : F4Plan{};
     const AttendPlan a = attend_plan(tokens, seqs, single, heads, kv_heads, dim, most);
-    const int64_t need = f.few ? few_workspace(f, tokens, heads, kv_heads, dim) : attend_workspace(a, tokens, heads, dim);
+    const int64_t need = f4 ? f4_workspace(f, tokens, heads, kv_heads, dim) : attend_workspace(a, tokens, heads, dim);
     if (workspace_bytes < need) return ST_WORKSPACE;
     if (need && (!workspace || unaligned(workspace, 256))) return ST_ARG;
     AttendParams p{};
@@ -361,12 +363,12 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
     p.dim = dim; p.page_shift = page_shift_of(page_size); p.pages = (int)pages;
     p.tile_tokens = a.tile_tokens; p.tiles = a.tiles; p.splits = a.splits; p.flags = flags;
     const hipStream_t s = (hipStream_t)stream;
-    if (f.few) {
+    if (f4) {
         const int64_t rows = (int64_t)f.pieces * kv_heads * f.tile_tokens * p.group;
-        p.tile_tokens = f.tile_tokens; p.even = f.even; p.pieces = f.pieces;
+        p.tile_tokens = f.tile_tokens; p.even = f.even; p.whole = f.whole; p.least = f.least; p.pieces = f.pieces;
         p.part_ml = (float*)((uint8_t*)workspace + align256(rows * dim * 4));
         p.part_rows = f.join ? (int4*)((uint8_t*)p.part_ml + align256(rows * 8)) : nullptr;
-        return status(launch_attend_few(p, s));
+        return status(f.few ? launch_attend_few(p, s) : launch_attend_f4(p, s));
     }
     hipError_t e = a.token ? launch_attend_token(p, s) : launch_attend(p, s);
     if (e == hipSuccess && a.splits > 1) e = launch_attend_join(p, s);

@@ -50,7 +50,7 @@ class PageTable:
             check_index(t, shape, torch.int32, index, what)
         if index < 0:
             raise ValueError(f"expected a CUDA device, got {table.device}")
-        self._held = (table, lengths, free, count)
+        self._held, self._fixed = (table, lengths, free, count), None
         self.sequences, self.columns, self.pages, self.page_size = sequences, columns, free.shape[0], page_size
         self.device = table.device
         self.lib = _lib.load()
@@ -73,14 +73,21 @@ class PageTable:
                    torch.arange(pages - 1, -1, -1, **as_int), torch.full((1,), pages, **as_int), page_size)
 
     def _words(self):
+        """The table's share of a call's words, at the addresses its tensors have now
+        (their storage may have moved)."""
         table, lengths, free, count = self._held
+        w = self._fixed
+        if w and table.data_ptr() == w[0] and lengths.data_ptr() == w[2] and free.data_ptr() == w[3] and (
+                count.data_ptr() == w[4]):
+            return w
         for t, shape in ((table, (self.sequences, self.columns)), (lengths, (self.sequences,)), (free, (self.pages,)),
                          (count, (1,))):
             if t.shape != shape or t.dtype != self._int32 or t.get_device() != self._index or not t.is_contiguous() or (
                     t.untyped_storage().nbytes() < (t.storage_offset() + t.numel()) * 4):
                 raise ValueError(f"a tensor of the table is no longer int32 {tuple(shape)}, contiguous, on {self.device}")
-        return (table.data_ptr(), self.columns, lengths.data_ptr(), free.data_ptr(), count.data_ptr(), self.sequences,
-                self.pages, self.page_size)
+        self._fixed = w = (table.data_ptr(), self.columns, lengths.data_ptr(), free.data_ptr(), count.data_ptr(),
+                           self.sequences, self.pages, self.page_size)
+        return w
 
     def extend(self, new, tokens: int, *, stream=None):
         """Room for new[b] >= 0 more tokens of each sequence (int32 [sequences]), in a
