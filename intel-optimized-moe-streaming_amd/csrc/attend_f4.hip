@@ -21,8 +21,8 @@
 
 namespace mqh {
 
-// kinds of instructions, as the scheduler numbers them, and LDS reads ahead of products
-constexpr int SCHED_MFMA = 0x8, SCHED_DS_READ = 0x100, SCHED_DS_WRITE = 0x200, SCHED_EXP = 0x400, AHEAD = 16;
+// kinds of instructions, as the scheduler numbers them
+constexpr int SCHED_MFMA = 0x8, SCHED_DS_READ = 0x100, SCHED_DS_WRITE = 0x200, SCHED_EXP = 0x400;
 
 template <int DIM, int QT>
 __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
@@ -100,7 +100,8 @@ __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
             else q_rest[(kk - KR) * 64] = __builtin_bit_cast(uintx4, v);
         }
     }
-    const float c = fmaxf(q_scale * p.scale_log2, 0x1p-126f);   // (never 0: a hidden key's score stays -infinity)
+    // (never 0 nor infinity: a hidden key's score stays -infinity, one of 0 stays 0)
+    const float c = fminf(fmaxf(q_scale * p.scale_log2, 0x1p-126f), 0x1p127f);
 
     // ---- loading: piece tid % PIECES of key tid / PIECES
     const int part = tid % PIECES, key_in = tid / PIECES;
@@ -173,27 +174,20 @@ __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
 
     floatx16 s[KB];      // scores, then of the next step
     vec8 probs[TB];
-    // O^T += V^T P^T: product t, d
-    auto values = [&](int buf) {
-#pragma unroll
-        for (int t = 0; t < TB; ++t)
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const uint8_t* at = v_from + buf * VTILE + 16 * t * VROW + 64 * d;
-                const vec4 lo = lds_transposed<vec4>(at), hi = lds_transposed<vec4>(at + 8 * VROW);
-                o[d] = M::mfma32(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), probs[t], o[d]);
-            }
+    // product i of O^T += V^T P^T, of S^T = K Q^T
+    auto value = [&](int buf, int i) {
+        const int t = i / DB, d = i % DB;
+        const uint8_t* at = v_from + buf * VTILE + 16 * t * VROW + 64 * d;
+        const vec4 lo = lds_transposed<vec4>(at), hi = lds_transposed<vec4>(at + 8 * VROW);
+        o[d] = M::mfma32(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), probs[t], o[d]);
     };
-    // S^T = K Q^T
-    auto scores = [&](int buf) {
-#pragma unroll
-        for (int j = 0; j < KB; ++j) s[j] = floatx16{0};
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-            for (int j = 0; j < KB; ++j)
-                s[j] = M::mfma32(bits_as<vec8>(*(const uintx4*)(k_from + buf * KTILE + 32 * j * KROW + 32 * kk)), query(kk), s[j]);
+    auto score = [&](int buf, int i) {
+        const int kk = i / KB, j = i % KB;
+        if (kk == 0) s[j] = floatx16{0};
+        s[j] = M::mfma32(bits_as<vec8>(*(const uintx4*)(k_from + buf * KTILE + 32 * j * KROW + 32 * kk)), query(kk), s[j]);
     };
+    constexpr int PRODUCTS = TB * DB;   // of each
+    static_assert(PRODUCTS == KB * KK, "as many products of values as of keys");
     // step t's reference exponent
     auto reference = [&](int t) {
         const int base = (step0 + t) * STEP;
@@ -277,7 +271,9 @@ __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
             load(0);
             __syncthreads();
         }
-        if (wave_live) scores(0);
+        if (wave_live)
+#pragma unroll
+            for (int i = 0; i < PRODUCTS; ++i) score(0, i);
         __syncthreads();
         for (int t = 0; t < n; ++t) {
             turn_pages(t + 1);
@@ -298,19 +294,29 @@ __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
             __syncthreads();
             if (wave_live) {
                 __builtin_amdgcn_s_setprio(1);
-                values(t & 1);
-                scores((t + 1) & 1);   // (past the last step: of keys that are there, for nothing)
-                load(t + 1);
-                if constexpr (DIM != 256) {
-                    // operands are read ahead of the products that they are for
-                    __builtin_amdgcn_sched_group_barrier(SCHED_DS_READ, AHEAD, 0);
+                // (scores past the last step: of keys that are there, for nothing)
+                if constexpr (DIM == 256) {
+                    // (no registers for more: 465 us for four chunks of 2,048 rows in all, 476 with
+                    // the two products' instructions in turn, 707 with six reads ahead)
 #pragma unroll
-                    for (int i = 0; i < TB * DB; ++i) {
+                    for (int i = 0; i < PRODUCTS; ++i) value(t & 1, i);
+#pragma unroll
+                    for (int i = 0; i < PRODUCTS; ++i) score((t + 1) & 1, i);
+                    load(t + 1);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < PRODUCTS; ++i) {
+                        value(t & 1, i);
+                        score((t + 1) & 1, i);
+                    }
+                    load(t + 1);
+                    // operands are read ahead of the products that they are for (a prompt of 8,192
+                    // tokens 502 us, 517 in the compiler's order)
+                    __builtin_amdgcn_sched_group_barrier(SCHED_DS_READ, 8, 0);
+#pragma unroll
+                    for (int i = 0; i < PRODUCTS; ++i) {
                         __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, 1, 0);
                         __builtin_amdgcn_sched_group_barrier(SCHED_DS_READ, 2, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < KB * KK; ++i) {
                         __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, 1, 0);
                         __builtin_amdgcn_sched_group_barrier(SCHED_DS_READ, 1, 0);
                     }
