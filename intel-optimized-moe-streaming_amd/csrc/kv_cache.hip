@@ -18,7 +18,8 @@
 // head of consecutive tokens, whose scales usually share a line: with the heads of
 // a token together, every line of scales was written piecemeal from several XCDs.
 // 16,384 BF16 tokens of 8 heads of 128: 27.1 us written as codes (3.8 TB/s), 16.8 read
-// back (6.0 TB/s, in part from the last-level cache).
+// back (6.0 TB/s, in part from the last-level cache); as 4-bit codes 18.9 us (4.5 TB/s) and
+// 15.7.
 
 #include "fp4.h"
 #include "mixers.h"

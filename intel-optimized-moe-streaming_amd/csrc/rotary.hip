@@ -13,7 +13,9 @@
 //
 // Bound by memory: rows are read and written once.  dim / 8 lanes own a row, eight
 // channels each; a workgroup takes the same few tokens of several heads, so that
-// the sines are computed once for all of them.
+// the sines are computed once for all of them.  16,384 tokens of 32 + 8 heads of 128,
+// BF16: 70 us, 4.8 TB/s (a large copy reaches 4.7 to 4.8); 4,099 FP32 tokens of 16 + 2
+// heads of 256, normed: 34 us, 4.5 TB/s.  64 tokens: 5 us, two round trips and the sines.
 
 #include "mixers.h"
 
