@@ -107,8 +107,9 @@ __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
             else q_rest[(kk - KR) * 64] = __builtin_bit_cast(uintx4, v);
         }
     }
-    // (never 0 nor infinity: a hidden key's score stays -infinity, one of 0 stays 0)
-    const float c = fminf(fmaxf(q_scale * p.scale_log2, 0x1p-126f), 0x1p127f);
+    // (never 0: a hidden key's score stays -infinity; at most 2^86: products of 2^40 at the
+    // most stay finite, and such a softmax is its largest score's already)
+    const float c = fminf(fmaxf(q_scale * p.scale_log2, 0x1p-126f), 0x1p86f);
 
     // ---- loading: piece tid % PIECES of key tid / PIECES
     const int part = tid % PIECES, key_in = tid / PIECES;

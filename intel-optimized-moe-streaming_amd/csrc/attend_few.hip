@@ -168,8 +168,9 @@ __global__ __launch_bounds__(256, DIM == 256 ? 2 : 4) void k_attend_few(AttendPa
             for (int kk = 0; kk < KK; ++kk) qf[kk] = bits_as<vec8>(raw[kk]);
         }
     }
-    // (never 0 nor infinity: a hidden key's score stays -infinity, one of 0 stays 0)
-    const float c = fminf(fmaxf(q_scale * p.scale_log2, 0x1p-126f), 0x1p127f);
+    // (never 0: a hidden key's score stays -infinity; at most 2^86: products of 2^40 at the
+    // most stay finite, and such a softmax is its largest score's already)
+    const float c = fminf(fmaxf(q_scale * p.scale_log2, 0x1p-126f), 0x1p86f);
 
     // ---- the V tile: which 16-byte pieces of a key are exchanged (xor), and this lane's places
     auto swap = [](int key) { return DIM == 64 ? (key & 6) | (key >> 1 & 1) : (key & 7) << 1 | (key >> 1 & 1); };

@@ -430,3 +430,80 @@ def test_captured_replayed_and_other_streams(single):
             assert torch.equal(c.attend(other, table, lengths, **kw), want2)
             assert torch.equal(y, w)
     assert c.status() == 0
+
+
+@pytest.mark.parametrize("kind", ["single", "few", "many"])
+def test_more_sequences_than_keys_are_shared_out_for(kind):
+    """Past 1,024 sequences every tile is one piece: single tokens, a few of each, tiles of many rows."""
+    seqs = 1100
+    new = [1] * seqs if kind == "single" else [(i * 7) % 4 for i in range(seqs)] if kind == "few" else [
+        (i * 5) % 67 for i in range(seqs)]
+    lengths = [n + (i * 37) % 90 if i % 7 else n for i, n in enumerate(new)]
+    lengths[700] = new[700] + 3000
+    p = problem(new, lengths, 8, 2, 64, 16, torch.bfloat16, seed=2)
+    c = f4.cache(*p["held"])
+    got = call(c, p, single=kind == "single").cpu()
+    assert c.status() == 0
+    ends = p["starts"].tolist()
+    for b in list(range(0, seqs, 43)) + [699, 700, 701, seqs - 1]:
+        if new[b]:
+            want, bound = ref.attend(p["q"][ends[b]:ends[b + 1]], p["k"][b], p["v"][b], 0.125, torch.int8)
+            assert ((got[ends[b]:ends[b + 1]].double() - want).abs() <= bound).all(), b
+    if kind != "single":
+        for starts in (torch.roll(p["starts"], 5), p["starts"] + 3, -p["starts"]):
+            p["starts"] = starts.contiguous()
+            assert call(c, p).shape == got.shape and c.status() in (-9, -4)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 300]])
+def test_two_calls_at_once(new):
+    """Two streams, one cache: each call has its own workspace."""
+    p = problem(new, [9000, 5000], 8, 2, 128, 64, torch.bfloat16, seed=4)
+    c = f4.cache(*p["held"])
+    q, table, lengths, starts = (t.cuda() for t in (p["q"], p["table"], p["lengths"], p["starts"]))
+    other = torch.randn_like(q.float()).to(q.dtype)
+    want = [c.attend(x, table, lengths, starts) for x in (q, other)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, (x, s) in enumerate(zip((q, other), streams)):
+            got[i].append(c.attend(x, table, lengths, starts, stream=s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs) and c.status() == 0
+
+
+def test_a_cache_follows_its_tensors():
+    from flash_moe_hip.kv_cache import PagedCache
+
+    c = PagedCache.empty(2, 1, 64, 16, f4.CODES)
+    x = rows(1, 1, 64, torch.float16, 1)
+    slots = torch.tensor([17]).cuda()
+    c.write(x, x, slots)
+    before = c.k.detach()
+    kept = before.view(torch.uint8).clone()
+    c.k.set_(torch.zeros(2, 1, 16, 32, dtype=torch.uint8, device="cuda").view(f4.CODES))
+    c.write(2 * x, 2 * x, slots)
+    assert torch.equal(before.view(torch.uint8), kept) and c.k.view(torch.uint8).any()
+    k, v = c.read(slots)
+    assert torch.equal(k, v) and c.status() == 0
+    c.v_scale.data = torch.zeros(2, 1, 16, 2, dtype=torch.uint8, device="cuda")
+    with pytest.raises(ValueError, match="no longer"):
+        c.read(slots)
+
+
+@pytest.mark.parametrize("new", [1, 5, 60])
+def test_large_queries_and_scales(new):
+    """A query's power of two times the softmax scale past FP32: scores of 0 stay 0, the largest key alone is left."""
+    p = problem([new], [300], 4, 2, 64, 16, torch.bfloat16, seed=6)
+    q = torch.zeros(new, 4, 64)
+    q[..., 0] = 1e38
+    k = torch.zeros(300, 2, 64)
+    k[1, :, 0] = 6.0
+    p["held"][0], p["held"][2], p["k"] = f4.paged([k], p["table"], 16, p["held"][0].shape[0])
+    p["q"] = q.bfloat16()
+    c = f4.cache(*p["held"])
+    got = call(c, p, single=new == 1, scale=100.0)
+    v = p["v"][0][1].repeat_interleave(2, 0)
+    assert c.status() == 0 and (got.cpu().double() - v).abs().max() <= 2.0 ** -8 * v.abs().max()
