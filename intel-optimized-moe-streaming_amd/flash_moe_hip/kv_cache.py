@@ -164,6 +164,7 @@ class PagedCache:
         self._index = k.device.index
         self._types = _types()
         self._empty, self._int32, self._int64, self._uint8 = torch.empty, torch.int32, torch.int64, torch.uint8
+        self._empty_like, self._format = torch.empty_like, torch.contiguous_format  # half of empty's host time
         codes = k.dtype in (torch.int8, torch.float4_e2m1fn_x2)
         self._q_types = (torch.float16, torch.bfloat16) if codes else (k.dtype,)
         self._read_type = torch.float32 if codes else k.dtype
@@ -334,7 +335,7 @@ class PagedCache:
 
     def _attend(self, handle, q, out, need, words):
         if out is None:
-            out = self._empty(q.shape, dtype=q.dtype, device=self.device)
+            out = self._empty_like(q, memory_format=self._format)
         if words[4] and words[6]:
             ws = self._empty(need, dtype=self._uint8, device=self.device) if need else None
             rc = self.lib.mqh_attend_words(_ATTEND_WORDS.pack(

@@ -98,8 +98,10 @@ class Rotary:
         self.device = self._turns.device
         self.lib = _lib.load()
         self._run, self._index = OnStream(self.device), self._turns.get_device()
-        self._types, self._empty, self._int32, self._float = _types(), torch.empty, torch.int32, (torch.float32,)
+        self._types, self._int32, self._float = _types(), torch.int32, (torch.float32,)
+        self._empty_like, self._format = torch.empty_like, torch.contiguous_format  # half of empty's host time
         self._flags = torch.zeros(64, dtype=torch.int32, device=self.device)
+        self._flag = self._flags.data_ptr()
 
     def apply(self, q, k, positions, *, q_weight=None, k_weight=None, eps: float = 1e-6, out=None, stream=None):
         """(q, k) turned: q [tokens, heads, head_dim], k [tokens, kv_heads, head_dim] of one
@@ -140,17 +142,16 @@ class Rotary:
 
     def _apply(self, handle, q, k, out, words):
         if out is None:
-            qo = self._empty(q.shape, dtype=q.dtype, device=self.device)
-            ko = self._empty(k.shape, dtype=k.dtype, device=self.device)
+            qo, ko = self._empty_like(q, memory_format=self._format), self._empty_like(k, memory_format=self._format)
         else:
             qo, ko = out
         if words[8]:
             rc = self.lib.mqh_rotary_words(_WORDS.pack(
-                *words, qo.data_ptr(), *qo.stride()[:2], ko.data_ptr(), *ko.stride()[:2], self._flags.data_ptr(), handle))
+                *words, qo.data_ptr(), *qo.stride()[:2], ko.data_ptr(), *ko.stride()[:2], self._flag, handle))
             if rc:
                 _lib.check(rc, "mqh_rotary")
         return qo, ko
 
     def status(self, stream=None) -> int:
         """Synchronizes; 0, or -4 (an output was not finite) since the last call."""
-        return int(self._run(stream, lambda handle: self.lib.mqh_status(self._flags.data_ptr(), handle)))
+        return int(self._run(stream, lambda handle: self.lib.mqh_status(self._flag, handle)))
