@@ -300,6 +300,18 @@ def test_strided_queries_and_tables_rows_of_no_sequence(qt):
         assert c.status() == 0
 
 
+@pytest.mark.parametrize("new", [[1, 1], [4, 2], [150, 70]], ids=str)
+def test_results_lie_row_by_row(new):
+    """Queries of other orders (heads outermost, one for all heads) give results in order."""
+    p = problem(new, [390, 133], 4, 2, 128, 16, torch.bfloat16, seed=8)
+    c = f4.cache(*p["held"])
+    table, lengths, starts = p["table"].cuda(), p["lengths"].cuda(), p["starts"].cuda()
+    for q in (p["q"].cuda().transpose(0, 1).contiguous().transpose(0, 1), p["q"][:, :1].cuda().expand(-1, 4, -1)):
+        got = c.attend(q, table, lengths, starts=starts)
+        assert got.is_contiguous() and torch.equal(got, c.attend(q.contiguous(), table, lengths, starts=starts))
+    assert c.status() == 0
+
+
 @pytest.mark.parametrize("single", [False, True])
 def test_bad_pages_and_lengths_are_reported(single):
     p = problem([1, 1], [300, 40], 4, 2, 64, 16, torch.float16)

@@ -125,6 +125,20 @@ def test_in_place_and_strided_outputs(layout):
     assert rot.status() == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_results_lie_row_by_row(dtype):
+    """Inputs of other orders (heads outermost, one row for all) give results in order."""
+    from flash_moe_hip.rotary import Rotary
+
+    rot, at = Rotary(64), places(37, 5).cuda()
+    q = torch.randn(6, 37, 64, generator=torch.Generator().manual_seed(2)).to(dtype).cuda().transpose(0, 1)
+    k = q[:1, :1].expand(37, 2, 64)
+    got = rot.apply(q, k, at)
+    want = rot.apply(q.contiguous(), k.contiguous(), at)
+    for g, w in zip(got, want):
+        assert g.is_contiguous() and torch.equal(g, w)
+
+
 def test_far_and_negative_positions():
     """Every 32-bit position, against angles of 60 digits; a turn back undoes a turn."""
     from flash_moe_hip.rotary import Rotary
