@@ -19,6 +19,13 @@ constexpr float ATTEND_GROWTH = 8.0f;   // how far (in log2) a row's probabiliti
 // of the largest, vs the largest product's scale.
 constexpr float ATTEND_ZERO_SCALE = 0x1p-80f;
 
+// Reference exponents past this are no longer a softmax's usual ones: FP32 holds them to
+// a sixteenth or worse, so that a score's exact product with the softmax scale may lie
+// whole units from the rounded one that became the reference (at 2^30 probabilities
+// passed FP16's range, at 2^36 a row's sum was 0), and the probabilities' own power of
+// two is lost in their difference.  Such a row's scores are taken relative to it first.
+constexpr float ATTEND_FAR = 0x1p20f;
+
 hipError_t launch_attend(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_token(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_join(const AttendParams& p, hipStream_t s);
@@ -83,6 +90,23 @@ struct MixMath<MIX_BF16> {
 template <class T>
 __device__ __forceinline__ T bits_as(uintx4 v) {
     return __builtin_bit_cast(T, v);
+}
+
+__device__ __forceinline__ bool exponent_far(float m) { return fabsf(m) > ATTEND_FAR && m != -INFINITY; }
+
+// what is subtracted in a row's exponentials: its reference exponent m without the
+// probabilities' power of two (0 where no key is seen yet, and where scores are relative
+// to m already)
+template <class M>
+__device__ __forceinline__ float exponent_base(float m) {
+    return (fabsf(m) > ATTEND_FAR ? 0.0f : m) - M::P_SHIFT;
+}
+
+// a score (of log2 x c) less m, both rounded products: the row's largest is 0 exactly
+__device__ __forceinline__ float score_from(float x, float c, float m) {
+#pragma clang fp contract(off)
+    const float t = x * c;
+    return t - m;
 }
 
 // four int8 codes as FP16: 1024 + (code + 128) is the half 0x6400 | (code + 128),

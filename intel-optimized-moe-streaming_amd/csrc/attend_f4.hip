@@ -216,7 +216,7 @@ __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
                 for (int e = 0; e < 4; ++e) part_mx[i] = fmaxf(part_mx[i], s[j][4 * i + e]);
         }
         float mx = fmaxf(fmaxf(part_mx[0], part_mx[1]), fmaxf(part_mx[2], part_mx[3])) * c;
-        if (__any(mx > m + ATTEND_GROWTH)) {
+        if (__any(mx - m > ATTEND_GROWTH)) {
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float mn = fmaxf(m, mx);
             const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -228,9 +228,17 @@ __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= a;
         }
+        if (__any(exponent_far(m))) {
+            const bool far = exponent_far(m);
+            const float back = 1.0f / c;   // (the exponential's argument multiplies by c again)
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[j][r] = far ? score_from(s[j][r], c, m) * back : s[j][r];
+        }
     };
     auto probabilities = [&]() {
-        const float ref = (m == -INFINITY ? 0.0f : m) - M::P_SHIFT;
+        const float ref = exponent_base<M>(m);
 #pragma unroll
         for (int t = 0; t < TB; ++t)
 #pragma unroll

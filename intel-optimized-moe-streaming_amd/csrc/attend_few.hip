@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 2 : 4) void k_attend_few(AttendPa
             }
             float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                              fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * c;
-            if (__any(mx > m + ATTEND_GROWTH)) {
+            if (__any(mx - m > ATTEND_GROWTH)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16));
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
                 const float mn = fmaxf(m, mx);
@@ -238,7 +238,15 @@ __global__ __launch_bounds__(256, DIM == 256 ? 2 : 4) void k_attend_few(AttendPa
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[i][d][e] *= a;
             }
-            const float ref = (m == -INFINITY ? 0.0f : m) - M::P_SHIFT;
+            if (__any(exponent_far(m))) {
+                const bool far = exponent_far(m);
+                const float back = 1.0f / c;   // (the exponential's argument multiplies by c again)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[j][e] = far ? score_from(s[j][e], c, m) * back : s[j][e];
+            }
+            const float ref = exponent_base<M>(m);
             vec8 pb;
 #pragma unroll
             for (int j = 0; j < 2; ++j)

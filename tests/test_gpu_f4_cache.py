@@ -519,3 +519,47 @@ def test_large_queries_and_scales(new):
     got = call(c, p, single=new == 1, scale=100.0)
     v = p["v"][0][1].repeat_interleave(2, 0)
     assert c.status() == 0 and (got.cpu().double() - v).abs().max() <= 2.0 ** -8 * v.abs().max()
+
+
+FAR = {   # new, length: a prompt from nothing, one token, drafts, chunks; keys of one workgroup and of several
+    "prompt": (9, 9), "single": (1, 300), "few": (5, 300), "many": (100, 300), "single split": (1, 9000),
+    "few split": (5, 9000), "many split": (100, 9000)}
+
+
+def means(v, chosen, new):
+    """What rows see whose chosen keys all have the same, by far the largest score: the mean of their values."""
+    some = chosen.double().view(-1, 1, 1)
+    total, n = (v * some).cumsum(0), some.cumsum(0).clamp(min=1)
+    return (total / n)[-new:], ((v.abs() * some).cumsum(0) / n)[-new:]
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kind", FAR)
+def test_scores_far_from_zero(kind, dim):
+    """Scores whose logarithms pass FP32's whole numbers, of either sign: the largest key alone, or equal ones alike.
+
+    Their probabilities are the same power of two or 0: a sum's rounding and the output's (near 2^20 one rounding of
+    FP16 for all of them)."""
+    new, length = FAR[kind]
+    g = torch.Generator().manual_seed(dim + length)
+    for qt, size in ((torch.bfloat16, 4e5), (torch.bfloat16, 3e8), (torch.bfloat16, 1e10), (torch.bfloat16, -1e12),
+                     (torch.bfloat16, 1e20), (torch.float16, 3e4), (torch.float16, -3e4)):
+        p = problem([new], [length], 4, 2, dim, 16, qt, seed=6)
+        factor = 1.0 if qt == torch.bfloat16 else 4096.0   # FP16 queries meet keys of 24,576
+        p["q"] = torch.zeros(new, 4, dim)
+        p["q"][..., 0] = size * (1 + torch.rand(new, 4, generator=g))
+        p["q"] = p["q"].to(qt)
+        i = torch.arange(length)
+        for name, high in (("one", i == 0), ("all", i >= 0), ("some", i % 3 == 0)):
+            k = torch.zeros(length, 2, dim)
+            k[..., 0] = torch.where(high, 6.0, 4.0 if name == "some" else 0.0).view(-1, 1) * factor * math.copysign(1, size)
+            if size < 0 and name == "all":
+                k = -k       # every score far below zero
+            p["held"][0], p["held"][2], _ = f4.paged([k], p["table"], 16, p["held"][0].shape[0])
+            c = f4.cache(*p["held"])
+            print(kind, dim, qt, size, name, flush=True)
+            got = call(c, p, single=new == 1, scale=0.3).cpu().double()
+            want, mass = (t.repeat_interleave(2, 1) for t in means(p["v"][0], high, new))
+            off = (2.0 ** -11 if abs(size) == 4e5 else 0.0) + (length + 64) * 2.0 ** -23
+            bound = ref.half_step(qt) * want.abs() + off * mass * 1.01 + (2.0 ** -25 if qt == torch.float16 else 0.0)
+            assert c.status() == 0 and ((got - want).abs() <= bound).all()
