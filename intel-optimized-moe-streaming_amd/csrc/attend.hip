@@ -334,7 +334,7 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
 #pragma unroll
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
             mx *= c;
-            if (__any(mx > m + ATTEND_GROWTH)) {
+            if (__any(mx - m > ATTEND_GROWTH)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
                 const float mn = fmaxf(m, mx);
                 const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -345,7 +345,15 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[d][r] *= a;
             }
-            const float ref = (m == -INFINITY ? 0.0f : m) - M::P_SHIFT;
+            if (__any(exponent_far(m))) {
+                const bool far = exponent_far(m);
+                const float back = 1.0f / c;   // (the exponential's argument multiplies by c again)
+#pragma unroll
+                for (int j = 0; j < KB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[j][r] = far ? score_from(s[j][r], c, m) * back : s[j][r];
+            }
+            const float ref = exponent_base<M>(m);
             vec8 probs[STEP / 16];
 #pragma unroll
             for (int t = 0; t < STEP / 16; ++t) {

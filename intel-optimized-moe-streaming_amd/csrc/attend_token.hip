@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
                 }
             }
             load_v(ra, rb);
-            if (__any(mx > m + ATTEND_GROWTH)) {
+            if (__any(mx - m > ATTEND_GROWTH)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16));
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
                 const float mn = fmaxf(m, mx);
@@ -225,7 +225,13 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[d][e] *= a;
             }
-            const float ref = (m == -INFINITY ? 0.0f : m) - M::P_SHIFT;
+            if (__any(exponent_far(m))) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[j][e] = exponent_far(m) ? s[j][e] - m : s[j][e];
+            }
+            const float ref = exponent_base<M>(m);
             vec8 pb;
 #pragma unroll
             for (int j = 0; j < 2; ++j)

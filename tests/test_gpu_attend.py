@@ -457,3 +457,82 @@ def test_a_seen_value_that_is_not_finite_is_not_lost_where_its_weight_underflows
     assert not got[..., 5].isfinite().any() and c.status() == -4
     others = [d for d in range(64) if d != 5]
     assert got[..., others].isfinite().all()
+
+
+FAR = {   # new, length: a prompt from nothing, one token, drafts; keys of one workgroup and of several
+    "prompt": (9, 9), "single": (1, 300), "many": (40, 300), "single split": (1, 9000), "many split": (40, 9000)}
+
+
+def with_keys(p, k, page, cache):
+    """The problem with other keys (of its one sequence)."""
+    kc, ks, _ = ref.paged([k], p["table"], page, p["cache"][0].shape[0], cache)
+    p["cache"][0] = kc.cuda()
+    p["cache"][2] = None if ks is None else ks.cuda()
+    return cache_of(p)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+@pytest.mark.parametrize("kind", FAR)
+def test_scores_far_from_zero(kind, cache, qt, dim):
+    """Scores whose logarithms pass FP32's whole numbers, of either sign: the largest key alone, or equal ones alike.
+
+    Their probabilities are the same power of two or 0: a sum's rounding and the output's (near 2^20 one rounding of the
+    16-bit type for all of them).  Equal ones only without codes: the values' scales are below a score's rounding."""
+    new, length = FAR[kind]
+    g = torch.Generator().manual_seed(dim + length)
+    sizes = (3e4, -3e4) if qt == torch.float16 else (4e5, 3e8, 1e10, -1e12, 1e20)
+    for size in sizes:
+        p = problem([new], [length], 4, 2, dim, 16, cache, qt, seed=6)
+        factor = 1.0 if qt == torch.bfloat16 else 4096.0
+        p["q"] = torch.zeros(new, 4, dim)
+        p["q"][..., 0] = size * (1 + torch.rand(new, 4, generator=g))
+        p["q"] = p["q"].to(qt)
+        v = p["cache"][1].cpu() if cache != torch.int8 else None
+        i = torch.arange(length)
+        page, off = p["table"][0, i // 16].long(), i % 16
+        if cache == torch.int8:
+            v = p["cache"][1].cpu()[page, :, off].double() * p["cache"][3].cpu()[page, :, off].double().unsqueeze(-1)
+        else:
+            v = v[page, :, off].double()
+        for name, high in (("one", i == 0), ("all", i >= 0), ("some", i % 3 == 0))[:1 if cache == torch.int8 else 3]:
+            k = torch.zeros(length, 2, dim)
+            k[..., 0] = torch.where(high, 6.0, 4.0 if name == "some" else 0.0).view(-1, 1) * factor * math.copysign(1, size)
+            if size < 0 and name == "all":
+                k = -k       # every score far below zero
+            c = with_keys(p, k, 16, cache)
+            print(kind, cache, qt, dim, size, name, flush=True)
+            got = call(c, p, single=new == 1, scale=0.3).cpu().double()
+            some = high.double().view(-1, 1, 1)
+            n = some.cumsum(0).clamp(min=1)
+            want = ((v * some).cumsum(0) / n)[-new:].repeat_interleave(2, 1)
+            mass = ((v.abs() * some).cumsum(0) / n)[-new:].repeat_interleave(2, 1)
+            # (codes: the exponential of a power of two, its reciprocal, a product, a quotient)
+            near = (ref.half_step(torch.bfloat16 if cache == torch.bfloat16 else torch.float16)
+                    if abs(size) == 4e5 or cache == torch.int8 else 0.0)
+            off_by = near + (length + 64) * 2.0 ** -23
+            bound = ref.half_step(qt) * want.abs() + off_by * mass * 1.01 + (2.0 ** -25 if qt == torch.float16 else 0.0)
+            assert c.status() == 0 and ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+@pytest.mark.parametrize("kind", ["single", "many", "single split", "many split"])
+def test_scores_just_above_far_ones(kind, cache, qt):
+    """Keys a few units above the first ones, where a score's last bit is as much: no probability leaves its type."""
+    new, length = FAR[kind]
+    for e in range(19, 30):
+        for more in (7.0, 8.0, 9.0, 16.0):
+            p = problem([new], [length], 4, 2, 64, 16, cache, qt, seed=6)
+            high = 2.0 ** 13 if qt == torch.float16 and cache == torch.float16 else 32.0
+            if 2.0 ** e / high > 65504 and qt == torch.float16:
+                continue
+            p["q"].zero_()
+            p["q"][..., 0], p["q"][..., 1] = 2.0 ** e / high, 1.0
+            k = torch.zeros(length, 2, 64)
+            k[..., 0] = high
+            k[130:, :, 1] = more
+            c = with_keys(p, k, 16, cache)
+            got = call(c, p, single=new == 1, scale=math.log(2))
+            most = max(float(t.abs().max()) for t in p["v"])
+            print(kind, cache, qt, e, more, flush=True)
+            assert c.status() == 0 and float(got.abs().max()) <= most * 1.01
