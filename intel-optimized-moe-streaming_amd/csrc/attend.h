@@ -26,6 +26,11 @@ constexpr float ATTEND_ZERO_SCALE = 0x1p-80f;
 // two is lost in their difference.  Such a row's scores are taken relative to it first.
 constexpr float ATTEND_FAR = 0x1p20f;
 
+// The reference exponent of a row that sees keys none of whose scores is above
+// -infinity (they are not FP32 numbers): not that of a row without keys, whose result is
+// zeros.  Its sum is 0, so that it becomes NaN where it is divided.
+constexpr float ATTEND_NO_SCORE = -0x1.fffffep127f;
+
 hipError_t launch_attend(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_token(const AttendParams& p, hipStream_t s);
 hipError_t launch_attend_join(const AttendParams& p, hipStream_t s);
@@ -107,6 +112,15 @@ __device__ __forceinline__ float score_from(float x, float c, float m) {
 #pragma clang fp contract(off)
     const float t = x * c;
     return t - m;
+}
+
+// a row's (or a part's) exponent as the division by its sum, and the join, take it
+__device__ __forceinline__ float exponent_seen(float m, float sum, bool sees) {
+    return m == -INFINITY && sum == 0.0f && sees ? ATTEND_NO_SCORE : m;
+}
+// what a row's sums are multiplied by: 0 for one without keys
+__device__ __forceinline__ float inverse_sum(float m, float sum) {
+    return m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
 }
 
 // four int8 codes as FP16: 1024 + (code + 128) is the half 0x6400 | (code + 128),

@@ -395,6 +395,7 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
     // ---- the rows out: this lane's channels 32 d + 8 r4 + 4 half + e
     if (!row_live) return;
     l += __shfl_xor(l, 32);   // (both halves of a row are live or neither)
+    m = exponent_seen(m, l, step0 < step1 && step0 * STEP <= seen);
     if (s_any_bad) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -423,7 +424,7 @@ __global__ __launch_bounds__(attend_threads(DIM), 2) void k_attend(AttendParams 
         }
         return;
     }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;   // a row that sees no key: zeros
+    const float inv = inverse_sum(m, l);
     uint16_t* out = (uint16_t*)p.out + out_row * DIM;
     bool finite = true;
 #pragma unroll
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendParams p) {
                 for (int e = 0; e < N; ++e) sum[e] = fmaf(w, v[i][e], sum[e]);
         }
     }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const float inv = inverse_sum(top, l);
     bool finite = true;
     uint16_t* out = (uint16_t*)p.out + row * DIM + lane * N;
     uint16_t y[N];

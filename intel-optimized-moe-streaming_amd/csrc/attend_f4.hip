@@ -353,6 +353,7 @@ __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
     if (!row_live) return;
     float sum = (l[0] + l[1]) + (l[2] + l[3]);
     sum += __shfl_xor(sum, 32);   // (both halves of a row are live or neither)
+    m = exponent_seen(m, sum, n > 0 && step0 * STEP <= seen);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
         if (s_nan[d] <= seen)
@@ -373,7 +374,7 @@ __global__ __launch_bounds__(F4_THREADS, 2) void k_attend_f4(AttendParams p) {
         }
         return;
     }
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;   // a row that sees no key: zeros
+    const float inv = inverse_sum(m, sum);
     uint16_t* out = (uint16_t*)p.out + ((int64_t)(seq.first + i0 + r_tok) * p.heads + r_head) * DIM;
     bool finite = true;
 #pragma unroll

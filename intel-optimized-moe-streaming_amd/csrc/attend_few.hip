@@ -331,6 +331,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 2 : 4) void k_attend_few(AttendPa
             for (int e = 0; e < 4; ++e) sum[e] = fmaf(a, v[e], sum[e]);
         }
         const int t = r / p.group, h = kvh * p.group + r - t * p.group;
+        top = exponent_seen(top, total, block0 < block1 && block0 * FEW_BLOCK <= first_pos + t);
         if (bad <= first_pos + t) sum = floatx4{NAN, NAN, NAN, NAN};
         if (w.splits > 1) {
             const int64_t at = ((int64_t)piece * p.kv_heads + kvh) * R + r;
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 2 : 4) void k_attend_few(AttendPa
             }
             continue;
         }
-        const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+        const float inv = inverse_sum(top, total);
         bool finite = true;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

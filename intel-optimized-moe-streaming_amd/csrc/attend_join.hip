@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void k_pieces_join(AttendParams p) {
     s_part[sub][tid % LANES] = sum;
     __syncthreads();
     if (tid >= LANES) return;
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const float inv = inverse_sum(top, l);
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(256) void k_pieces_join_many(AttendParams p) {
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const float inv = inverse_sum(top, l);
     float y[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) y[e] = sum[e] * inv;

@@ -290,6 +290,7 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
             for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, v[e], sum[e]);
         }
         const int64_t out_row = (int64_t)b * p.heads + kvh * p.group + r;
+        top = exponent_seen(top, total, block0 < block1);
         if (p.splits > 1) {
             const int64_t at = (int64_t)split * p.tokens * p.heads + out_row;
             *(floatx4*)(p.part_o + at * DIM + c) = sum;
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(256) void k_attend_token(AttendParams p) {
             }
             continue;
         }
-        const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+        const float inv = inverse_sum(top, total);
         bool finite = true;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

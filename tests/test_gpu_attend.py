@@ -536,3 +536,31 @@ def test_scores_just_above_far_ones(kind, cache, qt):
             most = max(float(t.abs().max()) for t in p["v"])
             print(kind, cache, qt, e, more, flush=True)
             assert c.status() == 0 and float(got.abs().max()) <= most * 1.01
+
+
+@pytest.mark.parametrize("kind", FAR)
+def test_scores_that_are_not_finite_are_reported(kind):
+    """Scores past FP32's range, before the softmax scale or with it, of either sign: no row of zeros, no silence."""
+    new, length = FAR[kind]
+    for cache, qt, size, key, scale in ((torch.bfloat16, torch.bfloat16, 1e30, 1e30, 0.3),
+                                        (torch.bfloat16, torch.bfloat16, 1e15, 1e15, 1e10),
+                                        (torch.float16, torch.float16, math.inf, 1.0, 0.3),
+                                        (torch.int8, torch.bfloat16, math.inf, 1.0, 0.3),
+                                        (torch.int8, torch.bfloat16, 1e30, 1e30, 0.3)):
+        p = problem([new], [length], 4, 2, 64, 16, cache, qt, seed=6)
+        k = torch.zeros(length, 2, 64)
+        k[..., 0] = key
+        c = with_keys(p, k, 16, cache)
+        p["q"][..., 0] = 0
+        clean = call(c, p, single=new == 1, scale=scale).cpu()
+        assert c.status() == 0
+        for sign in (-1, 1):
+            print(kind, cache, qt, size, scale, sign, flush=True)
+            q = p["q"].clone()
+            p["q"][-1, 1] = 0
+            p["q"][-1, 1, 0] = sign * size
+            got = call(c, p, single=new == 1, scale=scale).cpu()
+            assert got[-1, 1].isnan().all() and c.status() == -4
+            got[-1, 1] = clean[-1, 1]
+            assert torch.equal(got, clean)
+            p["q"] = q

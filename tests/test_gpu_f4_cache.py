@@ -563,3 +563,24 @@ def test_scores_far_from_zero(kind, dim):
             off = (2.0 ** -11 if abs(size) == 4e5 else 0.0) + (length + 64) * 2.0 ** -23
             bound = ref.half_step(qt) * want.abs() + off * mass * 1.01 + (2.0 ** -25 if qt == torch.float16 else 0.0)
             assert c.status() == 0 and ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("kind", FAR)
+def test_scores_that_are_not_finite_are_reported(kind):
+    """A query of infinities: no score is a number, none above the others."""
+    new, length = FAR[kind]
+    p = problem([new], [length], 4, 2, 64, 16, torch.bfloat16, seed=6)
+    k = torch.zeros(length, 2, 64)
+    k[..., 0] = 1.0
+    p["held"][0], p["held"][2], _ = f4.paged([k], p["table"], 16, p["held"][0].shape[0])
+    clean = call(f4.cache(*p["held"]), p, single=new == 1).cpu()
+    for size in (-math.inf, math.inf):
+        q = p["q"].clone()
+        p["q"][-1, 1] = 0
+        p["q"][-1, 1, 0] = size
+        c = f4.cache(*p["held"])
+        got = call(c, p, single=new == 1).cpu()
+        assert got[-1, 1].isnan().all() and c.status() == -4, size
+        got[-1, 1] = clean[-1, 1]
+        assert torch.equal(got, clean)
+        p["q"] = q
