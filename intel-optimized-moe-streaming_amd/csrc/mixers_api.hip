@@ -358,7 +358,7 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
     p.lengths = lengths; p.starts = starts; p.out = out;
     p.part_o = (float*)workspace;
     p.part_ml = (float*)((uint8_t*)workspace + align256((int64_t)a.splits * tokens * heads * dim * 4));
-    p.scale_log2 = scale * 1.44269504088896340736f;
+    p.scale_log2 = fminf(scale * 1.44269504088896340736f, 0x1.fffffep127f);   // (finite: a score of 0 stays 0)
     p.tokens = tokens; p.seqs = seqs; p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads;
     p.dim = dim; p.page_shift = page_shift_of(page_size); p.pages = (int)pages;
     p.tile_tokens = a.tile_tokens; p.tiles = a.tiles; p.splits = a.splits; p.flags = flags;

@@ -564,3 +564,15 @@ def test_scores_that_are_not_finite_are_reported(kind):
             got[-1, 1] = clean[-1, 1]
             assert torch.equal(got, clean)
             p["q"] = q
+
+
+@pytest.mark.parametrize("cache,qt", TYPES, ids=str)
+def test_the_largest_softmax_scales(cache, qt):
+    """A scale whose product with log2(e) is past FP32: scores of 0 stay 0."""
+    for new, length in FAR.values():
+        p = problem([new], [length], 4, 2, 64, 16, cache, qt, seed=6)
+        p["q"].zero_()
+        c = cache_of(p)
+        got = call(c, p, single=new == 1, scale=3e38)
+        assert c.status() == 0
+        check(got, p, 1.0, cache)
