@@ -153,6 +153,27 @@ typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 
+// sum over LANES neighbouring lanes (a power of two), in every one of them:
+// within 16 lanes by DPP, across them by the row and half swaps
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+#define MQH_DPP(x, ctrl) __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, 0xf, 0xf, true))
+    if constexpr (LANES >= 2) v += MQH_DPP(v, 0xb1);    // quad_perm 1,0,3,2
+    if constexpr (LANES >= 4) v += MQH_DPP(v, 0x4e);    // quad_perm 2,3,0,1
+    if constexpr (LANES >= 8) v += MQH_DPP(v, 0x141);   // row_half_mirror
+    if constexpr (LANES >= 16) v += MQH_DPP(v, 0x140);  // row_mirror
+#undef MQH_DPP
+    if constexpr (LANES >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (LANES >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
 // rows may start at any element (views of a wider tensor): loads and stores of
 // 8 or 16 bytes that ask for no more than the element's alignment
 template <class V>

@@ -3,7 +3,9 @@
 //   (a, b) -> (a cos - b sin, a sin + b cos),  angle = position * frequency,
 // pairs being halves (i, i + rotary / 2) or neighbours (2 i, 2 i + 1); before it,
 // where weights are given, the head's row goes through x / sqrt(mean x^2 + eps) * w.
-// All in FP32, rounded once.
+// All in FP32, rounded once; rows whose squares may pass FP32 take the norm of numbers
+// 2^96 times smaller, in a branch of their own (84 registers at FP32 where 79 were: heads
+// of 256 normed 34.5 -> 35.7 us; 16-bit rows are no slower).
 //
 // An angle far out needs more than FP32 (a million radians in FP32 are off by
 // 0.06).  Frequencies are held as turns a position in units of 2^-64, so that the
@@ -15,7 +17,7 @@
 // channels each; a workgroup takes the same few tokens of several heads, so that
 // the sines are computed once for all of them.  16,384 tokens of 32 + 8 heads of 128,
 // BF16: 70 us, 4.8 TB/s (a large copy reaches 4.7 to 4.8); 4,099 FP32 tokens of 16 + 2
-// heads of 256, normed: 34 us, 4.5 TB/s.  64 tokens: 5 us, two round trips and the sines.
+// heads of 256, normed: 35.5 us, 4.3 TB/s.  64 tokens: 5 us, two round trips and the sines.
 
 #include "mixers.h"
 
@@ -89,11 +91,24 @@ __global__ __launch_bounds__(256) void k_rotary(RotaryParams p) {
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sum = fmaf(x[n][i], x[n][i], sum);
+                sum = lane_sum<LANES>(sum);
+                float r = 1.0f / sqrtf(sum * (1.0f / DIM) + p.eps);
+                // rows whose squares may be past FP32: the same of numbers 2^96 times smaller
+                const bool past = !(sum <= 0x1p120f);
+                if (__any(past)) {
+                    constexpr float DOWN = 0x1p-96f;
+                    float part = 0.0f;
 #pragma unroll
-                for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor(sum, m);
-                const float r = 1.0f / sqrtf(sum * (1.0f / DIM) + p.eps);
+                    for (int i = 0; i < 8; ++i) part = fmaf(x[n][i] * DOWN, x[n][i] * DOWN, part);
+                    part = lane_sum<LANES>(part);
+                    part = 1.0f / sqrtf(part * (1.0f / DIM) + p.eps * DOWN * DOWN);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[n][i] *= r * w[c0 + i];
+                    for (int i = 0; i < 8; ++i) x[n][i] = past ? x[n][i] * part * DOWN : x[n][i];
+                    r = past ? 1.0f : r;
+                }
+                // (by the norm first: its product with a weight may lie where FP32 has no numbers)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[n][i] = x[n][i] * r * w[c0 + i];
             }
             float y[8];
 #pragma unroll

@@ -247,3 +247,33 @@ def test_refusals():
         with pytest.raises(ValueError, match=why):
             rot.apply(*args, **kw)
     assert rot.status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("dim,rotary,layout", [(64, 64, "half"), (128, 48, "interleaved"), (256, 64, "half")])
+def test_rows_whose_squares_are_past_fp32_are_normed(dim, rotary, layout, dtype):
+    """The norm of rows up to the type's largest numbers, beside rows of ones; weights that the norm's factor alone would
+    carry out of range."""
+    from flash_moe_hip.rotary import Rotary
+
+    rot = Rotary(dim, rotary, layout=layout)
+    at = places(7, 3)
+    g = torch.Generator().manual_seed(2)
+    for size, weight, eps in ((1e18, 1.0, 1e-6), (1e19, 1.0, 1e-6), (1e25, 1e-20, 1e-6), (5e37, 1.0, 1e30), (5e37, 1e-30, 1e-30),
+                              (1e-18, 1e30, 1e-30)):
+        w = weight * (1 + 0.1 * torch.randn(dim, generator=g))
+        q, k = rows(7, 5, dim, torch.float32, 8), rows(7, 3, dim, torch.float32, 9)
+        q[:, ::2], k[2:] = q[:, ::2] * size, k[2:] * size
+        q, k = q.to(dtype), k.to(dtype)
+        assert q.isfinite().all() and k.isfinite().all()
+        print(dim, rotary, layout, dtype, size, weight, eps, flush=True)
+        got = rot.apply(q, k, at.cuda(), q_weight=w.cuda(), k_weight=w.cuda(), eps=eps)
+        check(got[0], q, at, rot, w, eps)
+        check(got[1], k, at, rot, w, eps)
+        assert rot.status() == 0
+    q[3, 1, 5] = math.inf                # a row that is not finite is reported, the others stay
+    clean = got
+    got = rot.apply(q, k, at.cuda(), q_weight=w.cuda(), k_weight=w.cuda(), eps=eps)
+    assert rot.status() == -4 and got[0][3, 1].isnan().any() and torch.equal(got[1], clean[1])
+    got[0][3, 1] = clean[0][3, 1]
+    assert torch.equal(got[0], clean[0])
