@@ -411,12 +411,15 @@ int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int t
  * positions (int32; both 16-byte aligned), -1 past the last sequence.  A call that
  * cannot be served changes nothing and gives no rows (starts of 0, slots and
  * positions of -1): -10 latches if pages are lacking, -9 if grow is negative, a
- * sequence outgrows its columns, the new tokens are more than `rows`, or lengths,
- * count or pages are out of range.
+ * sequence outgrows its columns, the new tokens are more than `rows`, or lengths
+ * or count are out of range.  Numbers in `free_pages` and the table that are no
+ * pages are not such a call: it is carried out, the rows of such a page get the slot
+ * pages * page_size (past a cache of as many pages), and -9 latches.
  *
  * trim: sequence b keeps its first min(lengths[b], keep[b]) tokens, pages behind
  * them go back to the free ones (what the last extend took, to where it was).
- * keep[b] < 0, and lengths or count out of range, change nothing: -9.
+ * keep[b] < 0, and lengths or count out of range, change nothing: -9.  A number that
+ * is no page goes back like the others, and -9 latches.
  * Both return 0, -1 or -5. */
 int mqh_pages_extend(const int32_t* grow, int32_t* table, int cols, int32_t* lengths, int32_t* free_pages, int32_t* count,
                      int seqs, int pages, int page_size, int rows, int32_t* starts, int64_t* slots, int32_t* positions,

@@ -21,7 +21,9 @@
 // is 2); 24 prompts of 65,000 tokens in all in pages of 16: 7.1 and 6.2.
 //
 // A call whose arguments are out of range, or for which the pages do not suffice,
-// changes nothing and gives no rows.
+// changes nothing and gives no rows.  The numbers of the pages themselves are met only
+// where they are handed on: one that is none is reported there, and its rows get the slot
+// past a cache of p.pages.
 
 #include "mixers.h"
 
@@ -205,11 +207,15 @@ __global__ __launch_bounds__(PAGE_THREADS) void k_pages_trim(PageParams p) {
         for (int i = tid; i < p.seqs; i += PAGE_THREADS) p.lengths[i] = min(s.held[i], p.change[i]);
         if (tid == 0) *p.count = s.count + (int)s.moved;
     }
+    bool bad = false;
     for (int j = blockIdx.x * PAGE_THREADS + tid; j < (int)s.moved; j += gridDim.x * PAGE_THREADS) {
         const int b = owner(s.first, p.seqs, j);
         const int left = pages_of(s.held[b], p.page_shift) - (s.first[b + 1] - s.first[b]);
-        p.free_pages[s.count + s.moved - 1 - j] = p.table[(int64_t)b * p.cols + left + j - s.first[b]];
+        const int page = p.table[(int64_t)b * p.cols + left + j - s.first[b]];
+        bad |= (unsigned)page >= (unsigned)p.pages;
+        p.free_pages[s.count + s.moved - 1 - j] = page;
     }
+    if (bad) atomicOr(&p.flags[FLAG_BAD_ID], 1);
 }
 
 static size_t page_lds(const PageParams& p) { return (size_t)(3 * p.seqs + 2) * sizeof(int); }

@@ -100,7 +100,10 @@ class PageTable:
         A call that cannot be served changes nothing and gives no rows (starts of 0, slots
         and positions of -1): -10 latches where pages are lacking, -9 where a number is
         negative, a sequence outgrows its columns, or the new tokens are more than
-        `tokens`."""
+        `tokens`, or a length or the count is out of range.  Numbers in ``free`` and ``table``
+        that are no pages are found as they are handed out: the call is carried out, rows of
+        such a page get the slot pages * page_size, past a cache of as many pages (``write``
+        skips and reports it), and -9 latches."""
         check_index(new, (self.sequences,), self._int32, self._index, "new")
         if isinstance(tokens, bool) or not isinstance(tokens, int) or not 0 <= tokens <= 1 << 30:
             raise ValueError(f"tokens must be a whole number from 0 to 2^30, got {tokens!r}")
@@ -121,8 +124,9 @@ class PageTable:
     def trim(self, keep, *, stream=None):
         """Sequence b keeps its first min(lengths[b], keep[b]) tokens (int32 [sequences]);
         0 ends it.  Pages behind them become free: those that the last ``extend`` took
-        lie among the free ones where they were.  A negative number changes nothing and
-        latches -9."""
+        lie among the free ones where they were.  A negative number, or a length or count
+        out of range, changes nothing and latches -9; a number that is no page goes back
+        like the others and latches -9."""
         check_index(keep, (self.sequences,), self._int32, self._index, "keep")
         self._run(stream, self._trim, keep)
 

@@ -234,3 +234,33 @@ def test_refusals():
         t.extend(new, 3)
     t.lengths.data = torch.zeros(3, dtype=torch.int32, device="cuda")   # (another place: calls follow)
     assert extend(t, [1, 0, 0], 1)[1] == [0] and not kept.any() and t.lengths.tolist() == [1, 0, 0]
+
+
+def test_pages_that_are_none_are_reported_by_a_trim():
+    """A number in a sequence's columns that is no page goes back where it would, and is reported."""
+    from flash_moe_hip.page_table import PageTable
+
+    for tokens in (40, 40000):   # one workgroup's pages, several's
+        for bad in (-3, 10 ** 6, 4001):
+            t = PageTable.empty(2, 4000, 4001, 16)
+            t.extend(ints([tokens, 5]), tokens + 5)
+            t.table[0, 1] = bad
+            t.trim(ints([2 ** 31 - 1, 0]))
+            assert t.status() == 0                       # (no page of that sequence moved)
+            t.trim(ints([20, 0]))
+            assert t.status() == 0                       # (the column is still the sequence's)
+            t.trim(ints([1, 0]))
+            assert t.status() == -9 and t.lengths.tolist() == [1, 0] and int(t.count) == 4000
+            assert bad in t.free.tolist()
+
+
+def test_pages_that_are_none_lengths_grow_all_the_same():
+    """What a call does that hands out such a number: rows past the cache, the rest as ever."""
+    from flash_moe_hip.page_table import PageTable
+
+    t = PageTable.empty(2, 4, 8, 16)
+    t.free[6] = 99
+    starts, slots, positions = t.extend(ints([20, 3]), 24)
+    assert starts.tolist() == [0, 20, 23] and positions.tolist() == [*range(20), 0, 1, 2, -1]
+    assert slots.tolist() == [*range(16)] + [8 * 16] * 4 + [32, 33, 34, -1]
+    assert t.lengths.tolist() == [20, 3] and int(t.count) == 5 and t.table[0, 1] == 99 and t.status() == -9
