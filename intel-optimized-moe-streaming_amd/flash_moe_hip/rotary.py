@@ -50,6 +50,8 @@ def frequencies(rotary_dim: int, base: float = 10000.0, scaling=None):
         raise ValueError(f"a {kind} scaling has {known[kind]}, got {tuple(sc)}")
     if not all(0 < x < math.inf for x in sc.values()) or sc["factor"] < 1:
         raise ValueError(f"a scaling's numbers are positive and finite and its factor at least 1, got {sc}")
+    if not 2.0 ** -149 <= sc.get("amplitude", 1.0) < 2.0 ** 128 - 2.0 ** 103:
+        raise ValueError(f"amplitude must be an FP32 number, got {sc['amplitude']}")
     s = sc["factor"]
     if kind == "linear":
         return [x / s for x in f], 1.0

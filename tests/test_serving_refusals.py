@@ -179,3 +179,16 @@ def test_rotary_codes(lib):
     for bad in (dict(type=3), dict(type=5), dict(dim=96)):
         assert call(**bad) == -2, bad
     assert lib.mqh_rotary_words(None) == -1
+
+
+def test_rotary_amplitudes_fp32_cannot_hold():
+    """A factor that is 0 or infinite in FP32 is refused where it is stated, not at the first call."""
+    from flash_moe_hip.rotary import Rotary, frequencies
+
+    for a in (1e-46, 1e39, 1e300, 5e-324):
+        with pytest.raises(ValueError, match="amplitude"):
+            frequencies(64, 1e4, dict(kind="yarn", factor=2, original=100, amplitude=a))
+        with pytest.raises(ValueError, match="amplitude"):
+            Rotary(128, device="cpu", scaling=dict(kind="yarn", factor=2, original=100, amplitude=a))
+    for a in (1e-30, 1e30):
+        assert frequencies(64, 1e4, dict(kind="yarn", factor=2, original=100, amplitude=a))[1] == a
