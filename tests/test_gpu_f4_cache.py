@@ -584,3 +584,37 @@ def test_scores_that_are_not_finite_are_reported(kind):
         got[-1, 1] = clean[-1, 1]
         assert torch.equal(got, clean)
         p["q"] = q
+
+
+@pytest.mark.parametrize("new,lengths", [([2, 1], [300, 40]), ([2, 1], [3000, 4000]), ([150, 200], [300, 400]),
+                                         ([150, 200], [5000, 4000])])
+def test_bad_starts_are_reported_and_write_no_other_rows(new, lengths):
+    total = sum(new)
+    for starts in ([0, total + 5, 2], [-3, 1, total], [0, 1, total + 9], [total, 0, 1], [1, total, 0]):
+        print(new, lengths, starts, flush=True)
+        p = problem(new, lengths, 4, 2, 64, 16, torch.float16)
+        p["starts"] = torch.tensor(starts, dtype=torch.int32)
+        c = f4.cache(*p["held"])
+        room = torch.full((total + 16, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+        call(c, p, out=room[8:8 + total])
+        assert c.status() == -9
+        free = torch.ones(total + 16, dtype=torch.bool)
+        for a, b in zip(starts, starts[1:]):
+            a = min(max(a, 0), total)
+            free[8 + a:8 + max(min(b, total), a)] = False
+        assert (room.cpu()[free] == 7).all(), starts
+
+
+@pytest.mark.parametrize("kind", ["few", "many"])
+def test_bad_starts_of_many_sequences_are_reported(kind):
+    """Past 1,024 sequences, where every tile is one piece."""
+    seqs = 1100
+    new = [(i * 7) % 4 if kind == "few" else (i * 5) % 67 for i in range(seqs)]
+    p = problem(new, [n + (i * 37) % 90 for i, n in enumerate(new)], 8, 2, 64, 16, torch.bfloat16, seed=2)
+    c = f4.cache(*p["held"])
+    total = sum(new)
+    for starts in (torch.roll(p["starts"], 5), p["starts"] + 3, -p["starts"]):
+        p["starts"] = starts.contiguous()
+        room = torch.full((total + 16, 8, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        call(c, p, out=room[8:8 + total])
+        assert c.status() == -9 and (room[:8] == 7).all() and (room[8 + total:] == 7).all()
