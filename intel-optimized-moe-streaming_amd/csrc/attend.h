@@ -156,10 +156,9 @@ struct SeqRange {
     int first, count, length;   // query rows [first, first + count), cached tokens
 };
 
-// Sequence b's range with every bound forced into what the tensors hold; one
-// that had to be is a fault.
-__device__ __forceinline__ SeqRange sequence_range(const AttendParams& p, int b, bool report) {
-    SeqRange r;
+// Sequence b's range with every bound forced into what the tensors hold; whether one
+// had to be
+__device__ __forceinline__ bool clamped_range(const AttendParams& p, int b, SeqRange& r) {
     int s0 = b, s1 = b + 1;
     bool bad = false;
     if (p.starts) {
@@ -174,7 +173,13 @@ __device__ __forceinline__ SeqRange sequence_range(const AttendParams& p, int b,
     r.first = s0;
     r.count = s1 - s0;
     r.length = min(max(len, 0), most);
-    if (bad && report) atomicOr(&p.flags[FLAG_BAD_ID], 1);
+    return bad;
+}
+
+// the same where a bound that had to be forced is a fault
+__device__ __forceinline__ SeqRange sequence_range(const AttendParams& p, int b, bool report) {
+    SeqRange r;
+    if (clamped_range(p, b, r) && report) atomicOr(&p.flags[FLAG_BAD_ID], 1);
     return r;
 }
 

@@ -38,25 +38,6 @@ struct Piece {
     bool live;
 };
 
-// Sequence i's tokens and length with every bound forced into what the tensors hold.
-__device__ __forceinline__ bool piece_sequence(const AttendParams& p, int i, SeqRange& r) {
-    int s0 = i, s1 = i + 1;
-    bool bad = false;
-    if (p.starts) {
-        s0 = p.starts[i];
-        s1 = p.starts[i + 1];
-        bad = s0 < 0 || s1 < s0 || s1 > p.tokens;
-        s0 = min(max(s0, 0), p.tokens);
-        s1 = min(max(s1, s0), p.tokens);
-    }
-    const int len = p.lengths[i], most = p.table_cols << p.page_shift;
-    bad |= len < 0 || len > most;
-    r.first = s0;
-    r.count = s1 - s0;
-    r.length = min(max(len, 0), most);
-    return bad;
-}
-
 // The piece of a workgroup: blocks of `block` keys
 __device__ __forceinline__ Piece piece_found(const AttendParams& p, int piece, int block, bool report) {
     Piece r{};
@@ -74,13 +55,13 @@ __device__ __forceinline__ Piece piece_found(const AttendParams& p, int piece, i
             }
             if (report) {
                 bool bad = false;
-                for (int i = lane; i < p.seqs; i += 64) bad |= piece_sequence(p, i, r.seq);
+                for (int i = lane; i < p.seqs; i += 64) bad |= clamped_range(p, i, r.seq);
                 if (bad) atomicOr(&p.flags[FLAG_BAD_ID], 1);
             }
             if (b < 0) return r;
         }
         r.b = b = __builtin_amdgcn_readfirstlane(b);
-        if (piece_sequence(p, b, r.seq) && lane == 0) atomicOr(&p.flags[FLAG_BAD_ID], 1);
+        if (clamped_range(p, b, r.seq) && lane == 0) atomicOr(&p.flags[FLAG_BAD_ID], 1);
         r.tile = p.starts ? piece - (r.seq.first / p.tile_tokens + b) : 0;
         r.splits = 1;
         r.first = piece;
@@ -95,7 +76,7 @@ __device__ __forceinline__ Piece piece_found(const AttendParams& p, int piece, i
     bool bad = false;
     for (int i0 = 0; i0 < p.seqs; i0 += 64) {
         seq = SeqRange{};
-        if (i0 + lane < p.seqs) bad |= piece_sequence(p, i0 + lane, seq);
+        if (i0 + lane < p.seqs) bad |= clamped_range(p, i0 + lane, seq);
         const int tiles = (seq.count + p.tile_tokens - 1) / p.tile_tokens, blocks = (seq.length + block - 1) / block;
         total += (float)tiles * (float)blocks;
         all_tiles += tiles;
@@ -116,7 +97,7 @@ __device__ __forceinline__ Piece piece_found(const AttendParams& p, int piece, i
     for (int i0 = 0; i0 < p.seqs; i0 += 64) {
         if (p.seqs > 64) {   // (else the first loop's values are still here)
             seq = SeqRange{};
-            if (i0 + lane < p.seqs) piece_sequence(p, i0 + lane, seq);
+            if (i0 + lane < p.seqs) clamped_range(p, i0 + lane, seq);
         }
         const int tiles = (seq.count + p.tile_tokens - 1) / p.tile_tokens, blocks = (seq.length + block - 1) / block;
         const int splits = max((blocks + r.per - 1) / r.per, 1);
