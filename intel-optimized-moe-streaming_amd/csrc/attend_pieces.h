@@ -47,11 +47,16 @@ __device__ __forceinline__ Piece piece_found(const AttendParams& p, int piece, i
         // starts[b] / tile_tokens + b, which leaves room for its partial tiles
         int b = piece;
         if (p.starts) {
+            // the last sequence that begins at this piece or before it: of those between b
+            // and `past` every lane looks at one, evenly spaced
+            int past = p.seqs;
             b = -1;
-            for (int i0 = 0; i0 < p.seqs; i0 += 64) {
-                const int i = i0 + lane;
-                b += __builtin_popcountll(__ballot(
-                    i < p.seqs && min(max(p.starts[min(i, p.seqs - 1)], 0), p.tokens) / p.tile_tokens + i <= piece));
+            while (past - b > 1) {
+                const int step = (past - b - 1 + 63) >> 6, i = b + (lane + 1) * step;
+                const int begin = min(max(p.starts[min(i, p.seqs - 1)], 0), p.tokens);
+                const int here = __builtin_popcountll(__ballot(i < past && begin / p.tile_tokens + i <= piece));
+                past = min(b + (here + 1) * step, past);
+                b += here * step;
             }
             if (report) {
                 bool bad = false;

@@ -618,3 +618,28 @@ def test_bad_starts_of_many_sequences_are_reported(kind):
         room = torch.full((total + 16, 8, 64), 7.0, dtype=torch.bfloat16, device="cuda")
         call(c, p, out=room[8:8 + total])
         assert c.status() == -9 and (room[:8] == 7).all() and (room[8 + total:] == 7).all()
+
+
+@pytest.mark.parametrize("seqs,rows", [(1025, 3), (4096, 3), (4161, 40), (70001, 2)])
+def test_sequences_are_found_among_thousands(seqs, rows):
+    """Past 1,024 sequences a workgroup searches for its own: with none before it, none behind, runs without tokens."""
+    g = torch.Generator().manual_seed(seqs)
+    new = torch.randint(0, rows + 1, (seqs,), generator=g)
+    new[:70], new[200:333], new[-1] = 0, 0, rows
+    lengths = (new + torch.randint(0, 30, (seqs,), generator=g)).clamp(max=48)
+    p = problem([48], [48], 8, 2, 64, 16, torch.bfloat16, seed=2)   # (all sequences share three pages)
+    c = f4.cache(*p["held"])
+    starts = torch.nn.functional.pad(new.cumsum(0), (1, 0))
+    q = torch.randn(int(starts[-1]), 8, 64, generator=g).bfloat16()
+    got = c.attend(q.cuda(), p["table"].expand(seqs, -1).contiguous().cuda(), lengths.int().cuda(), starts.int().cuda()).cpu()
+    assert c.status() == 0
+    k, v = (t[0].float().repeat_interleave(4, 1) for t in (p["k"], p["v"]))
+    position = torch.repeat_interleave(lengths - new, new) + torch.arange(len(q)) - torch.repeat_interleave(starts[:-1], new)
+    worst = 0.0
+    for at in range(0, len(q), 8192):   # (FP32 here: the bounds of the checked rows are far above its errors)
+        s = torch.einsum("thd,khd->htk", q[at:at + 8192].float(), k) * 0.125
+        s = s.masked_fill(torch.arange(48).view(1, 1, -1) > position[at:at + 8192].view(1, -1, 1), -math.inf)
+        want = torch.einsum("htk,khd->thd", s.softmax(-1), v)
+        worst = max(worst, float((got[at:at + 8192].float() - want).abs().max()))
+    # BF16's half step of the result, FP16's of the probabilities and FP32's of the scores, twice, of the largest value
+    assert worst <= (2.0 ** -8 + 2.0 ** -11 + 2 * 2.0 ** -16) * float(v.abs().max())
