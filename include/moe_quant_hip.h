@@ -390,7 +390,9 @@ int64_t mqh_attend_f4_workspace_bytes(int tokens, int seqs, int single, int head
  * type (FP16 for Q8 and F4); BF16 queries of such a cache as FP16 times a power of two of
  * their row, exact down to 2^-17 of its largest.  Q8 scales are 0,
  * NaN or at least 2^-100, F4 scales 104 to 140 or 255 (or 0 with codes of 0), as
- * mqh_kv_write leaves them.  The workspace (256-byte aligned) is the call's own until
+ * mqh_kv_write leaves them; numbers of an F4 cache that FP16 cannot hold are lost in silence
+ * where scales are others.  A row that sees keys and none of whose scores is an FP32 number
+ * is NaN (-4).  The workspace (256-byte aligned) is the call's own until
  * its kernels have run.  Returns 0, -1, -2, -5 or -6. */
 int mqh_attend(const void* q, int64_t q_token, int64_t q_head, int q_type, int tokens, const int32_t* starts,
                int seqs, int heads, const void* kc, const void* vc, const void* ks, const void* vs, int cache_type,

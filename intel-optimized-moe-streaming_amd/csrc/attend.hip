@@ -33,10 +33,10 @@
 // that do not see the key) and put back per channel at the end for the rows that
 // see them.
 //
-// A prompt of 8,192 tokens, 32 heads of 128 over 8, BF16: 580 us, 950 TFLOP/s (a
+// A prompt of 8,192 tokens, 32 heads of 128 over 8, BF16: 587 us, 936 TFLOP/s (a
 // large library product reaches 1184), the matrix unit 46 % busy beside the
 // exponentials and the LDS loads; four ragged chunks of 2,048 tokens in all after up to
-// 16,384, 16 heads of 256 over 2, 8-bit cache: 571 us, 755 TFLOP/s, and 19 to join (the
+// 16,384, 16 heads of 256 over 2, 8-bit cache: 575 us, 750 TFLOP/s, and 18 to join (the
 // splits are equal in number, not in keys: the busiest CU goes 296 steps where an equal
 // share is 205).
 

@@ -13,11 +13,11 @@
 // probabilities and stores the keys of the steps to come.  Two buffers of keys and of
 // values in LDS suffice.
 //
-// A prompt of 8,192 tokens, 32 heads of 128 over 8: 504 us, 1090 TFLOP/s (a large library
+// A prompt of 8,192 tokens, 32 heads of 128 over 8: 508 us, 1080 TFLOP/s (a large library
 // product reaches 1170 to 1210), the matrix unit 52 % busy at 2.0 GHz: beside the
 // exponentials the chip lowers its clock (2.4 GHz with the products alone, 1.8 where the
 // stores into LDS are left out), so fewer cycles no longer are less time.  Four ragged
-// chunks of 2,048 tokens in all after up to 16,384, 16 heads of 256 over 2: 466 us, 925
+// chunks of 2,048 tokens in all after up to 16,384, 16 heads of 256 over 2: 460 us, 937
 // TFLOP/s, and 17 to join; there is no register for operands read ahead.
 //
 // Steps that some row does not see whole test positions and come last; blocks of

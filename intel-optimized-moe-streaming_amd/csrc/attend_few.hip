@@ -21,8 +21,8 @@
 // keys' pieces) nor the transposing reads (eight keys) meet in a bank (half of the bank
 // conflicts that there are with pieces exchanged for two and four keys).
 //
-// 64 ragged sequences of up to 8,192 keys, 32 heads of 128 over 8: 62 us, 4.6 TB/s, and
-// 4.7 to join.  One sequence of 32,771 keys, 16 heads of 256 over 2: 12.1 us and 4.0, a
+// 64 ragged sequences of up to 8,192 keys, 32 heads of 128 over 8: 63 us, 4.5 TB/s, and
+// 4.8 to join.  One sequence of 32,771 keys, 16 heads of 256 over 2: 12.2 us and 4.0, a
 // chain of round trips: 1.5 us from a workgroup's start to its piece, 2.4 to its first
 // keys, 3.3 for two blocks a wave, 1.9 to join the waves.
 

@@ -110,7 +110,9 @@ class PagedCache:
     Or 4-bit: k and v float4_e2m1fn_x2 [pages, kv_heads, page_size, head_dim / 2] (the
     even channel in a byte's low half), k_scale and v_scale float8_e8m0fnu [pages,
     kv_heads, page_size, head_dim / 32], one a 32 channels: those that ``write``
-    stores, 2^-23 to 2^13 or NaN (or 2^-127 with codes of 0, as ``empty`` has them).
+    stores, 2^-23 to 2^13 or NaN (or 2^-127 with codes of 0, as ``empty`` has them).  Of
+    blocks with other scales ``read`` gives the numbers, ``attend`` takes what FP16 holds
+    of them: what is lost so is not reported.
 
     A *slot* is page * page_size + offset; a sequence's page table lists its
     pages in order."""
@@ -290,7 +292,7 @@ class PagedCache:
         position; a row that sees none (a length below its queries) is zeros; rows
         of `out` that belong to no sequence are left as they were (without `out`
         they hold anything).  scale > 0
-        (default head_dim ** -0.5).  Returns out [tokens, heads, head_dim] of q's
+        (default head_dim ** -0.5); a row whose scores FP32 cannot hold is NaN.  Returns out [tokens, heads, head_dim] of q's
         type.  Probabilities are rounded once to the cache's 16-bit type (FP16 for
         codes), sums are FP32; BF16 queries of a cache of codes are multiplied as FP16
         times a power of two of their row (exact down to 2^-17 of its largest).  Page
