@@ -438,7 +438,7 @@ int mqh_pages_trim(const int32_t* keep, int32_t* table, int cols, int32_t* lengt
  * may be negative).  q_weight, k_weight [dim] FP32 or NULL: the row first goes
  * through x / sqrt(mean x^2 + eps) * weight.  FP32 throughout, rounded once; the
  * outputs may be the inputs themselves.  An output that its type cannot hold
- * latches -4.  Returns 0, -1, -2 or -5. */
+ * latches -4, but in rows of position -1, a batch's padding.  Returns 0, -1, -2 or -5. */
 int mqh_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, int type,
                const int32_t* positions, int tokens, int heads, int kv_heads, int dim, const uint64_t* turns, int rotary,
                int interleaved, float amplitude, const float* q_weight, const float* k_weight, float eps, void* q_out,

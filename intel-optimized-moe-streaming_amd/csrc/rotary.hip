@@ -13,6 +13,9 @@
 // are the angle to 2^-32 of a turn.  An eighth of a turn either way is left by the
 // quadrant, where Taylor's series to the ninth and tenth power are exact to FP32.
 //
+// Rows of position -1 are what a page table gives to a batch's padding: whatever they
+// hold (a layer before may have left them as they were) is turned, but not reported.
+//
 // Bound by memory: rows are read and written once.  dim / 8 lanes own a row, eight
 // channels each; a workgroup takes the same few tokens of several heads, so that
 // the sines are computed once for all of them.  16,384 tokens of 32 + 8 heads of 128,
@@ -122,7 +125,7 @@ __global__ __launch_bounds__(256) void k_rotary(RotaryParams p) {
             if (!live || h >= head1) continue;
             if (h < p.heads) store8<TYPE>(p.q_out, token * p.qo_token + (int64_t)h * p.qo_head + c0, x[n]);
             else store8<TYPE>(p.k_out, token * p.ko_token + (int64_t)(h - p.heads) * p.ko_head + c0, x[n]);
-            if (!finite) atomicOr(&p.flags[FLAG_NONFINITE], 1);
+            if (!finite && position != -1) atomicOr(&p.flags[FLAG_NONFINITE], 1);
         }
     }
 }

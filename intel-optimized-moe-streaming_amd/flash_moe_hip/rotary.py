@@ -110,10 +110,11 @@ class Rotary:
         type (FP32, FP16 or BF16; any token and head strides), positions int32 [tokens].
         Channels from rotary_dim on stay as they are.  q_weight, k_weight (FP32 [head_dim],
         either or both): the row first goes through x / sqrt(mean x^2 + eps) * weight.
-        FP32 inside, rounded once.  A negative position turns the other way (a row of
-        padding is turned by one position back).  out: two tensors like q and k to write
+        FP32 inside, rounded once.  A negative position turns the other way; rows of position
+        -1, a batch's padding, are turned by one position back and never reported.  out: two tensors like q and k to write
         to, of any token and head strides; q and k themselves turn them in place, other
-        overlaps are not allowed.  An output that its type cannot hold latches -4."""
+        overlaps are not allowed.  An output of another row that its type cannot hold latches
+        -4."""
         if q.dim() != 3 or k.dim() != 3:
             raise ValueError("q and k must be [tokens, heads, head_dim]")
         index, dim = self._index, self.head_dim

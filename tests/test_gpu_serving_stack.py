@@ -144,3 +144,21 @@ def test_a_step_without_free_pages_leaves_everything():
     assert layer.table.lengths.tolist() == [16, 16, 16, 0, 12]
     layer.run(rows(2, 3), ints([1, 1, 0, 0, 0]))
     layer.check()
+
+
+@pytest.mark.parametrize("cache_type", CACHES, ids=str)
+def test_rows_of_padding_hold_anything(cache_type):
+    """Rows behind the last sequence that a layer before left unwritten: real rows are the same, nothing is reported."""
+    clean, other = Layer(cache_type), Layer(cache_type)
+    for i, new in enumerate(([30, 0, 7, 200, 1], [1, 1, 1, 1, 1], [4, 0, 5, 3, 0])):
+        n = sum(new)
+        x, y = rows(n + 19, i), rows(n + 19, i)
+        y[n:n + 7], y[n + 7:] = float("nan"), float("inf")
+        want, got = clean.run(x, ints(new))[0], other.run(y, ints(new))[0]
+        assert torch.equal(got[:n], want[:n])
+        other.check()
+    # a row of a sequence is still reported
+    x = rows(5, 9)
+    x[2, 1, 70] = float("inf")
+    other.run(x, ints([1] * 5))
+    assert other.rotary.status() == -4 and other.table.status() == 0
